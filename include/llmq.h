@@ -324,6 +324,98 @@ llmq_status llmq_batch_generate(llmq_ctx *ctx, llmq_batch *b, const int *prompts
 llmq_status llmq_batch_generate_async(llmq_ctx *ctx, llmq_batch *b, const int *prompts_dev, int B, int n_prompt,
                                       int steps, int *ids_dev);
 
+/* ---- serving: a cache in pages, its eviction, rules on logits -------------- */
+/* No counterparts in the reference, whose caches are one contiguous block per
+ * sequence (kvcache.mojo) and whose sampler takes the head's logits as they
+ * are. All calls are asynchronous on the context's stream; their workspaces
+ * belong to the context, one per stream, and grow on first use (outside any
+ * stream capture).
+ *
+ * A paged cache: one pool of pages for all sequences, k and v
+ * [n_layer][n_pages][n_kv_head][page_size][head_dim] in int8
+ * (LLMQ_KV_QUANT8, with float32 scales ks, vs [n_layer][n_pages][n_kv_head]
+ * [page_size]), float32 or bfloat16. head_dim is 32, 64, 96 or 128; any page
+ * size. The caller's page table (device, [n_seqs] rows of table_cols
+ * page ids, table_stride apart) says where sequence b's position j is: slot j % page_size of page
+ * table[b][j / page_size]. An entry outside [0, n_pages) is no page. */
+typedef struct llmq_paged llmq_paged;
+llmq_status llmq_paged_create(llmq_ctx *ctx, int kind, int n_layer, int n_pages, int page_size, int n_kv_head,
+                              int head_dim, llmq_paged **out);
+llmq_status llmq_paged_free(llmq_paged *p);
+/* The pool's device buffers (ks, vs: NULL without scales). Any pointer may be
+ * NULL. */
+llmq_status llmq_paged_buffers(const llmq_paged *p, void **k, void **v, float **ks, float **vs);
+/* Stores n_rows tokens' keys and values into `layer`: row r (k_dev + r *
+ * k_stride floats, [n_kv_head][head_dim]) at position pos_dev[r] of sequence
+ * seq_dev[r] (seq_dev NULL: sequence r). int8 rows are quantized by
+ * QuantKV[8]'s rule (kvcache.mojo:319-331). A row with a negative position,
+ * or whose page the table does not have, is not stored. No two rows of a call
+ * may share a position. */
+llmq_status llmq_paged_store(llmq_ctx *ctx, llmq_paged *p, int layer, const float *k_dev, long long k_stride,
+                             const float *v_dev, long long v_stride, const int *seq_dev, const int *pos_dev,
+                             int n_rows, const int *table_dev, long long table_stride, int table_cols,
+                             int n_seqs);
+/* Attention of one new token per sequence: for sequence b and query head h
+ * (kv head h / (n_head / n_kv_head)), out = sum_j softmax_j(scale * q . k_j)
+ * v_j over the positions j < lens_dev[b] whose page exists; 0 where there is
+ * none. Lengths are cut to max_len, which sizes the launch, and to the table.
+ * q_dev, out_dev: [n_head][head_dim] rows, q_stride / out_stride floats
+ * apart. With weights_out_dev, the softmax weights are accumulated per kv
+ * head: weights_out[b][kv head][j] = weights[b][kv head][j] + the sum of its
+ * query heads' weights of position j, for j < max_len; rows weights_stride
+ * floats apart, weights_dev NULL for zeros and weights_out_dev ==
+ * weights_dev to add in place. The same inputs give the same bits. */
+llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, const float *q_dev, long long q_stride,
+                              float *out_dev, long long out_stride, int n_seqs, int n_head, const int *table_dev,
+                              long long table_stride, int table_cols, const int *lens_dev, int max_len, float scale,
+                              const float *weights_dev, float *weights_out_dev, long long weights_stride);
+/* Eviction by accumulated weight, for layers [layer0, layer0 + n_layers):
+ * every (layer, sequence, kv head) row keeps n = min(length, budget)
+ * positions. A row above the budget keeps its first `sinks`, its last
+ * `recent` and of the others those of the largest weights_dev[layer -
+ * layer0][b][kv head][j] (rows weights_stride floats apart; equal weights:
+ * the lower position; NaN below every number). The kept positions' keys and
+ * values move, in order, to positions 0 .. n - 1 of dst_table_dev
+ * [n_seqs][dst_cols], whose pages must differ from the source's (pages
+ * that sequences share are only read). kept_dev [n_layers][n_seqs]
+ * [n_kv_head][budget]: the positions, -1 past n. weights_out_dev (same row
+ * order, weights_out_stride floats apart): their weights, 0 past n.
+ * lens_out_dev[b] = n. Lengths are cut as in llmq_paged_attend. */
+llmq_status llmq_paged_evict(llmq_ctx *ctx, llmq_paged *p, int layer0, int n_layers, int n_seqs, const int *table_dev,
+                             long long table_stride, int table_cols, const int *lens_dev, int max_len,
+                             const float *weights_dev,
+                             long long weights_stride, int budget, int sinks, int recent, const int *dst_table_dev,
+                             long long dst_stride, int dst_cols, int *kept_dev, float *weights_out_dev, long long weights_out_stride,
+                             int *lens_out_dev);
+/* What may change logits between the head and llmq_sample; device pointers,
+ * NULL leaves a rule out. Per row r, in this order:
+ *  - the history ids[r][0 .. n_ids[r]) (rows ids_stride apart, n_ids cut to max_ids; its first
+ *    n_prompt[r] are the prompt, NULL: none; ids outside the vocabulary count
+ *    for nothing): a token that occurs in it has its logit divided by
+ *    repetition[r] if positive, else multiplied by it; a token that occurs c
+ *    > 0 times after the prompt loses frequency[r] * c, then presence[r];
+ *  - the bias: bias_values[i] is added to token bias_ids[i] for i in
+ *    [bias_offsets[r], bias_offsets[r + 1]); a row's ids ascend, equal ids
+ *    add up; offsets are cut to [0, n_bias];
+ *  - the mask: bit t % 32 of word mask[r][t / 32] is 1 where token t is
+ *    allowed, rows mask_stride words apart; other logits become -infinity. */
+typedef struct llmq_logit_rules {
+  const float *repetition, *presence, *frequency;
+  const int *ids, *n_ids, *n_prompt;
+  long long ids_stride;
+  int max_ids, n_bias;
+  const int *bias_offsets, *bias_ids;
+  const float *bias_values;
+  const uint32_t *mask;
+  long long mask_stride;
+} llmq_logit_rules;
+/* out[r][V] = the rules on logits[r][V] (rows n, strides in floats; out_dev
+ * may be logits_dev) and, if argmax_dev, argmax[r] = the first index of the
+ * largest one, -1 where none is above -infinity (NaN is not picked).
+ * V <= 2^24. The struct is on the host and read during the call. */
+llmq_status llmq_process_logits(llmq_ctx *ctx, const float *logits_dev, long long logits_stride, float *out_dev,
+                                long long out_stride, int n, int V, const llmq_logit_rules *rules, int *argmax_dev);
+
 #ifdef __cplusplus
 }
 #endif

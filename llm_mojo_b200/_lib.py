@@ -81,6 +81,13 @@ SIGNATURES = {
     "llmq_model_check": (I, [P, P]),
     "llmq_model_profile": (I, [P, P, I]),
     "llmq_model_profile_read": (I, [P, P, P, I, I]),
+    "llmq_paged_create": (I, [P, I, I, I, I, I, I, PP]),
+    "llmq_paged_free": (I, [P]),
+    "llmq_paged_buffers": (I, [P, PP, PP, PP, PP]),
+    "llmq_paged_store": (I, [P, P, I, P, LL, P, LL, P, P, I, P, LL, I, I]),
+    "llmq_paged_attend": (I, [P, P, I, P, LL, P, LL, I, I, P, LL, I, P, I, C.c_float, P, P, LL]),
+    "llmq_paged_evict": (I, [P, P, I, I, I, P, LL, I, P, I, P, LL, I, I, I, P, LL, I, P, P, LL, P]),
+    "llmq_process_logits": (I, [P, P, LL, P, LL, I, I, P, P]),
 }
 
 _lib = None

@@ -10,6 +10,7 @@ call fmaf() where the reference calls .fma.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -17,7 +18,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libllmq.so")
-SOURCES = ["llmq.cu", "quant_host.cpp"]
+SOURCES = ["llmq.cu", "serving.cu", "quant_host.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -28,28 +29,42 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def sources() -> list[str]:
-    out = []
-    for f in os.listdir(CSRC):
-        if f.endswith((".cu", ".cuh", ".cpp", ".h")):
-            out.append(os.path.join(CSRC, f))
-    out.append(os.path.join(os.path.dirname(HERE), "include", "llmq.h"))
-    return out
+def includes(path: str, seen: set[str] | None = None) -> set[str]:
+    """path and the project's files that it includes, directly or not."""
+    seen = set() if seen is None else seen
+    if path not in seen:
+        seen.add(path)
+        with open(path) as f:
+            for name in re.findall(r'^#include "(.+)"', f.read(), flags=re.M):
+                includes(os.path.normpath(os.path.join(os.path.dirname(path), name)), seen)
+    return seen
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(LIB):
-        return False
-    t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(s) <= t for s in sources())
+def stale(target: str, deps) -> bool:
+    return not os.path.exists(target) or any(os.path.getmtime(d) > os.path.getmtime(target) for d in deps)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and up_to_date():
+    """Compiles the sources that changed, side by side, and links them."""
+    srcs = [os.path.join(CSRC, s) for s in SOURCES]
+    if not force and not stale(LIB, set().union(*(includes(s) for s in srcs))):
         return LIB
-    cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-shared",
-           "-Xcompiler", "-fPIC,-ffp-contract=off,-O2", "-o", LIB]
-    cmd += [os.path.join(CSRC, s) for s in SOURCES]
+    obj_dir = os.path.join(HERE, "_build")
+    os.makedirs(obj_dir, exist_ok=True)
+    objs, running = [], []
+    for s in srcs:
+        o = os.path.join(obj_dir, os.path.basename(s) + ".o")
+        objs.append(o)
+        if force or stale(o, includes(s)):
+            cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-Xcompiler",
+                   "-fPIC,-ffp-contract=off,-O2", "-c", s, "-o", o]
+            if verbose:
+                print(" ".join(cmd))
+            running.append((cmd, subprocess.Popen(cmd, cwd=CSRC)))
+    for cmd, p in running:
+        if p.wait():
+            raise subprocess.CalledProcessError(p.returncode, cmd)
+    cmd = [nvcc(), *ARCH, "-shared", "-o", LIB, *objs]
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True, cwd=CSRC)

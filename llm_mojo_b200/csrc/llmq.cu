@@ -10,6 +10,7 @@
 #include "../../include/llmq.h"
 #include "attention.cuh"
 #include "batch.cuh"
+#include "context.cuh"
 #include "dense.cuh"
 #include "gemv_a16.cuh"
 #include "gemv_float.cuh"
@@ -21,30 +22,6 @@
 #include "tcl_gemm.cuh"
 
 using namespace llmq;
-
-struct llmq_ctx {
-  int device = 0;
-  int num_sms = 148;
-  cudaStream_t own = nullptr;
-  cudaStream_t stream = nullptr;
-  std::string err;
-  // scratch owned by the context (grown on demand)
-  void *scratch = nullptr;
-  size_t scratch_bytes = 0;
-  DecodeState *state = nullptr;  // device, for llmq_head_argmax
-  int dense_parts = 4;           // gemv's parts: the reference team of 4 threads (gpt2t.mojo:281 on 4 cores)
-  int prefill_kernel = LLMQ_PREFILL_AUTO;
-  long long wait_cycles = 4000000000LL;  // limit of a persistent kernel's or a row GEMV's device-side wait
-  int *tc_err = nullptr;         // device error code of the tcgen05 GEMM (a wait that gave up)
-  bool tc_used = false;          // a tcgen05 GEMM ran since the last check
-  // sampling scratch (device, grown on demand): sort keys, chunk candidates,
-  // the Rng state of llmq_generate_sampled
-  unsigned long long *samp_keys = nullptr;
-  unsigned long long *samp_cand = nullptr;
-  unsigned long long *samp_rng = nullptr;
-  int *samp_done = nullptr;  // set by topk_fast_kernel when it finished the draw
-  int samp_n = 0;
-};
 
 enum { WK_AFFINE = 0, WK_GGUF = 1, WK_DENSE = 2 };
 
@@ -127,24 +104,6 @@ struct llmq_model {
 };
 
 namespace {
-
-llmq_status fail(llmq_ctx *ctx, llmq_status st, const std::string &msg) {
-  if (ctx) ctx->err = msg;
-  return st;
-}
-
-#define CK(call)                                                                                 \
-  do {                                                                                           \
-    cudaError_t e_ = (call);                                                                     \
-    if (e_ != cudaSuccess)                                                                       \
-      return fail(ctx, LLMQ_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_));     \
-  } while (0)
-
-#define CKL()                                                                                    \
-  do {                                                                                           \
-    cudaError_t e_ = cudaGetLastError();                                                         \
-    if (e_ != cudaSuccess) return fail(ctx, LLMQ_ERR_CUDA, std::string("launch: ") + cudaGetErrorString(e_)); \
-  } while (0)
 
 constexpr int kMaxPrefillSmem = 225 * 1024;  // the several-token attention's staging limit
 constexpr int kBgemvSmem = 200 * 1024;       // the batched GEMV's shared memory limit
@@ -439,6 +398,10 @@ llmq_status llmq_destroy(llmq_ctx *ctx) {
   if (ctx->tc_err) cudaFree(ctx->tc_err);
   for (void *q : {(void *)ctx->samp_keys, (void *)ctx->samp_cand, (void *)ctx->samp_rng, (void *)ctx->samp_done})
     if (q) cudaFree(q);
+  for (auto &w : ctx->serve_ws) {
+    if (w.second.buf) cudaFree(w.second.buf);
+    if (w.second.tickets) cudaFree(w.second.tickets);
+  }
   if (ctx->own) cudaStreamDestroy(ctx->own);
   delete ctx;
   return LLMQ_OK;

@@ -1,0 +1,210 @@
+// paged.cuh -- a KV cache in pages and the attention of one new token per
+// sequence over it.
+//
+// The pool holds keys and values as [layer][page][kv_head][slot][dim] in
+// int8 (with a float32 scale per [layer][page][kv_head][slot], QuantKV[8]'s
+// rule), bfloat16 or float32. A page of one key head is contiguous, so a
+// tile of positions is one run of memory. Position j of sequence b is slot
+// j % page_size of page table[b][j / page_size]; an entry outside
+// [0, n_pages) is no page: nothing is stored there and its positions are
+// masked.
+#pragma once
+
+#include "common.cuh"
+
+namespace llmq {
+
+struct PagedView {
+  void *k, *v;
+  float *ks, *vs;  // int8 only
+  int kind, n_layer, n_pages, page_size, n_kv_head, head_dim;
+
+  // Index of (layer, page, kv head, slot) in rows of head_dim elements.
+  __host__ __device__ size_t row(int layer, int page, int h, int slot) const {
+    return (((size_t)layer * n_pages + page) * n_kv_head + h) * page_size + slot;
+  }
+};
+
+struct PageTable {
+  const int *ids;  // [n_seqs] rows of cols entries
+  long long stride;
+  int cols, n_seqs;
+
+  __device__ int page(int seq, int i) const { return ids[seq * stride + i]; }
+};
+
+// The element types of the pool.
+struct PgInt8 {
+  typedef int8_t T;
+  static constexpr bool kScaled = true;
+  static __device__ __forceinline__ float load(T x) { return (float)x; }
+};
+struct PgBf16 {
+  typedef uint16_t T;
+  static constexpr bool kScaled = false;
+  static __device__ __forceinline__ float load(T x) { return __uint_as_float((uint32_t)x << 16); }
+};
+struct PgF32 {
+  typedef float T;
+  static constexpr bool kScaled = false;
+  static __device__ __forceinline__ float load(T x) { return x; }
+};
+
+struct StoreArgs {
+  PagedView c;
+  PageTable t;
+  int layer, n_rows;
+  const float *k, *v;
+  long long k_stride, v_stride;
+  const int *seq, *pos;
+};
+
+// One warp per (row, kv head, key or value): lane L holds elements L + 32 j.
+// int8: s = max|x| / 127 (1 when 0), codes round(x * (1 / s)), half away
+// from zero, as QuantKV.quantize (kvcache.mojo:319-331).
+template <typename E>
+__global__ void __launch_bounds__(256) paged_store_kernel(StoreArgs a) {
+  const long long gw = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, nh = a.c.n_kv_head, D = a.c.head_dim;
+  const int which = gw & 1, h = (int)((gw >> 1) % nh);
+  const long long r = (gw >> 1) / nh;
+  if (r >= a.n_rows) return;
+  const int pos = a.pos[r], sq = a.seq ? a.seq[r] : (int)r;
+  if (pos < 0 || sq < 0 || sq >= a.t.n_seqs) return;
+  const int pi = pos / a.c.page_size;
+  if (pi >= a.t.cols) return;
+  const int page = a.t.page(sq, pi);
+  if (page < 0 || page >= a.c.n_pages) return;
+  const float *src = (which ? a.v + r * a.v_stride : a.k + r * a.k_stride) + (size_t)h * D;
+  const size_t row = a.c.row(a.layer, page, h, pos % a.c.page_size);
+  typename E::T *dst = (typename E::T *)(which ? a.c.v : a.c.k) + row * D;
+  float x[4];
+  float m = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    x[j] = lane + 32 * j < D ? src[lane + 32 * j] : 0.0f;
+    m = fmaxf(m, fabsf(x[j]));
+  }
+  if constexpr (E::kScaled) {
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float s = m / 127.0f;
+    if (s == 0.0f) s = 1.0f;
+    const float inv = 1.0f / s;
+    if (lane == 0) (which ? a.c.vs : a.c.ks)[row] = s;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (lane + 32 * j < D) dst[lane + 32 * j] = (int8_t)roundf(x[j] * inv);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (lane + 32 * j < D) {
+        if constexpr (sizeof(typename E::T) == 2)
+          dst[lane + 32 * j] = __bfloat16_as_ushort(__float2bfloat16_rn(x[j]));
+        else
+          dst[lane + 32 * j] = x[j];
+      }
+  }
+}
+
+struct AttendArgs {
+  PagedView c;
+  PageTable t;
+  int layer, n_head, max_len;
+  const float *q;
+  float *out;
+  long long q_stride, out_stride;
+  const int *lens;
+  float scale;
+  float *scores;  // [n_seqs][n_head][max_len], for the weights; else null
+  float *stat;    // [n_seqs][n_head][2]: the maximum score and the sum of exp(score - maximum)
+};
+
+// The positions sequence b attends to.
+__device__ __forceinline__ int paged_len(const AttendArgs &a, int b) {
+  const long long cap = (long long)a.t.cols * a.c.page_size;
+  return max(0, min(min(a.lens[b], a.max_len), (int)min(cap, (long long)INT_MAX)));
+}
+
+// out = sum_j softmax_j(scale q . k_j) v_j for one (sequence, head) per CTA,
+// in one pass: each warp takes every eighth position with its own running
+// maximum and sum, lanes hold dimensions lane + 32 i; the warps' states are
+// joined at the end. grid (n_seqs * n_head), 256 threads.
+template <typename E>
+__global__ void __launch_bounds__(256) paged_attend_kernel(AttendArgs a) {
+  __shared__ float sm[8], sl[8], so[8][128];
+  const int b = blockIdx.x / a.n_head, h = blockIdx.x % a.n_head, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int D = a.c.head_dim, kh = h / (a.n_head / a.c.n_kv_head), len = paged_len(a, b);
+  float q[4], acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    q[i] = lane + 32 * i < D ? a.q[(size_t)b * a.q_stride + (size_t)h * D + lane + 32 * i] : 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  for (int j = warp; j < len; j += 8) {
+    const int page = a.t.page(b, j / a.c.page_size);
+    float s = -INFINITY;
+    if (page >= 0 && page < a.c.n_pages) {
+      const size_t row = a.c.row(a.layer, page, kh, j % a.c.page_size);
+      const typename E::T *k = (const typename E::T *)a.c.k + row * D, *v = (const typename E::T *)a.c.v + row * D;
+      float d = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (lane + 32 * i < D) d = fmaf(q[i], E::load(k[lane + 32 * i]), d);
+      for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      if (E::kScaled) d *= a.c.ks[row];
+      s = d * a.scale;
+      const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(s - mn);
+      l = fmaf(l, c, p);
+      m = mn;
+      const float w = E::kScaled ? p * a.c.vs[row] : p;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (lane + 32 * i < D) acc[i] = fmaf(w, E::load(v[lane + 32 * i]), acc[i] * c);
+    }
+    if (a.scores && lane == 0) a.scores[((size_t)b * a.n_head + h) * a.max_len + j] = s;
+  }
+  if (lane == 0) {
+    sm[warp] = m;
+    sl[warp] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) so[warp][lane + 32 * i] = acc[i];
+  __syncthreads();
+  float M = -INFINITY, L = 0.0f;
+  for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w]);
+  float c[8];
+  for (int w = 0; w < 8; w++) {
+    c[w] = sm[w] == -INFINITY ? 0.0f : expf(sm[w] - M);
+    L = fmaf(sl[w], c[w], L);
+  }
+  if (a.stat && threadIdx.x == 0) {
+    a.stat[2 * blockIdx.x] = M;
+    a.stat[2 * blockIdx.x + 1] = L;
+  }
+  if (threadIdx.x < D) {
+    float o = 0.0f;
+    for (int w = 0; w < 8; w++) o = fmaf(so[w][threadIdx.x], c[w], o);
+    a.out[(size_t)b * a.out_stride + (size_t)h * D + threadIdx.x] = L == 0.0f ? 0.0f : o / L;
+  }
+}
+
+// weights_out[b][kv head][j] = weights[b][kv head][j] + sum over the kv
+// head's query heads of their softmax weight of position j (0 past the
+// length). grid (ceil(max_len / 256), n_seqs * n_kv_head), 256 threads.
+__global__ void __launch_bounds__(256) paged_weights_kernel(AttendArgs a, const float *win, float *wout,
+                                                            long long stride) {
+  const int j = blockIdx.x * 256 + threadIdx.x, G = a.n_head / a.c.n_kv_head;
+  if (j >= a.max_len) return;
+  for (int u = blockIdx.y; u < a.t.n_seqs * a.c.n_kv_head; u += gridDim.y) {
+    const int b = u / a.c.n_kv_head, kh = u % a.c.n_kv_head;
+    float w = win ? win[(size_t)u * stride + j] : 0.0f;
+    if (j < paged_len(a, b))
+      for (int g = 0; g < G; g++) {
+        const size_t r = (size_t)b * a.n_head + kh * G + g;
+        const float s = a.scores[r * a.max_len + j];
+        if (s != -INFINITY) w += expf(s - a.stat[2 * r]) / a.stat[2 * r + 1];
+      }
+    wout[(size_t)u * stride + j] = w;
+  }
+}
+
+}  // namespace llmq

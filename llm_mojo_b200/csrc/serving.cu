@@ -1,0 +1,249 @@
+// C entry points of the serving operators: the paged cache's store, attention
+// and eviction, and the rules on logits (include/llmq.h).
+#include <algorithm>
+#include <climits>
+
+#include "context.cuh"
+#include "evict.cuh"
+#include "logits.cuh"
+#include "paged.cuh"
+
+using namespace llmq;
+
+struct llmq_paged {
+  llmq_ctx *ctx;
+  PagedView v{};
+};
+
+namespace {
+
+// The stream's workspace with at least `bytes` of buffer and `tickets` zeroed
+// tickets. Growing waits for the stream, whose queued calls use the old one.
+llmq_status serve_ws(llmq_ctx *ctx, size_t bytes, size_t tickets, ServeWs **out) {
+  ServeWs &w = ctx->serve_ws[ctx->stream];
+  if (w.bytes < bytes || w.n_tickets < tickets) CK(cudaStreamSynchronize(ctx->stream));
+  if (w.bytes < bytes) {
+    if (w.buf) cudaFree(w.buf);
+    w.buf = nullptr;
+    w.bytes = 0;
+    if (cudaMalloc(&w.buf, bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(ctx, LLMQ_ERR_NOMEM, "serving workspace of " + std::to_string(bytes) + " bytes");
+    }
+    w.bytes = bytes;
+  }
+  if (w.n_tickets < tickets) {
+    if (w.tickets) cudaFree(w.tickets);
+    w.tickets = nullptr;
+    w.n_tickets = 0;
+    if (cudaMalloc(&w.tickets, tickets * sizeof(int)) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(ctx, LLMQ_ERR_NOMEM, "serving tickets");
+    }
+    CK(cudaMemsetAsync(w.tickets, 0, tickets * sizeof(int), ctx->stream));
+    w.n_tickets = tickets;
+  }
+  *out = &w;
+  return LLMQ_OK;
+}
+
+int elem_bytes(int kind) { return kind == LLMQ_KV_F32 ? 4 : kind == LLMQ_KV_BF16 ? 2 : 1; }
+
+// What store, attend and evict all check.
+llmq_status paged_check(llmq_ctx *ctx, const llmq_paged *p, int layer0, int n_layers, const int *table,
+                        long long table_stride, int table_cols, int n_seqs) {
+  if (!ctx || !p || !table) return fail(ctx, LLMQ_ERR_INVALID, "null argument");
+  if (p->ctx->device != ctx->device) return fail(ctx, LLMQ_ERR_INVALID, "the cache is on another device");
+  if (layer0 < 0 || n_layers <= 0 || layer0 > p->v.n_layer - n_layers) return fail(ctx, LLMQ_ERR_INVALID, "bad layer");
+  if (n_seqs <= 0 || table_cols <= 0 || table_stride < 0) return fail(ctx, LLMQ_ERR_INVALID, "bad page table shape");
+  return LLMQ_OK;
+}
+
+// Blocks of a one-dimensional grid, or 0 when there would be too many.
+unsigned grid1(long long n) { return n > 0 && n <= INT_MAX ? (unsigned)n : 0u; }
+
+}  // namespace
+
+extern "C" {
+
+llmq_status llmq_paged_create(llmq_ctx *ctx, int kind, int n_layer, int n_pages, int page_size, int n_kv_head,
+                              int head_dim, llmq_paged **out) {
+  if (!ctx || !out) return fail(ctx, LLMQ_ERR_INVALID, "null argument");
+  *out = nullptr;
+  if (kind != LLMQ_KV_QUANT8 && kind != LLMQ_KV_F32 && kind != LLMQ_KV_BF16)
+    return fail(ctx, LLMQ_ERR_UNSUPPORTED, "a paged cache holds int8, float32 or bfloat16");
+  if (n_layer <= 0 || n_pages <= 0 || page_size <= 0 || n_kv_head <= 0 || head_dim <= 0 || head_dim % 32 ||
+      head_dim > 128)
+    return fail(ctx, LLMQ_ERR_INVALID, "bad paged cache shape (head_dim: 32, 64, 96 or 128)");
+  CK(cudaSetDevice(ctx->device));
+  const double rows_d = (double)n_layer * n_pages * n_kv_head * page_size;
+  if (rows_d * head_dim * 4 > 4e12) return fail(ctx, LLMQ_ERR_NOMEM, "paged cache larger than any device");
+  const size_t rows = (size_t)n_layer * n_pages * n_kv_head * page_size;
+  const size_t bytes = rows * head_dim * elem_bytes(kind);
+  llmq_paged *p = new llmq_paged();
+  p->ctx = ctx;
+  p->v = PagedView{nullptr, nullptr, nullptr, nullptr, kind, n_layer, n_pages, page_size, n_kv_head, head_dim};
+  cudaError_t e = cudaMalloc(&p->v.k, bytes);
+  if (e == cudaSuccess) e = cudaMalloc(&p->v.v, bytes);
+  if (e == cudaSuccess && kind == LLMQ_KV_QUANT8) e = cudaMalloc(&p->v.ks, rows * 4);
+  if (e == cudaSuccess && kind == LLMQ_KV_QUANT8) e = cudaMalloc(&p->v.vs, rows * 4);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p->v.k, 0, bytes, ctx->stream);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p->v.v, 0, bytes, ctx->stream);
+  if (e == cudaSuccess && kind == LLMQ_KV_QUANT8) e = cudaMemsetAsync(p->v.ks, 0, rows * 4, ctx->stream);
+  if (e == cudaSuccess && kind == LLMQ_KV_QUANT8) e = cudaMemsetAsync(p->v.vs, 0, rows * 4, ctx->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+  if (e != cudaSuccess) {
+    llmq_paged_free(p);
+    cudaGetLastError();
+    return fail(ctx, e == cudaErrorMemoryAllocation ? LLMQ_ERR_NOMEM : LLMQ_ERR_CUDA,
+                std::string("paged cache: ") + cudaGetErrorString(e));
+  }
+  *out = p;
+  return LLMQ_OK;
+}
+
+llmq_status llmq_paged_free(llmq_paged *p) {
+  if (!p) return LLMQ_ERR_INVALID;
+  cudaSetDevice(p->ctx->device);
+  for (void *q : {p->v.k, p->v.v, (void *)p->v.ks, (void *)p->v.vs})
+    if (q) cudaFree(q);
+  delete p;
+  return LLMQ_OK;
+}
+
+llmq_status llmq_paged_buffers(const llmq_paged *p, void **k, void **v, float **ks, float **vs) {
+  if (!p) return LLMQ_ERR_INVALID;
+  if (k) *k = p->v.k;
+  if (v) *v = p->v.v;
+  if (ks) *ks = p->v.ks;
+  if (vs) *vs = p->v.vs;
+  return LLMQ_OK;
+}
+
+llmq_status llmq_paged_store(llmq_ctx *ctx, llmq_paged *p, int layer, const float *k, long long k_stride,
+                             const float *v, long long v_stride, const int *seq, const int *pos, int n_rows,
+                             const int *table, long long table_stride, int table_cols, int n_seqs) {
+  llmq_status st = paged_check(ctx, p, layer, 1, table, table_stride, table_cols, n_seqs);
+  if (st != LLMQ_OK) return st;
+  if (!k || !v || !pos) return fail(ctx, LLMQ_ERR_INVALID, "null argument");
+  if (n_rows <= 0 || (!seq && n_rows > n_seqs)) return fail(ctx, LLMQ_ERR_INVALID, "bad row count");
+  if (k_stride < 0 || v_stride < 0) return fail(ctx, LLMQ_ERR_INVALID, "negative stride");
+  CK(cudaSetDevice(ctx->device));
+  const unsigned g = grid1(((long long)n_rows * p->v.n_kv_head * 2 + 7) / 8);
+  if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
+  const StoreArgs a{p->v, PageTable{table, table_stride, table_cols, n_seqs}, layer, n_rows, k, v, k_stride, v_stride, seq, pos};
+  if (p->v.kind == LLMQ_KV_QUANT8)
+    paged_store_kernel<PgInt8><<<g, 256, 0, ctx->stream>>>(a);
+  else if (p->v.kind == LLMQ_KV_BF16)
+    paged_store_kernel<PgBf16><<<g, 256, 0, ctx->stream>>>(a);
+  else
+    paged_store_kernel<PgF32><<<g, 256, 0, ctx->stream>>>(a);
+  CKL();
+  return LLMQ_OK;
+}
+
+llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, const float *q, long long q_stride,
+                              float *out, long long out_stride, int n_seqs, int n_head, const int *table,
+                              long long table_stride, int table_cols, const int *lens, int max_len, float scale, const float *weights,
+                              float *weights_out, long long weights_stride) {
+  llmq_status st = paged_check(ctx, p, layer, 1, table, table_stride, table_cols, n_seqs);
+  if (st != LLMQ_OK) return st;
+  if (!q || !out || !lens) return fail(ctx, LLMQ_ERR_INVALID, "null argument");
+  if (n_head <= 0 || n_head % p->v.n_kv_head) return fail(ctx, LLMQ_ERR_INVALID, "n_head must be a multiple of n_kv_head");
+  const long long C = (long long)n_head * p->v.head_dim;
+  if (q_stride < 0 || (n_seqs > 1 && out_stride < C)) return fail(ctx, LLMQ_ERR_INVALID, "rows overlap");
+  if (max_len <= 0) return fail(ctx, LLMQ_ERR_INVALID, "bad max_len");
+  if (weights && !weights_out) return fail(ctx, LLMQ_ERR_INVALID, "weights without weights_out");
+  if (weights_out && weights_stride < max_len) return fail(ctx, LLMQ_ERR_INVALID, "weights_stride below max_len");
+  CK(cudaSetDevice(ctx->device));
+  AttendArgs a{p->v, PageTable{table, table_stride, table_cols, n_seqs}, layer, n_head, max_len, q, out, q_stride, out_stride,
+               lens, scale, nullptr, nullptr};
+  const unsigned g = grid1((long long)n_seqs * n_head);
+  if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many sequences for one call");
+  if (weights_out) {
+    ServeWs *ws;
+    const size_t rows = (size_t)n_seqs * n_head;
+    if ((st = serve_ws(ctx, rows * (max_len + 2) * 4, 0, &ws)) != LLMQ_OK) return st;
+    a.stat = (float *)ws->buf;
+    a.scores = a.stat + rows * 2;
+  }
+  if (p->v.kind == LLMQ_KV_QUANT8)
+    paged_attend_kernel<PgInt8><<<g, 256, 0, ctx->stream>>>(a);
+  else if (p->v.kind == LLMQ_KV_BF16)
+    paged_attend_kernel<PgBf16><<<g, 256, 0, ctx->stream>>>(a);
+  else
+    paged_attend_kernel<PgF32><<<g, 256, 0, ctx->stream>>>(a);
+  CKL();
+  if (weights_out) {
+    const dim3 wg((max_len + 255) / 256, (unsigned)std::min((long long)n_seqs * p->v.n_kv_head, 65535LL));
+    paged_weights_kernel<<<wg, 256, 0, ctx->stream>>>(a, weights, weights_out, weights_stride);
+    CKL();
+  }
+  return LLMQ_OK;
+}
+
+llmq_status llmq_paged_evict(llmq_ctx *ctx, llmq_paged *p, int layer0, int n_layers, int n_seqs, const int *table,
+                             long long table_stride, int table_cols, const int *lens, int max_len, const float *weights,
+                             long long weights_stride, int budget, int sinks, int recent, const int *dst_table,
+                             long long dst_stride, int dst_cols, int *kept, float *weights_out, long long weights_out_stride,
+                             int *lens_out) {
+  llmq_status st = paged_check(ctx, p, layer0, n_layers, table, table_stride, table_cols, n_seqs);
+  if (st != LLMQ_OK) return st;
+  if (!lens || !weights || !dst_table || !kept || !weights_out || !lens_out)
+    return fail(ctx, LLMQ_ERR_INVALID, "null argument");
+  if (max_len <= 0 || budget <= 0 || sinks < 0 || recent < 0 || sinks > budget || recent > budget - sinks)
+    return fail(ctx, LLMQ_ERR_INVALID, "sinks and recent must fit in a positive budget");
+  if (weights_stride < max_len || weights_out_stride < budget || weights_out_stride > INT_MAX)
+    return fail(ctx, LLMQ_ERR_INVALID, "bad weights stride");
+  if (dst_cols <= 0 || dst_stride < 0 || (long long)dst_cols * p->v.page_size < std::min(budget, max_len))
+    return fail(ctx, LLMQ_ERR_INVALID, "dst_table holds fewer positions than the budget");
+  CK(cudaSetDevice(ctx->device));
+  EvictArgs a{p->v, PageTable{table, table_stride, table_cols, n_seqs}, PageTable{dst_table, dst_stride, dst_cols, n_seqs}, layer0, n_layers,
+              max_len, budget, sinks, recent, lens, weights, weights_stride, kept, weights_out, weights_out_stride,
+              lens_out};
+  const long long rows = (long long)n_layers * n_seqs * p->v.n_kv_head;
+  const unsigned g = grid1(rows), gm = grid1((long long)((double)rows * budget < 1e14 ? (rows * budget + 7) / 8 : 0));
+  if (!g || !gm) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
+  evict_select_kernel<<<g, 1024, 0, ctx->stream>>>(a);
+  CKL();
+  evict_move_kernel<<<gm, 256, 0, ctx->stream>>>(a, p->v.head_dim * elem_bytes(p->v.kind));
+  CKL();
+  return LLMQ_OK;
+}
+
+llmq_status llmq_process_logits(llmq_ctx *ctx, const float *logits, long long logits_stride, float *out,
+                                long long out_stride, int n, int V, const llmq_logit_rules *rules, int *argmax) {
+  if (!ctx || !logits || !out || !rules) return fail(ctx, LLMQ_ERR_INVALID, "null argument");
+  if (n <= 0 || V <= 0 || V > (1 << 24)) return fail(ctx, LLMQ_ERR_INVALID, "bad logits shape");
+  if (n > 1 && (logits_stride < 0 || out_stride < V)) return fail(ctx, LLMQ_ERR_INVALID, "rows overlap");
+  const llmq_logit_rules &u = *rules;
+  if ((u.ids != nullptr) != (u.n_ids != nullptr) || (u.n_prompt && !u.ids) || (u.ids && (u.ids_stride < 0 || u.max_ids < 0)))
+    return fail(ctx, LLMQ_ERR_INVALID, "a history needs ids and n_ids");
+  if ((u.repetition || u.presence || u.frequency) && !u.ids)
+    return fail(ctx, LLMQ_ERR_INVALID, "a penalty needs a history");
+  if ((u.bias_offsets != nullptr) != (u.bias_ids != nullptr) || (u.bias_ids != nullptr) != (u.bias_values != nullptr))
+    return fail(ctx, LLMQ_ERR_INVALID, "a bias needs offsets, ids and values");
+  if ((u.bias_ids && u.n_bias < 0) || (u.mask && u.mask_stride < 0)) return fail(ctx, LLMQ_ERR_INVALID, "negative size");
+  CK(cudaSetDevice(ctx->device));
+  const int tiles = (V + kRuleTile - 1) / kRuleTile;
+  const unsigned g = grid1((long long)n * tiles);
+  if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
+  RuleArgs a{logits, out, logits_stride, out_stride, n, V, tiles, u.repetition, u.presence, u.frequency, u.ids,
+             u.n_ids, u.n_prompt, u.ids_stride, u.max_ids, u.n_bias, u.bias_offsets, u.bias_ids, u.bias_values, u.mask, u.mask_stride,
+             nullptr};
+  if (argmax) {
+    ServeWs *ws;
+    llmq_status st = serve_ws(ctx, (size_t)g * 8, 0, &ws);
+    if (st != LLMQ_OK) return st;
+    a.best = (unsigned long long *)ws->buf;
+  }
+  logit_rules_kernel<<<g, 256, 0, ctx->stream>>>(a);
+  CKL();
+  if (argmax) {
+    logit_argmax_kernel<<<n, 32, 0, ctx->stream>>>(a.best, tiles, argmax);
+    CKL();
+  }
+  return LLMQ_OK;
+}
+
+}  // extern "C"

@@ -16,6 +16,9 @@ import numpy as np
 from ._lib import check, lib
 
 
+CUDA_STREAM_LEGACY = 1  # cudaStreamLegacy
+
+
 def _ptr(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
 
@@ -28,12 +31,28 @@ class Context:
         check(lib().llmq_init(device, C.byref(h)))
         self.h = h
         self.device = device
+        self.stream = None  # the handle given to set_stream; None: the context's own
 
     def sync(self):
         check(lib().llmq_sync(self.h), self.h)
 
     def set_stream(self, stream_handle: int | None):
         check(lib().llmq_set_stream(self.h, C.c_void_p(stream_handle or 0)), self.h)
+        self.stream = stream_handle or None
+
+    def use_torch_stream(self):
+        """Issues the context's work on torch's current stream (the legacy
+        default stream, whose torch handle is 0, as cudaStreamLegacy)."""
+        import torch
+
+        self.set_stream(torch.cuda.current_stream(self.device).cuda_stream or CUDA_STREAM_LEGACY)
+
+    def on_torch_stream(self) -> bool:
+        """Whether the context's work is ordered with torch's current stream
+        because it is issued on it."""
+        import torch
+
+        return self.stream == (torch.cuda.current_stream(self.device).cuda_stream or CUDA_STREAM_LEGACY)
 
     def close(self):
         if self.h:
