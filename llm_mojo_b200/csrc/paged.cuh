@@ -114,10 +114,20 @@ struct AttendArgs {
   float *out;
   long long q_stride, out_stride;
   const int *lens;
-  float scale;
+  float scale2;   // scale * log2(e): scores are exponents of two
   float *scores;  // [n_seqs][n_head][max_len], for the weights; else null
-  float *stat;    // [n_seqs][n_head][2]: the maximum score and the sum of exp(score - maximum)
+  float *stat;    // [n_seqs][n_head][2]: the maximum score M and the sum of 2^(score - M)
+  // the split over positions (paged_mma.cuh)
+  int chunk, splits, head_chunks;
+  float *part;   // [unit][split][8][D + 2]: sums, then M and L of each head
+  int *tickets;  // [unit], zero between launches
 };
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // The positions sequence b attends to.
 __device__ __forceinline__ int paged_len(const AttendArgs &a, int b) {
@@ -151,8 +161,8 @@ __global__ void __launch_bounds__(256) paged_attend_kernel(AttendArgs a) {
         if (lane + 32 * i < D) d = fmaf(q[i], E::load(k[lane + 32 * i]), d);
       for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
       if (E::kScaled) d *= a.c.ks[row];
-      s = d * a.scale;
-      const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(s - mn);
+      s = d * a.scale2;
+      const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : exp2_approx(m - mn), p = exp2_approx(s - mn);
       l = fmaf(l, c, p);
       m = mn;
       const float w = E::kScaled ? p * a.c.vs[row] : p;
@@ -173,7 +183,7 @@ __global__ void __launch_bounds__(256) paged_attend_kernel(AttendArgs a) {
   for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w]);
   float c[8];
   for (int w = 0; w < 8; w++) {
-    c[w] = sm[w] == -INFINITY ? 0.0f : expf(sm[w] - M);
+    c[w] = sm[w] == -INFINITY ? 0.0f : exp2_approx(sm[w] - M);
     L = fmaf(sl[w], c[w], L);
   }
   if (a.stat && threadIdx.x == 0) {
@@ -189,11 +199,11 @@ __global__ void __launch_bounds__(256) paged_attend_kernel(AttendArgs a) {
 
 // weights_out[b][kv head][j] = weights[b][kv head][j] + sum over the kv
 // head's query heads of their softmax weight of position j (0 past the
-// length). grid (ceil(max_len / 256), n_seqs * n_kv_head), 256 threads.
-__global__ void __launch_bounds__(256) paged_weights_kernel(AttendArgs a, const float *win, float *wout,
+// length) for j < n. grid (ceil(n / 256), n_seqs * n_kv_head), 256 threads.
+__global__ void __launch_bounds__(256) paged_weights_kernel(AttendArgs a, int n, const float *win, float *wout,
                                                             long long stride) {
   const int j = blockIdx.x * 256 + threadIdx.x, G = a.n_head / a.c.n_kv_head;
-  if (j >= a.max_len) return;
+  if (j >= n) return;
   for (int u = blockIdx.y; u < a.t.n_seqs * a.c.n_kv_head; u += gridDim.y) {
     const int b = u / a.c.n_kv_head, kh = u % a.c.n_kv_head;
     float w = win ? win[(size_t)u * stride + j] : 0.0f;
@@ -201,7 +211,7 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(AttendArgs a, const 
       for (int g = 0; g < G; g++) {
         const size_t r = (size_t)b * a.n_head + kh * G + g;
         const float s = a.scores[r * a.max_len + j];
-        if (s != -INFINITY) w += expf(s - a.stat[2 * r]) / a.stat[2 * r + 1];
+        if (s != -INFINITY) w += exp2_approx(s - a.stat[2 * r]) / a.stat[2 * r + 1];
       }
     wout[(size_t)u * stride + j] = w;
   }

@@ -7,6 +7,7 @@
 #include "evict.cuh"
 #include "logits.cuh"
 #include "paged.cuh"
+#include "paged_mma.cuh"
 
 using namespace llmq;
 
@@ -59,6 +60,30 @@ llmq_status paged_check(llmq_ctx *ctx, const llmq_paged *p, int layer0, int n_la
   return LLMQ_OK;
 }
 
+// What the kernels of one cache shape have in common.
+template <bool I8, int D>
+cudaError_t launch_attend_mma(const AttendArgs &a, unsigned grid, cudaStream_t s) {
+  const bool fast = a.c.page_size % 16 == 0;
+  const size_t sm = pm_smem(a.chunk, D, fast);
+  if (fast)
+    paged_mma_kernel<I8, D, true><<<grid, kPmWarps * 32, sm, s>>>(a);
+  else
+    paged_mma_kernel<I8, D, false><<<grid, kPmWarps * 32, sm, s>>>(a);
+  return cudaGetLastError();
+}
+cudaError_t launch_attend(const AttendArgs &a, unsigned grid, cudaStream_t s) {
+  const bool i8 = a.c.kind == LLMQ_KV_QUANT8;
+  switch (a.c.head_dim) {
+    case 32: return i8 ? launch_attend_mma<true, 32>(a, grid, s) : launch_attend_mma<false, 32>(a, grid, s);
+    case 64: return i8 ? launch_attend_mma<true, 64>(a, grid, s) : launch_attend_mma<false, 64>(a, grid, s);
+    case 96: return i8 ? launch_attend_mma<true, 96>(a, grid, s) : launch_attend_mma<false, 96>(a, grid, s);
+    default: return i8 ? launch_attend_mma<true, 128>(a, grid, s) : launch_attend_mma<false, 128>(a, grid, s);
+  }
+}
+
+constexpr int kMaxSplits = 256;  // chunks of one unit that its last CTA joins
+constexpr int kMaxChunk = 4096;  // positions whose rows fit in shared memory without asking for more
+
 // Blocks of a one-dimensional grid, or 0 when there would be too many.
 unsigned grid1(long long n) { return n > 0 && n <= INT_MAX ? (unsigned)n : 0u; }
 
@@ -72,6 +97,8 @@ llmq_status llmq_paged_create(llmq_ctx *ctx, int kind, int n_layer, int n_pages,
   *out = nullptr;
   if (kind != LLMQ_KV_QUANT8 && kind != LLMQ_KV_F32 && kind != LLMQ_KV_BF16)
     return fail(ctx, LLMQ_ERR_UNSUPPORTED, "a paged cache holds int8, float32 or bfloat16");
+  if ((double)n_pages * n_kv_head * page_size > INT_MAX)
+    return fail(ctx, LLMQ_ERR_INVALID, "more than 2^31 - 1 rows in a layer");
   if (n_layer <= 0 || n_pages <= 0 || page_size <= 0 || n_kv_head <= 0 || head_dim <= 0 || head_dim % 32 ||
       head_dim > 128)
     return fail(ctx, LLMQ_ERR_INVALID, "bad paged cache shape (head_dim: 32, 64, 96 or 128)");
@@ -156,27 +183,52 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   if (weights && !weights_out) return fail(ctx, LLMQ_ERR_INVALID, "weights without weights_out");
   if (weights_out && weights_stride < max_len) return fail(ctx, LLMQ_ERR_INVALID, "weights_stride below max_len");
   CK(cudaSetDevice(ctx->device));
-  AttendArgs a{p->v, PageTable{table, table_stride, table_cols, n_seqs}, layer, n_head, max_len, q, out, q_stride, out_stride,
-               lens, scale, nullptr, nullptr};
-  const unsigned g = grid1((long long)n_seqs * n_head);
+  AttendArgs a{};
+  a.c = p->v;
+  a.t = PageTable{table, table_stride, table_cols, n_seqs};
+  a.layer = layer;
+  a.n_head = n_head;
+  a.max_len = (int)std::min((long long)max_len, (long long)table_cols * p->v.page_size);
+  a.q = q;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.lens = lens;
+  a.scale2 = (float)(scale * 1.4426950408889634);
+  const size_t rows = (size_t)n_seqs * n_head;
+  const int D = p->v.head_dim, G = n_head / p->v.n_kv_head;
+  const bool split = p->v.kind != LLMQ_KV_F32;
+  a.head_chunks = (G + 7) / 8;
+  const long long units = (long long)n_seqs * p->v.n_kv_head * a.head_chunks;
+  // chunks so that the longest call's CTAs fill the GPU about twice over
+  const long long want = std::max(1LL, (long long)ctx->num_sms * 8 / units);
+  long long chunk = std::max(64LL, (a.max_len + want - 1) / want);
+  chunk = std::max(chunk, (long long)(a.max_len + kMaxSplits - 1) / kMaxSplits);
+  a.chunk = (int)std::min((chunk + 63) / 64 * 64, (long long)kMaxChunk);
+  a.splits = (a.max_len + a.chunk - 1) / a.chunk;
+  const unsigned g = grid1(split ? units * a.splits : (long long)rows);
   if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many sequences for one call");
-  if (weights_out) {
+  const size_t parts = split && a.splits > 1 ? (size_t)units * a.splits * 8 * (D + 2) : 0;
+  if (weights_out || parts) {
     ServeWs *ws;
-    const size_t rows = (size_t)n_seqs * n_head;
-    if ((st = serve_ws(ctx, rows * (max_len + 2) * 4, 0, &ws)) != LLMQ_OK) return st;
-    a.stat = (float *)ws->buf;
-    a.scores = a.stat + rows * 2;
+    const size_t floats = parts + (weights_out ? rows * (a.max_len + 2) : 0);
+    if ((st = serve_ws(ctx, floats * 4, parts ? (size_t)units : 0, &ws)) != LLMQ_OK) return st;
+    a.part = (float *)ws->buf;
+    a.tickets = ws->tickets;
+    if (weights_out) {
+      a.stat = a.part + parts;
+      a.scores = a.stat + rows * 2;
+    }
   }
-  if (p->v.kind == LLMQ_KV_QUANT8)
-    paged_attend_kernel<PgInt8><<<g, 256, 0, ctx->stream>>>(a);
-  else if (p->v.kind == LLMQ_KV_BF16)
-    paged_attend_kernel<PgBf16><<<g, 256, 0, ctx->stream>>>(a);
-  else
+  if (split) {
+    CK(launch_attend(a, g, ctx->stream));
+  } else {
     paged_attend_kernel<PgF32><<<g, 256, 0, ctx->stream>>>(a);
-  CKL();
+    CKL();
+  }
   if (weights_out) {
     const dim3 wg((max_len + 255) / 256, (unsigned)std::min((long long)n_seqs * p->v.n_kv_head, 65535LL));
-    paged_weights_kernel<<<wg, 256, 0, ctx->stream>>>(a, weights, weights_out, weights_stride);
+    paged_weights_kernel<<<wg, 256, 0, ctx->stream>>>(a, max_len, weights, weights_out, weights_stride);
     CKL();
   }
   return LLMQ_OK;
