@@ -38,102 +38,185 @@ __device__ __forceinline__ unsigned evict_key(float x) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// One CTA per row: the need-th largest key of the middle positions by
-// bisection over its bits (32 counts of the row), then the kept positions by
-// prefix sums in order. grid (n_layers * n_seqs * n_kv_head), 1024 threads.
-__global__ void __launch_bounds__(1024) evict_select_kernel(EvictArgs a) {
-  __shared__ int part[33], part2[33];
+constexpr int kEvThreads = 1024;
+
+// A thread's four weights from position j on, j a multiple of 4 (positions
+// past the row's end: unspecified).
+template <bool VEC>
+__device__ __forceinline__ float4 evict_load(const float *w, int j, int len) {
+  if (j >= len) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (VEC && j + 3 < len) return *(const float4 *)(w + j);
+  return make_float4(w[j], j + 1 < len ? w[j + 1] : 0.0f, j + 2 < len ? w[j + 2] : 0.0f, j + 3 < len ? w[j + 3] : 0.0f);
+}
+
+// One CTA per row. The need-th largest key of the positions between the
+// sinks and the recent ones by radix select: digits of 11, 11 and 10 bits
+// from the top, each a histogram of the keys that agree with the digits
+// found so far, in shared memory (integer atomics: exact). Then the kept
+// positions in order: one prefix sum of (above the threshold or always kept,
+// equal to it) per 4096 positions, of the equal ones the first `ties`. The
+// row is read four times, but for the first time from L2.
+// grid (n_layers * n_seqs * n_kv_head), 1024 threads.
+template <bool VEC>
+__global__ void __launch_bounds__(kEvThreads) evict_select_kernel(EvictArgs a) {
+  __shared__ int hist[2048];
+  __shared__ int wsum[32];
+  __shared__ int s_bin, s_need;
   const int row = blockIdx.x, b = row / a.c.n_kv_head % a.src.n_seqs, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int len = evict_len(a, b), n = min(len, a.budget);
   const float *w = a.w + row * a.w_stride;
   float *wout = a.wout + row * a.wout_stride;
   int *kept = a.kept + (size_t)row * a.budget;
   if (row < a.src.n_seqs * a.c.n_kv_head && row % a.c.n_kv_head == 0 && tid == 0) a.lens_out[b] = n;
-  for (long long j = n + tid; j < a.wout_stride; j += 1024) wout[j] = 0.0f;
-  for (int j = n + tid; j < a.budget; j += 1024) kept[j] = -1;
+  for (long long j = n + tid; j < a.wout_stride; j += kEvThreads) wout[j] = 0.0f;
+  for (int j = n + tid; j < a.budget; j += kEvThreads) kept[j] = -1;
   if (len <= a.budget) {
-    for (int j = tid; j < len; j += 1024) {
+    for (int j = tid; j < len; j += kEvThreads) {
       kept[j] = j;
       wout[j] = w[j];
     }
     return;
   }
-  const int lo = a.sinks, hi = len - a.recent, need = a.budget - a.sinks - a.recent;
-  auto block_sum = [&](int v) {
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if (lane == 0) part[wid] = v;
-    __syncthreads();
-    int t = 0;
-    for (int i = 0; i < 32; i++) t += part[i];
-    return t;
-  };
-  // the largest key that at least `need` positions reach
-  unsigned thr = 0;
-  for (int bit = 31; bit >= 0; bit--) {
-    const unsigned t = thr | (1u << bit);
-    int c = 0;
-    for (int j = lo + tid; j < hi; j += 1024) c += evict_key(w[j]) >= t;
-    if (block_sum(c) >= need) thr = t;
+  const int lo = a.sinks, hi = len - a.recent;
+  int need = a.budget - a.sinks - a.recent;
+  unsigned thr = 0;  // the digits found, from the top
+  if (need > 0) {
+#pragma unroll 1
+    for (int pass = 0; pass < 3; pass++) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+      const unsigned known = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
+      for (int i = tid; i < 2048; i += kEvThreads) hist[i] = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (int j = tid * 4; j < hi; j += kEvThreads * 4) {
+        const float4 x = evict_load<VEC>(w, j, hi);
+        const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const unsigned key = evict_key(y[i]);
+          if (j + i >= lo && j + i < hi && ((key ^ thr) & known) == 0) atomicAdd(&hist[key >> shift & (bins - 1)], 1);
+        }
+      }
+      __syncthreads();
+      // the bin of the need-th largest: bins from the top, two a thread
+      const int b1 = 2047 - 2 * tid, h1 = hist[b1], h0 = hist[b1 - 1];
+      int s = h1 + h0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+      }
+      if (lane == 31) wsum[wid] = s;
+      __syncthreads();
+      if (wid == 0) {
+        int t = wsum[lane];
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, t, o);
+          if (lane >= o) t += u;
+        }
+        wsum[lane] = t;
+      }
+      __syncthreads();
+      s += wid ? wsum[wid - 1] : 0;  // keys in this thread's bins and above
+      const int above = s - h1 - h0;
+      if (above < need && need <= s) {
+        const bool first = need <= above + h1;
+        s_bin = first ? b1 : b1 - 1;
+        s_need = need - above - (first ? 0 : h1);
+      }
+      __syncthreads();
+      thr |= (unsigned)s_bin << shift;
+      need = s_need;
+      __syncthreads();
+    }
+  } else {
+    thr = 0xffffffffu;  // no key reaches it (NaN of any kind maps to 0)
   }
-  int above = 0;
-  for (int j = lo + tid; j < hi; j += 1024) above += evict_key(w[j]) > thr;
-  const int ties = need - block_sum(above);  // how many of the equal ones stay
+  // need is now how many of the keys equal to thr stay
   int base = 0, tbase = 0;
-  for (int j0 = 0; j0 < len; j0 += 1024) {
-    const int j = j0 + tid;
-    const bool mid = j >= lo && j < hi;
-    const unsigned key = mid ? evict_key(w[j]) : 0u;
-    const bool eq = mid && key == thr;
-    const unsigned eb = __ballot_sync(0xffffffffu, eq);
-    __syncthreads();
-    if (lane == 0) part2[wid] = __popc(eb);
-    __syncthreads();
-    int before = tbase + __popc(eb & ((1u << lane) - 1)), tall = 0;
-    for (int i = 0; i < 32; i++) {
-      if (i < wid) before += part2[i];
-      tall += part2[i];
+  for (int j0 = 0; j0 < len; j0 += kEvThreads * 4) {
+    const int j = j0 + tid * 4;
+    const float4 x = evict_load<VEC>(w, j, len);
+    const float y[4] = {x.x, x.y, x.z, x.w};
+    int flag[4], mine = 0;  // low half: kept whatever the ties; high half: equal to the threshold
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const unsigned key = evict_key(y[i]);
+      const bool mid = j + i >= lo && j + i < hi;
+      flag[i] = j + i >= len ? 0 : (!mid || key > thr) ? 1 : key == thr ? 0x10000 : 0;
+      mine += flag[i];
     }
-    const bool keep = j < len && (!mid || key > thr || (eq && before < ties));
-    const unsigned kb = __ballot_sync(0xffffffffu, keep);
-    if (lane == 0) part[wid] = __popc(kb);
+    int s = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += t;
+    }
+    if (lane == 31) wsum[wid] = s;
     __syncthreads();
-    int at = base + __popc(kb & ((1u << lane) - 1)), all = 0;
-    for (int i = 0; i < 32; i++) {
-      if (i < wid) at += part[i];
-      all += part[i];
+    int t = wsum[lane];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) t += u;
     }
-    if (keep) {
-      kept[at] = j;
-      wout[at] = w[j];
+    const int all = __shfl_sync(0xffffffffu, t, 31), before = wid ? __shfl_sync(0xffffffffu, t, max(wid - 1, 0)) : 0;
+    s += before - mine;
+    int sure = base + (s & 0xffff), ties = tbase + (s >> 16);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (flag[i] == 1 || (flag[i] && ties < need)) {
+        const int at = sure + min(ties, need);
+        kept[at] = j + i;
+        wout[at] = y[i];
+      }
+      sure += flag[i] & 1;
+      ties += flag[i] >> 16;
     }
-    base += all;
-    tbase += tall;
+    base += all & 0xffff;
+    tbase += all >> 16;
+    __syncthreads();
   }
 }
 
-// Moves the kept rows: one warp per (row, kept position), key and value (and
-// scales). grid over warps, 256 threads.
-__global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, int row_bytes) {
-  const long long gw = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const long long row = gw / a.budget;
-  const int j = (int)(gw % a.budget);
-  if (row >= (long long)a.n_layers * a.src.n_seqs * a.c.n_kv_head) return;
-  const int h = row % a.c.n_kv_head, b = (int)(row / a.c.n_kv_head % a.src.n_seqs);
-  const int layer = a.layer0 + (int)(row / a.c.n_kv_head / a.src.n_seqs);
-  const int s = a.kept[row * a.budget + j], ps = a.c.page_size;
-  if (s < 0 || j / ps >= a.dst.cols) return;
-  const int sp = a.src.page(b, s / ps), dp = a.dst.page(b, j / ps);
-  if (sp < 0 || sp >= a.c.n_pages || dp < 0 || dp >= a.c.n_pages) return;
-  const size_t from = a.c.row(layer, sp, h, s % ps), to = a.c.row(layer, dp, h, j % ps);
-  for (int i = lane * 4; i < row_bytes; i += 128) {
-    *(uint32_t *)((char *)a.c.k + to * row_bytes + i) = *(const uint32_t *)((const char *)a.c.k + from * row_bytes + i);
-    *(uint32_t *)((char *)a.c.v + to * row_bytes + i) = *(const uint32_t *)((const char *)a.c.v + from * row_bytes + i);
+constexpr int kEvPos = 64;  // kept positions that a CTA moves
+
+// Moves the kept rows, key and value (and scales), of kEvPos positions of one
+// row (layer, sequence, kv head) per CTA: 16-byte pieces, 8 in flight a
+// thread. NV: pieces of a cache row.
+template <int NV>
+__global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, int tiles) {
+  __shared__ long long from[kEvPos], to[kEvPos];  // rows; from < 0: nothing to move
+  const int row = blockIdx.x / tiles, j0 = blockIdx.x % tiles * kEvPos, tid = threadIdx.x;
+  const int h = row % a.c.n_kv_head, b = row / a.c.n_kv_head % a.src.n_seqs;
+  const int layer = a.layer0 + row / a.c.n_kv_head / a.src.n_seqs, ps = a.c.page_size;
+  if (tid < kEvPos) {
+    const int j = j0 + tid, s = j < a.budget ? a.kept[(size_t)row * a.budget + j] : -1;
+    from[tid] = -1;
+    if (s >= 0 && j / ps < a.dst.cols) {
+      const int sp = a.src.page(b, s / ps), dp = a.dst.page(b, j / ps);
+      if (sp >= 0 && sp < a.c.n_pages && dp >= 0 && dp < a.c.n_pages) {
+        from[tid] = (long long)a.c.row(layer, sp, h, s % ps);
+        to[tid] = (long long)a.c.row(layer, dp, h, j % ps);
+        if (a.c.ks) {
+          a.c.ks[to[tid]] = a.c.ks[from[tid]];
+          a.c.vs[to[tid]] = a.c.vs[from[tid]];
+        }
+      }
+    }
   }
-  if (a.c.ks && lane == 0) {
-    a.c.ks[to] = a.c.ks[from];
-    a.c.vs[to] = a.c.vs[from];
+  __syncthreads();
+  constexpr int kAll = 2 * kEvPos * NV, kU = 8;
+  for (int i0 = tid; i0 < kAll; i0 += 256 * kU) {
+    uint4 x[kU];
+#pragma unroll
+    for (int u = 0; u < kU; u++) {
+      const int i = i0 + u * 256, p = i / NV % kEvPos;
+      if (i < kAll && from[p] >= 0)
+        x[u] = __ldcs((const uint4 *)(i < kAll / 2 ? a.c.k : a.c.v) + from[p] * NV + i % NV);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; u++) {
+      const int i = i0 + u * 256, p = i / NV % kEvPos;
+      if (i < kAll && from[p] >= 0) ((uint4 *)(i < kAll / 2 ? a.c.k : a.c.v))[to[p] * NV + i % NV] = x[u];
+    }
   }
 }
 

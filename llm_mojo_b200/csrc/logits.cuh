@@ -6,8 +6,6 @@
 
 namespace llmq {
 
-constexpr int kRuleTile = 4096;  // logits of one CTA
-
 struct RuleArgs {
   const float *x;
   float *out;
@@ -21,9 +19,12 @@ struct RuleArgs {
   const float *bias_val;
   const uint32_t *mask;
   long long mask_stride;
-  unsigned long long *best;  // [n][tiles] (ordered value, ~id) of each tile's largest logit; or null
+  unsigned long long *best;  // [n][tiles] (ordered value, ~id) of each tile's largest logit
+  int *tickets;              // [n], zero between launches
+  int *argmax;               // or null
 };
 
+// (ordered value, ~id): the largest key is the first of the largest logits;
 // 0 for a logit that nothing picks (-inf and NaN).
 __device__ __forceinline__ unsigned long long rule_key(float x, int id) {
   if (!(x > -INFINITY)) return 0ull;
@@ -32,68 +33,223 @@ __device__ __forceinline__ unsigned long long rule_key(float x, int id) {
   return ((unsigned long long)asc << 32) | (unsigned)~id;
 }
 
-// One CTA per (row, tile): the history's counts of the tile's tokens in
-// shared memory (integer atomics: any order gives the same counts), then the
-// biases, then one pass over the logits.
-__global__ void __launch_bounds__(256) logit_rules_kernel(RuleArgs a) {
-  __shared__ unsigned cnt[kRuleTile];  // bit 31: seen; the rest: times in the answer
-  __shared__ float bias[kRuleTile];
-  __shared__ unsigned long long red[8];
-  const int r = blockIdx.x / a.tiles, t0 = blockIdx.x % a.tiles * kRuleTile, tid = threadIdx.x;
-  const int nv = min(kRuleTile, a.V - t0);
-  for (int i = tid; i < nv; i += 256) {
-    cnt[i] = 0;
-    bias[i] = 0.0f;
-  }
-  __syncthreads();
-  const int H = a.ids ? min(max(0, a.n_ids[r]), a.max_ids) : 0, P = a.n_prompt ? a.n_prompt[r] : 0;
-  for (int i = tid; i < H; i += 256) {
-    const int id = a.ids[r * a.ids_stride + i] - t0;
-    if (id >= 0 && id < nv) {
-      atomicOr(&cnt[id], 0x80000000u);
-      if (i >= P) atomicAdd(&cnt[id], 1u);
+// The tile of one item, as a thread holds it.
+template <int NG>
+struct RuleTile {
+  int r, t0, lo, hi;  // row; tokens: of the tile's first slot, of its first and past its last
+  unsigned mine;      // bits of the tokens 32 lane .. of the warp's run: allowed and in the row
+  float4 x[NG];
+};
+
+// Each warp has a run of 32 VPT logits, a lane VPT / 4 groups of four,
+// aligned to 16 bytes whatever the row's start (a row of odd length starts
+// anywhere: the first group may begin before it).
+template <int NTH, int VPT>
+__device__ __forceinline__ void rule_open(const RuleArgs &a, int item, RuleTile<VPT / 4> &w) {
+  const int lane = threadIdx.x & 31, tile = item % a.tiles;
+  w.r = item / a.tiles;
+  const float *xr = a.x + w.r * a.x_stride;
+  const int lead = (int)(((uintptr_t)xr >> 2) & 3);  // logits between the 16-byte boundary and the row's start
+  w.t0 = tile * NTH * VPT - lead;
+  w.lo = max(w.t0, 0);
+  w.hi = min(w.t0 + NTH * VPT, a.V);
+  w.mine = 0;
+  const int v = w.t0 + (threadIdx.x >> 5) * 32 * VPT + lane * 32;
+  if (lane < VPT && v < w.hi && v + 32 > w.lo) {
+    w.mine = 0xffffffffu;
+    if (a.mask) {
+      const uint32_t *m = a.mask + w.r * a.mask_stride;
+      const uint32_t w0 = m[max(v, 0) >> 5], w1 = m[min(v + 31, a.V - 1) >> 5];
+      w.mine = v >= 0 ? __funnelshift_r(w0, w1, v & 31) : w0 << -v;
     }
-  }
-  if (a.bias_off) {
-    const int b0 = max(a.bias_off[r], 0), b1 = min(a.bias_off[r + 1], a.n_bias);
-    for (int i = b0 + tid; i < b1; i += 256) {
-      const int id = a.bias_ids[i];
-      if (id < t0 || id >= t0 + nv || (i > b0 && a.bias_ids[i - 1] == id)) continue;
-      float s = a.bias_val[i];
-      for (int e = i + 1; e < b1 && a.bias_ids[e] == id; e++) s += a.bias_val[e];
-      bias[id - t0] = s;
-    }
-  }
-  __syncthreads();
-  const float rep = a.repetition ? a.repetition[r] : 1.0f, fr = a.frequency ? a.frequency[r] : 0.0f,
-              pr = a.presence ? a.presence[r] : 0.0f;
-  unsigned long long best = 0;
-  for (int i = tid; i < nv; i += 256) {
-    float x = a.x[r * a.x_stride + t0 + i];
-    const unsigned c = cnt[i], co = c & 0x7fffffffu;
-    if (c) x = x > 0.0f ? x / rep : x * rep;
-    if (co) x = (x - fr * (float)co) - pr;
-    if (a.bias_off) x += bias[i];
-    if (a.mask && !(a.mask[r * a.mask_stride + ((t0 + i) >> 5)] >> ((t0 + i) & 31) & 1u)) x = -INFINITY;
-    a.out[r * a.out_stride + t0 + i] = x;
-    best = max(best, rule_key(x, t0 + i));
-  }
-  if (!a.best) return;
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if ((tid & 31) == 0) red[tid >> 5] = best;
-  __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < 8; i++) best = max(best, red[i]);
-    a.best[blockIdx.x] = best;
+    if (v < 0) w.mine &= 0xffffffffu << -v;
+    if (v + 32 > w.hi) w.mine &= 0xffffffffu >> (v + 32 - w.hi);
   }
 }
 
-// argmax[r] from the tiles' best; -1 when no logit is above -inf. One warp a row.
-__global__ void logit_argmax_kernel(const unsigned long long *best, int tiles, int *argmax) {
-  unsigned long long k = 0;
-  for (int i = threadIdx.x; i < tiles; i += 32) k = max(k, best[(size_t)blockIdx.x * tiles + i]);
+// The allowed ones of group i's four tokens.
+__device__ __forceinline__ unsigned rule_keep(unsigned mine, int i) {
+  return __shfl_sync(0xffffffffu, mine, i * 4 + ((threadIdx.x & 31) >> 3)) >> (threadIdx.x & 7) * 4 & 15u;
+}
+
+template <int VPT>
+__device__ __forceinline__ void rule_load(const RuleArgs &a, RuleTile<VPT / 4> &w) {
+  const float *xr = a.x + w.r * a.x_stride;
+  const int v0 = w.t0 + (threadIdx.x >> 5) * 32 * VPT + (threadIdx.x & 31) * 4;
+#pragma unroll
+  for (int i = 0; i < VPT / 4; i++) {
+    const unsigned keep = rule_keep(w.mine, i);
+    const int v = v0 + i * 128;
+    w.x[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (!keep) continue;
+    if (v >= 0 && v + 3 < a.V) {
+      w.x[i] = *(const float4 *)(xr + v);
+    } else {
+      if (keep & 1u) w.x[i].x = xr[v];
+      if (keep & 2u) w.x[i].y = xr[v + 1];
+      if (keep & 4u) w.x[i].z = xr[v + 2];
+      if (keep & 8u) w.x[i].w = xr[v + 3];
+    }
+  }
+}
+
+// One CTA per (row, tile of NTH VPT logits). The mask is read first, a word
+// per lane, and only groups that it leaves something of are loaded: a
+// grammar's mask spares most of the read. While those loads are in flight
+// the history is counted in shared memory (integer atomics: any order gives
+// the same counts; each CTA reads the whole history and keeps its tile's
+// tokens) and the biases are laid out; then every rule is applied in
+// registers. The row's last CTA joins the tiles' argmax (exact in any
+// order).
+// Dynamic shared memory: 4 bytes per logit of the tile for a history, and
+// for a bias.
+template <int NTH, int VPT>
+__global__ void __launch_bounds__(NTH) logit_rules_kernel(RuleArgs a) {
+  constexpr int T = NTH * VPT, NG = VPT / 4;
+  extern __shared__ __align__(16) unsigned rsm[];
+  __shared__ unsigned long long red[NTH / 32];
+  unsigned *cnt = rsm;                             // bit 31: in the prompt; the rest: times in the answer
+  float *bias = (float *)(rsm + (a.ids ? T : 0));  // of the tile
+  const int tid = threadIdx.x, lane = tid & 31, r = blockIdx.x / a.tiles;
+  // the first quads of each thread's history, on their way with the logits
+  const int *ids = a.ids ? a.ids + r * a.ids_stride : nullptr;
+  const int first = (int)((4 - (((uintptr_t)ids >> 2) & 3)) & 3);  // ids before a 16-byte boundary
+  const int quads = a.ids ? max(a.max_ids - first, 0) / 4 : 0;
+  const int4 *q4 = (const int4 *)(ids + first);
+  int4 early[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+    if (tid + j * NTH < quads) early[j] = q4[tid + j * NTH];
+  RuleTile<NG> w;
+  rule_open<NTH, VPT>(a, blockIdx.x, w);
+  rule_load<VPT>(a, w);
+  if (a.ids || a.bias_off) {
+    uint4 *z = (uint4 *)rsm;
+    const int n = ((a.ids ? T : 0) + (a.bias_off ? T : 0)) / 4;
+#pragma unroll 4
+    for (int i = tid; i < n; i += NTH) z[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+  if (a.ids) {
+    const int H = min(max(0, a.n_ids[r]), a.max_ids), P = a.n_prompt ? a.n_prompt[r] : 0;
+    const unsigned span = w.hi - w.lo;
+    unsigned *c0 = cnt + (w.lo - w.t0);
+    auto count = [&](int i, int id) {
+      const unsigned k = (unsigned)id - (unsigned)w.lo;
+      if (k < span && i < H) {
+        if (i >= P)
+          atomicAdd(&c0[k], 1u);
+        else
+          atomicOr(&c0[k], 0x80000000u);
+      }
+    };
+    auto count4 = [&](int q, const int4 &v) {
+      const int i = first + 4 * q;
+      count(i, v.x);
+      count(i + 1, v.y);
+      count(i + 2, v.z);
+      count(i + 3, v.w);
+    };
+    if (tid < min(first, H)) count(tid, ids[tid]);
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      if (tid + j * NTH < quads) count4(tid + j * NTH, early[j]);
+    const int end = min(quads, (max(H - first, 0) + 3) / 4);
+    for (int q = tid + 2 * NTH; q < end; q += 4 * NTH) {
+      int4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = q4[min(q + j * NTH, end - 1)];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (q + j * NTH < end) count4(q + j * NTH, v[j]);
+    }
+    const int rest = first + quads * 4 + tid;
+    if (rest < H) count(rest, ids[rest]);
+  }
+  if (a.bias_off) {
+    const int b0 = max(a.bias_off[r], 0), b1 = min(a.bias_off[r + 1], a.n_bias);
+    for (int i = b0 + tid; i < b1; i += NTH) {
+      const int id = a.bias_ids[i];
+      if (id < w.lo || id >= w.hi || (i > b0 && a.bias_ids[i - 1] == id)) continue;
+      float s = a.bias_val[i];
+      for (int e = i + 1; e < b1 && a.bias_ids[e] == id; e++) s += a.bias_val[e];
+      bias[id - w.t0] = s;
+    }
+  }
+  if (a.ids || a.bias_off) __syncthreads();
+  const float rep = a.repetition ? a.repetition[r] : 1.0f, fr = a.frequency ? a.frequency[r] : 0.0f,
+              pr = a.presence ? a.presence[r] : 0.0f;
+  float *outr = a.out + r * a.out_stride;
+  const bool vec_out = (((uintptr_t)(outr + w.t0) >> 2) & 3) == 0;
+  const int at0 = (tid >> 5) * 32 * VPT + lane * 4;  // the thread's group i: at0 + 128 i
+  float bv = -INFINITY;                              // the thread's largest logit and its token, first of equals
+  int bt = -1;
+#pragma unroll
+  for (int i = 0; i < NG; i++) {
+    const unsigned keep = rule_keep(w.mine, i);
+    const int at = at0 + i * 128, v = w.t0 + at;
+    if (v >= w.hi || v + 3 < w.lo) continue;
+    float y[4] = {w.x[i].x, w.x[i].y, w.x[i].z, w.x[i].w};
+    if (a.ids) {
+      const uint4 c4 = *(const uint4 *)(cnt + at);
+      const unsigned c[4] = {c4.x, c4.y, c4.z, c4.w};
+      if (c4.x | c4.y | c4.z | c4.w) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const unsigned co = c[j] & 0x7fffffffu;
+          if (c[j]) y[j] = y[j] > 0.0f ? y[j] / rep : y[j] * rep;
+          if (co) y[j] = (y[j] - fr * (float)co) - pr;
+        }
+      }
+    }
+    if (a.bias_off) {
+      const float4 b4 = *(const float4 *)(bias + at);
+      y[0] += b4.x;
+      y[1] += b4.y;
+      y[2] += b4.z;
+      y[3] += b4.w;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (!(keep >> j & 1u)) y[j] = -INFINITY;
+      if (y[j] > bv) {
+        bv = y[j];
+        bt = v + j;
+      }
+    }
+    if (vec_out && v >= w.lo && v + 3 < w.hi) {
+      *(float4 *)(outr + v) = make_float4(y[0], y[1], y[2], y[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (v + j >= w.lo && v + j < w.hi) outr[v + j] = y[j];
+    }
+  }
+  if (!a.argmax) return;
+  unsigned long long k = rule_key(bv, bt);
   for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
-  if (threadIdx.x == 0) argmax[blockIdx.x] = k ? (int)~(unsigned)k : -1;
+  if (lane == 0) red[tid >> 5] = k;
+  __syncthreads();
+  if (tid >= 32) return;
+  k = lane < NTH / 32 ? red[lane] : 0ull;
+  for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+  int last = a.tiles == 1;
+  if (!last) {
+    unsigned long long *best = a.best + (size_t)r * a.tiles;
+    if (lane == 0) {
+      best[blockIdx.x % a.tiles] = k;
+      __threadfence();
+      last = atomicAdd(&a.tickets[r], 1) == a.tiles - 1;
+      if (last) __threadfence();
+    }
+    last = __shfl_sync(0xffffffffu, last, 0);
+    if (last) {
+      for (int i = lane; i < a.tiles; i += 32) k = max(k, __ldcg(best + i));
+      for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+      if (lane == 0) a.tickets[r] = 0;
+    }
+  }
+  if (last && lane == 0) a.argmax[r] = k ? (int)~(unsigned)k : -1;
 }
 
 }  // namespace llmq

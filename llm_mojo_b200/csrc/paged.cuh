@@ -59,50 +59,75 @@ struct StoreArgs {
   const int *seq, *pos;
 };
 
-// One warp per (row, kv head, key or value): lane L holds elements L + 32 j.
-// int8: s = max|x| / 127 (1 when 0), codes round(x * (1 / s)), half away
-// from zero, as QuantKV.quantize (kvcache.mojo:319-331).
+// Elements as the pool keeps them, four at a time.
 template <typename E>
-__global__ void __launch_bounds__(256) paged_store_kernel(StoreArgs a) {
-  const long long gw = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, nh = a.c.n_kv_head, D = a.c.head_dim;
-  const int which = gw & 1, h = (int)((gw >> 1) % nh);
-  const long long r = (gw >> 1) / nh;
-  if (r >= a.n_rows) return;
-  const int pos = a.pos[r], sq = a.seq ? a.seq[r] : (int)r;
-  if (pos < 0 || sq < 0 || sq >= a.t.n_seqs) return;
-  const int pi = pos / a.c.page_size;
-  if (pi >= a.t.cols) return;
-  const int page = a.t.page(sq, pi);
-  if (page < 0 || page >= a.c.n_pages) return;
-  const float *src = (which ? a.v + r * a.v_stride : a.k + r * a.k_stride) + (size_t)h * D;
-  const size_t row = a.c.row(a.layer, page, h, pos % a.c.page_size);
-  typename E::T *dst = (typename E::T *)(which ? a.c.v : a.c.k) + row * D;
-  float x[4];
-  float m = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    x[j] = lane + 32 * j < D ? src[lane + 32 * j] : 0.0f;
-    m = fmaxf(m, fabsf(x[j]));
-  }
+__device__ __forceinline__ void pack_store(typename E::T *dst, const float4 &x, float inv) {
   if constexpr (E::kScaled) {
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float s = m / 127.0f;
-    if (s == 0.0f) s = 1.0f;
-    const float inv = 1.0f / s;
-    if (lane == 0) (which ? a.c.vs : a.c.ks)[row] = s;
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (lane + 32 * j < D) dst[lane + 32 * j] = (int8_t)roundf(x[j] * inv);
+    const int c0 = (int)roundf(x.x * inv) & 255, c1 = (int)roundf(x.y * inv) & 255, c2 = (int)roundf(x.z * inv) & 255,
+              c3 = (int)roundf(x.w * inv) & 255;
+    *(unsigned *)dst = c0 | c1 << 8 | c2 << 16 | c3 << 24;
+  } else if constexpr (sizeof(typename E::T) == 2) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+    *(uint2 *)dst = make_uint2(*(const unsigned *)&a, *(const unsigned *)&b);
   } else {
+    *(float4 *)dst = x;
+  }
+}
+
+// A group of LG lanes (D / 4, and 8 of 32 idle at D = 96) has a head's key
+// or value, four elements a lane, kStoreItems of them in flight: memory is
+// all that this kernel does. int8: s = max|x| / 127 (1 when 0), codes round(x
+// * (1 / s)), half away from zero, as QuantKV.quantize (kvcache.mojo:319-331).
+// VEC: 16-byte loads (aligned rows). grid of 256 threads over the items, (row,
+// kv head, key or value) in that order.
+constexpr int kStoreItems = 4;
+
+template <typename E, int D, bool VEC>
+__global__ void __launch_bounds__(256) paged_store_kernel(StoreArgs a) {
+  constexpr int LG = D == 96 ? 32 : D / 4, kPer = 256 / LG;
+  const int lane = threadIdx.x % LG, nh = a.c.n_kv_head;
+  const long long i0 = ((long long)blockIdx.x * kPer + threadIdx.x / LG) * kStoreItems;
+  const long long items = (long long)a.n_rows * nh * 2;
+  float4 x[kStoreItems];
+  long long row[kStoreItems];
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (lane + 32 * j < D) {
-        if constexpr (sizeof(typename E::T) == 2)
-          dst[lane + 32 * j] = __bfloat16_as_ushort(__float2bfloat16_rn(x[j]));
-        else
-          dst[lane + 32 * j] = x[j];
-      }
+  for (int j = 0; j < kStoreItems; j++) {
+    const long long i = i0 + j;
+    row[j] = -1;
+    x[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (i >= items) continue;
+    const int which = i & 1;
+    const unsigned q = (unsigned)(i >> 1), r = q / (unsigned)nh, h = q - r * nh;
+    const float *src = (which ? a.v + r * a.v_stride : a.k + r * a.k_stride) + h * D + lane * 4;
+    if (lane * 4 < D) {
+      if constexpr (VEC)
+        x[j] = __ldcs((const float4 *)src);
+      else
+        x[j] = make_float4(src[0], src[1], src[2], src[3]);
+    }
+    const int pos = a.pos[r], sq = a.seq ? a.seq[r] : (int)r;
+    if (pos < 0 || sq < 0 || sq >= a.t.n_seqs) continue;
+    const int pi = pos / a.c.page_size;
+    if (pi >= a.t.cols) continue;
+    const int page = a.t.page(sq, pi);
+    if (page < 0 || page >= a.c.n_pages) continue;
+    row[j] = (long long)a.c.row(a.layer, page, h, pos - pi * a.c.page_size);
+  }
+#pragma unroll
+  for (int j = 0; j < kStoreItems; j++) {
+    const int which = j & 1;
+    float inv = 0.0f;
+    if constexpr (E::kScaled) {
+      float m = fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w)));
+#pragma unroll
+      for (int o = LG / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      float s = m / 127.0f;
+      if (s == 0.0f) s = 1.0f;
+      inv = 1.0f / s;
+      if (lane == 0 && row[j] >= 0) (which ? a.c.vs : a.c.ks)[row[j]] = s;
+    }
+    if (row[j] >= 0 && lane * 4 < D)
+      pack_store<E>((typename E::T *)(which ? a.c.v : a.c.k) + row[j] * D + lane * 4, x[j], inv);
   }
 }
 

@@ -22,7 +22,15 @@ namespace {
 // tickets. Growing waits for the stream, whose queued calls use the old one.
 llmq_status serve_ws(llmq_ctx *ctx, size_t bytes, size_t tickets, ServeWs **out) {
   ServeWs &w = ctx->serve_ws[ctx->stream];
-  if (w.bytes < bytes || w.n_tickets < tickets) CK(cudaStreamSynchronize(ctx->stream));
+  if (w.bytes >= bytes && w.n_tickets >= tickets) {
+    *out = &w;
+    return LLMQ_OK;
+  }
+  cudaStreamCaptureStatus cap;
+  CK(cudaStreamIsCapturing(ctx->stream, &cap));
+  if (cap != cudaStreamCaptureStatusNone)
+    return fail(ctx, LLMQ_ERR_INVALID, "the serving workspace grows on first use: run the call once before capturing it");
+  CK(cudaStreamSynchronize(ctx->stream));
   if (w.bytes < bytes) {
     if (w.buf) cudaFree(w.buf);
     w.buf = nullptr;
@@ -81,6 +89,46 @@ cudaError_t launch_attend(const AttendArgs &a, unsigned grid, cudaStream_t s) {
   }
 }
 
+template <typename E, int D>
+void launch_store_d(const StoreArgs &a, bool vec, unsigned grid, cudaStream_t s) {
+  if (vec)
+    paged_store_kernel<E, D, true><<<grid, 256, 0, s>>>(a);
+  else
+    paged_store_kernel<E, D, false><<<grid, 256, 0, s>>>(a);
+}
+template <typename E>
+void launch_store_e(const StoreArgs &a, bool vec, unsigned grid, cudaStream_t s) {
+  switch (a.c.head_dim) {
+    case 32: return launch_store_d<E, 32>(a, vec, grid, s);
+    case 64: return launch_store_d<E, 64>(a, vec, grid, s);
+    case 96: return launch_store_d<E, 96>(a, vec, grid, s);
+    default: return launch_store_d<E, 128>(a, vec, grid, s);
+  }
+}
+cudaError_t launch_store(const StoreArgs &a, bool vec, unsigned grid, cudaStream_t s) {
+  if (a.c.kind == LLMQ_KV_QUANT8)
+    launch_store_e<PgInt8>(a, vec, grid, s);
+  else if (a.c.kind == LLMQ_KV_BF16)
+    launch_store_e<PgBf16>(a, vec, grid, s);
+  else
+    launch_store_e<PgF32>(a, vec, grid, s);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_move(const EvictArgs &a, int tiles, unsigned grid, cudaStream_t s) {
+  switch (a.c.head_dim * elem_bytes(a.c.kind) / 16) {
+    case 2: evict_move_kernel<2><<<grid, 256, 0, s>>>(a, tiles); break;
+    case 4: evict_move_kernel<4><<<grid, 256, 0, s>>>(a, tiles); break;
+    case 6: evict_move_kernel<6><<<grid, 256, 0, s>>>(a, tiles); break;
+    case 8: evict_move_kernel<8><<<grid, 256, 0, s>>>(a, tiles); break;
+    case 12: evict_move_kernel<12><<<grid, 256, 0, s>>>(a, tiles); break;
+    case 16: evict_move_kernel<16><<<grid, 256, 0, s>>>(a, tiles); break;
+    case 24: evict_move_kernel<24><<<grid, 256, 0, s>>>(a, tiles); break;
+    default: evict_move_kernel<32><<<grid, 256, 0, s>>>(a, tiles);
+  }
+  return cudaGetLastError();
+}
+
 constexpr int kMaxSplits = 256;  // chunks of one unit that its last CTA joins
 constexpr int kMaxChunk = 4096;  // positions whose rows fit in shared memory without asking for more
 
@@ -97,14 +145,14 @@ llmq_status llmq_paged_create(llmq_ctx *ctx, int kind, int n_layer, int n_pages,
   *out = nullptr;
   if (kind != LLMQ_KV_QUANT8 && kind != LLMQ_KV_F32 && kind != LLMQ_KV_BF16)
     return fail(ctx, LLMQ_ERR_UNSUPPORTED, "a paged cache holds int8, float32 or bfloat16");
-  if ((double)n_pages * n_kv_head * page_size > INT_MAX)
-    return fail(ctx, LLMQ_ERR_INVALID, "more than 2^31 - 1 rows in a layer");
   if (n_layer <= 0 || n_pages <= 0 || page_size <= 0 || n_kv_head <= 0 || head_dim <= 0 || head_dim % 32 ||
       head_dim > 128)
     return fail(ctx, LLMQ_ERR_INVALID, "bad paged cache shape (head_dim: 32, 64, 96 or 128)");
   CK(cudaSetDevice(ctx->device));
   const double rows_d = (double)n_layer * n_pages * n_kv_head * page_size;
   if (rows_d * head_dim * 4 > 4e12) return fail(ctx, LLMQ_ERR_NOMEM, "paged cache larger than any device");
+  if ((double)n_pages * n_kv_head * page_size > INT_MAX)
+    return fail(ctx, LLMQ_ERR_INVALID, "more than 2^31 - 1 rows in a layer");
   const size_t rows = (size_t)n_layer * n_pages * n_kv_head * page_size;
   const size_t bytes = rows * head_dim * elem_bytes(kind);
   llmq_paged *p = new llmq_paged();
@@ -156,16 +204,14 @@ llmq_status llmq_paged_store(llmq_ctx *ctx, llmq_paged *p, int layer, const floa
   if (n_rows <= 0 || (!seq && n_rows > n_seqs)) return fail(ctx, LLMQ_ERR_INVALID, "bad row count");
   if (k_stride < 0 || v_stride < 0) return fail(ctx, LLMQ_ERR_INVALID, "negative stride");
   CK(cudaSetDevice(ctx->device));
-  const unsigned g = grid1(((long long)n_rows * p->v.n_kv_head * 2 + 7) / 8);
+  const StoreArgs a{p->v, PageTable{table, table_stride, table_cols, n_seqs}, layer, n_rows, k, v, k_stride, v_stride,
+                    seq, pos};
+  const int per = kStoreItems * (p->v.head_dim == 96 ? 8 : 1024 / p->v.head_dim);  // items of a CTA
+  const long long items = (long long)n_rows * p->v.n_kv_head * 2;
+  const unsigned g = items <= 2LL * INT_MAX ? grid1((items + per - 1) / per) : 0;
   if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
-  const StoreArgs a{p->v, PageTable{table, table_stride, table_cols, n_seqs}, layer, n_rows, k, v, k_stride, v_stride, seq, pos};
-  if (p->v.kind == LLMQ_KV_QUANT8)
-    paged_store_kernel<PgInt8><<<g, 256, 0, ctx->stream>>>(a);
-  else if (p->v.kind == LLMQ_KV_BF16)
-    paged_store_kernel<PgBf16><<<g, 256, 0, ctx->stream>>>(a);
-  else
-    paged_store_kernel<PgF32><<<g, 256, 0, ctx->stream>>>(a);
-  CKL();
+  const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && (n_rows == 1 || (k_stride % 4 == 0 && v_stride % 4 == 0));
+  CK(launch_store(a, vec, g, ctx->stream));
   return LLMQ_OK;
 }
 
@@ -254,12 +300,15 @@ llmq_status llmq_paged_evict(llmq_ctx *ctx, llmq_paged *p, int layer0, int n_lay
               max_len, budget, sinks, recent, lens, weights, weights_stride, kept, weights_out, weights_out_stride,
               lens_out};
   const long long rows = (long long)n_layers * n_seqs * p->v.n_kv_head;
-  const unsigned g = grid1(rows), gm = grid1((long long)((double)rows * budget < 1e14 ? (rows * budget + 7) / 8 : 0));
+  const int tiles = (std::min(budget, max_len) + kEvPos - 1) / kEvPos;
+  const unsigned g = grid1(rows), gm = g ? grid1(rows * tiles) : 0;
   if (!g || !gm) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
-  evict_select_kernel<<<g, 1024, 0, ctx->stream>>>(a);
+  if ((uintptr_t)weights % 16 == 0 && weights_stride % 4 == 0)
+    evict_select_kernel<true><<<g, kEvThreads, 0, ctx->stream>>>(a);
+  else
+    evict_select_kernel<false><<<g, kEvThreads, 0, ctx->stream>>>(a);
   CKL();
-  evict_move_kernel<<<gm, 256, 0, ctx->stream>>>(a, p->v.head_dim * elem_bytes(p->v.kind));
-  CKL();
+  CK(launch_move(a, tiles, gm, ctx->stream));
   return LLMQ_OK;
 }
 
@@ -277,24 +326,33 @@ llmq_status llmq_process_logits(llmq_ctx *ctx, const float *logits, long long lo
     return fail(ctx, LLMQ_ERR_INVALID, "a bias needs offsets, ids and values");
   if ((u.bias_ids && u.n_bias < 0) || (u.mask && u.mask_stride < 0)) return fail(ctx, LLMQ_ERR_INVALID, "negative size");
   CK(cudaSetDevice(ctx->device));
-  const int tiles = (V + kRuleTile - 1) / kRuleTile;
+  // tiles of 4096 logits; smaller ones while the call has fewer CTAs than two
+  // per SM
+  int vpt = 16;
+  constexpr int nth = 256;
+  while (vpt > 4 && (long long)n * ((V + 3 + nth * vpt - 1) / (nth * vpt)) < 2 * ctx->num_sms) vpt /= 2;
+  const int T = nth * vpt;
+  const int tiles = (V + 3 + T - 1) / T;  // a row may start 3 logits past a 16-byte boundary
   const unsigned g = grid1((long long)n * tiles);
   if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
+  const size_t sm = (size_t)T * 4 * ((u.ids ? 1 : 0) + (u.bias_ids ? 1 : 0));
   RuleArgs a{logits, out, logits_stride, out_stride, n, V, tiles, u.repetition, u.presence, u.frequency, u.ids,
-             u.n_ids, u.n_prompt, u.ids_stride, u.max_ids, u.n_bias, u.bias_offsets, u.bias_ids, u.bias_values, u.mask, u.mask_stride,
-             nullptr};
-  if (argmax) {
+             u.n_ids, u.n_prompt, u.ids_stride, u.max_ids, u.n_bias, u.bias_offsets, u.bias_ids, u.bias_values, u.mask,
+             u.mask_stride, nullptr, nullptr, argmax};
+  if (argmax && tiles > 1) {
     ServeWs *ws;
-    llmq_status st = serve_ws(ctx, (size_t)g * 8, 0, &ws);
+    llmq_status st = serve_ws(ctx, (size_t)g * 8, n, &ws);
     if (st != LLMQ_OK) return st;
     a.best = (unsigned long long *)ws->buf;
+    a.tickets = ws->tickets;
   }
-  logit_rules_kernel<<<g, 256, 0, ctx->stream>>>(a);
+  if (vpt == 16)
+    logit_rules_kernel<nth, 16><<<g, nth, sm, ctx->stream>>>(a);
+  else if (vpt == 8)
+    logit_rules_kernel<nth, 8><<<g, nth, sm, ctx->stream>>>(a);
+  else
+    logit_rules_kernel<nth, 4><<<g, nth, sm, ctx->stream>>>(a);
   CKL();
-  if (argmax) {
-    logit_argmax_kernel<<<n, 32, 0, ctx->stream>>>(a.best, tiles, argmax);
-    CKL();
-  }
   return LLMQ_OK;
 }
 
