@@ -37,17 +37,14 @@ struct PageTable {
 struct PgInt8 {
   typedef int8_t T;
   static constexpr bool kScaled = true;
-  static __device__ __forceinline__ float load(T x) { return (float)x; }
 };
 struct PgBf16 {
   typedef uint16_t T;
   static constexpr bool kScaled = false;
-  static __device__ __forceinline__ float load(T x) { return __uint_as_float((uint32_t)x << 16); }
 };
 struct PgF32 {
   typedef float T;
   static constexpr bool kScaled = false;
-  static __device__ __forceinline__ float load(T x) { return x; }
 };
 
 struct StoreArgs {
@@ -158,68 +155,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ int paged_len(const AttendArgs &a, int b) {
   const long long cap = (long long)a.t.cols * a.c.page_size;
   return max(0, min(min(a.lens[b], a.max_len), (int)min(cap, (long long)INT_MAX)));
-}
-
-// out = sum_j softmax_j(scale q . k_j) v_j for one (sequence, head) per CTA,
-// in one pass: each warp takes every eighth position with its own running
-// maximum and sum, lanes hold dimensions lane + 32 i; the warps' states are
-// joined at the end. grid (n_seqs * n_head), 256 threads.
-template <typename E>
-__global__ void __launch_bounds__(256) paged_attend_kernel(AttendArgs a) {
-  __shared__ float sm[8], sl[8], so[8][128];
-  const int b = blockIdx.x / a.n_head, h = blockIdx.x % a.n_head, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int D = a.c.head_dim, kh = h / (a.n_head / a.c.n_kv_head), len = paged_len(a, b);
-  float q[4], acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-    q[i] = lane + 32 * i < D ? a.q[(size_t)b * a.q_stride + (size_t)h * D + lane + 32 * i] : 0.0f;
-  float m = -INFINITY, l = 0.0f;
-  for (int j = warp; j < len; j += 8) {
-    const int page = a.t.page(b, j / a.c.page_size);
-    float s = -INFINITY;
-    if (page >= 0 && page < a.c.n_pages) {
-      const size_t row = a.c.row(a.layer, page, kh, j % a.c.page_size);
-      const typename E::T *k = (const typename E::T *)a.c.k + row * D, *v = (const typename E::T *)a.c.v + row * D;
-      float d = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (lane + 32 * i < D) d = fmaf(q[i], E::load(k[lane + 32 * i]), d);
-      for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-      if (E::kScaled) d *= a.c.ks[row];
-      s = d * a.scale2;
-      const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : exp2_approx(m - mn), p = exp2_approx(s - mn);
-      l = fmaf(l, c, p);
-      m = mn;
-      const float w = E::kScaled ? p * a.c.vs[row] : p;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (lane + 32 * i < D) acc[i] = fmaf(w, E::load(v[lane + 32 * i]), acc[i] * c);
-    }
-    if (a.scores && lane == 0) a.scores[((size_t)b * a.n_head + h) * a.max_len + j] = s;
-  }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++) so[warp][lane + 32 * i] = acc[i];
-  __syncthreads();
-  float M = -INFINITY, L = 0.0f;
-  for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w]);
-  float c[8];
-  for (int w = 0; w < 8; w++) {
-    c[w] = sm[w] == -INFINITY ? 0.0f : exp2_approx(sm[w] - M);
-    L = fmaf(sl[w], c[w], L);
-  }
-  if (a.stat && threadIdx.x == 0) {
-    a.stat[2 * blockIdx.x] = M;
-    a.stat[2 * blockIdx.x + 1] = L;
-  }
-  if (threadIdx.x < D) {
-    float o = 0.0f;
-    for (int w = 0; w < 8; w++) o = fmaf(so[w][threadIdx.x], c[w], o);
-    a.out[(size_t)b * a.out_stride + (size_t)h * D + threadIdx.x] = L == 0.0f ? 0.0f : o / L;
-  }
 }
 
 // weights_out[b][kv head][j] = weights[b][kv head][j] + sum over the kv

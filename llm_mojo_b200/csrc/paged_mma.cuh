@@ -1,5 +1,5 @@
-// paged_mma.cuh -- attention of one new token over a paged int8 or bfloat16
-// cache on the tensor cores, split over positions and joined.
+// paged_mma.cuh -- attention of one new token over a paged cache on the
+// tensor cores, split over positions and joined.
 //
 // One pass over the cache: scores S = Q K^T, running maximum M and sum L of
 // 2^(s - M), and O = P V, as m16n8k16 products with float32 accumulators,
@@ -11,21 +11,24 @@
 //             second (22 bits; codes are exact in f16),
 //   bfloat16: x = bf16 + bf16 + bf16 by truncation (all 24 bits): rows 0-7
 //             and 8-15 the first two, a second product the third,
-// and a head's result is the sum of its rows. One pass with the terms in
-// otherwise idle rows costs no more issue slots than a half-empty tile would.
+//   float32:  both factors in three bf16 terms, the products of weight
+//             2^-24 and above,
+// and a head's result is the sum of its rows. The terms sit in rows that one
+// query head or a few would leave idle.
 //
 // Both products may take dimensions and positions in any order that their
-// two operands share, so a lane loads contiguous bytes of a row straight
-// from memory into operand registers: of K, rows (lane / 4) and + 8, bytes
-// of the lane's quarter of each run; of V, the four rows whose weights the
-// lane holds, an eighth each.
+// two operands share, so a lane reads contiguous bytes of a row as its
+// operand: of K, rows (lane / 4) and + 8, pieces of every run; of V, the
+// four rows whose weights the lane holds, an eighth each. A lane copies
+// (cp.async) the bytes that it will read itself into its own slots of a ring
+// in shared memory, [piece][lane], so that reads have no bank conflicts,
+// nothing waits for another lane, and the copies in flight cost no
+// registers.
 #pragma once
 
 #include "paged.cuh"
 
 namespace llmq {
-
-constexpr int kPmWarps = 4;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -39,17 +42,25 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// BYTES (4, 8 or 16) of the cache into registers; read once, so not kept in L1.
+// BYTES (4, 8 or 16) into the lane's slot; 16 bypass L1: the cache is read once.
 template <int BYTES>
-__device__ __forceinline__ void pm_load(uint32_t *d, const char *p) {
+__device__ __forceinline__ void pm_copy(unsigned dst, const void *src) {
   if constexpr (BYTES == 16)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                 : "l"(p));
-  else if constexpr (BYTES == 8)
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "l"(p));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   else
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(d[0]) : "l"(p));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void pm_read(uint32_t *d, unsigned src) {
+  if constexpr (BYTES == 16)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(src)
+                 : "memory");
+  else if constexpr (BYTES == 8)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "r"(src) : "memory");
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(d[0]) : "r"(src) : "memory");
 }
 
 // Two f16 from two biased codes (code ^ 0x80) in bytes i and j of x: 1024 +
@@ -83,13 +94,21 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t &t0, uint3
 
 // How a lane's bytes of a row map to dimensions. K: runs of 4 kCk bytes, a
 // lane's piece t; V: runs of 8 kCv bytes, piece g.
-template <bool I8, int D>
+enum { PM_I8 = 0, PM_BF16 = 1, PM_F32 = 2 };
+template <int KIND, int D>
 struct PmShape {
-  static constexpr int kEs = I8 ? 1 : 2;
-  static constexpr int kKb = D / 4 * kEs, kVb = D / 8 * kEs;  // a lane's bytes of a K / V row
+  static constexpr int kEs = KIND == PM_I8 ? 1 : KIND == PM_BF16 ? 2 : 4;
+  static constexpr int kRow = D * kEs;
+  static constexpr int kKb = kRow / 4, kVb = kRow / 8;  // a lane's bytes of a K / V row
   static constexpr int kCk = kKb % 16 == 0 ? 16 : 8;
   static constexpr int kCv = kVb % 16 == 0 ? 16 : (kVb % 8 == 0 ? 8 : 4);
+  static constexpr int kNk = kKb / kCk, kNv = kVb / kCv;  // pieces
   static constexpr int kSteps = D / 16;
+  // a stage of a warp's ring: two K rows, four V rows and (int8) the scales
+  // of four positions for keys and values, of each lane
+  static constexpr int kStage = 32 * (2 * kKb + 4 * kVb + (KIND == PM_I8 ? 32 : 0));
+  // stages: about 3 KB or more in flight per warp
+  static constexpr int kStages = kStage <= 2048 ? 4 : kStage <= 4096 ? 3 : 2;
   static __device__ __forceinline__ int kdim(int x, int t) {  // dimension of a lane's x-th K element
     constexpr int E = kCk / kEs;
     return (x / E * 4 + t) * E + x % E;
@@ -100,23 +119,28 @@ struct PmShape {
   }
 };
 
-__host__ __device__ inline size_t pm_smem(int chunk, int D, bool fast) {
-  // the tiles' first rows (page_size % 16 == 0) or every position's row; then the warps' states
-  const size_t rows = ((size_t)(fast ? chunk / 16 : chunk) * 4 + 15) / 16 * 16;
-  const size_t join = (size_t)kPmWarps * 8 * (D + 2) * 4;
-  return rows + join;
+// Dynamic shared memory: the rows of the tiles (page_size % 16 == 0) or of
+// every position of a chunk; then the rings, and in their place, at the end,
+// the warps' states.
+__host__ __device__ inline int pm_rows_bytes(int chunk, bool fast) { return ((fast ? chunk / 16 : chunk) * 4 + 15) / 16 * 16; }
+template <int KIND, int D, int W>
+__host__ __device__ inline size_t pm_smem(int chunk, bool fast) {
+  typedef PmShape<KIND, D> Sh;
+  const size_t ring = (size_t)W * Sh::kStages * Sh::kStage, join = (size_t)W * 8 * (D + 2) * 4;
+  return pm_rows_bytes(chunk, fast) + (ring > join ? ring : join);
 }
 
 // One CTA: one unit (sequence, kv head, up to 8 of its query heads) and one
-// chunk of positions, tiles of 16 dealt to the 4 warps. FAST: page_size is a
+// chunk of positions, tiles of 16 dealt to the W warps. FAST: page_size is a
 // multiple of 16, a tile lies in one page. The chunks of a unit write their
 // sums to a.part; the last to arrive joins them in chunk order (so the bits
 // do not depend on the order of arrival) and leaves its ticket zero.
 // grid n_seqs * n_kv_head * head_chunks * splits.
-template <bool I8, int D, bool FAST>
-__global__ void __launch_bounds__(kPmWarps * 32) paged_mma_kernel(AttendArgs a) {
-  typedef PmShape<I8, D> Sh;
-  constexpr int kKw = Sh::kKb / 4, kVw = Sh::kVb / 4, NT = D / 8;
+template <int KIND, int D, bool FAST, int W>
+__global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
+  typedef PmShape<KIND, D> Sh;
+  constexpr bool I8 = KIND == PM_I8;
+  constexpr int NT = D / 8, S = Sh::kStages;
   extern __shared__ __align__(16) char smem[];
   __shared__ int s_last;
   const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
@@ -127,18 +151,18 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_mma_kernel(AttendArgs a) 
   const int len = paged_len(a, b), ps = a.c.page_size;
   const int ns = max(1, (len + a.chunk - 1) / a.chunk);
   if (split >= ns) return;
-  const int c0 = split * a.chunk, c1 = min(len, c0 + a.chunk);
-  const int ntiles = (c1 - c0 + 15) / 16;
+  const int c0 = split * a.chunk, n = min(len - c0, a.chunk);  // the chunk's positions
+  const int ntiles = (n + 15) / 16;
   int *rows = (int *)smem;
-  float *join = (float *)(smem + ((size_t)(FAST ? a.chunk / 16 : a.chunk) * 4 + 15) / 16 * 16);
+  char *pool = smem + pm_rows_bytes(a.chunk, FAST);
 
   // rows of the chunk, relative to this layer's and kv head's first; -1: no page
-  for (int i = tid; i < (FAST ? ntiles : ntiles * 16); i += kPmWarps * 32) {
-    const int pos = c0 + (FAST ? i * 16 : i);
+  for (int i = tid; i < (FAST ? ntiles : ntiles * 16); i += W * 32) {
+    const int j = FAST ? i * 16 : i;
     int row = -1;
-    if (pos < c1) {
-      const int pi = pos / ps, page = a.t.page(b, pi);
-      if (page >= 0 && page < a.c.n_pages) row = page * (a.c.n_kv_head * ps) + (pos - pi * ps);
+    if (j < n) {
+      const int pi = (c0 + j) / ps, page = a.t.page(b, pi);
+      if (page >= 0 && page < a.c.n_pages) row = page * (a.c.n_kv_head * ps) + (c0 + j - pi * ps);
     }
     rows[i] = row;
   }
@@ -176,107 +200,137 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_mma_kernel(AttendArgs a) 
       }
     }
   }
-  __syncthreads();
+  if constexpr (W > 1)
+    __syncthreads();
+  else
+    __syncwarp();
 
+  // the lane's first bytes in the pool, and its slots
   const size_t first = a.c.row(a.layer, 0, kh, 0);
-  const char *kb = (const char *)a.c.k + first * (D * Sh::kEs), *vb = (const char *)a.c.v + first * (D * Sh::kEs);
-  uint32_t kr[2][kKw], vr[4][kVw];
-  float ksc[4], vsc[4];  // the scales of the lane's positions 2t, 2t + 1, 8 + 2t, 9 + 2t
-  auto pos_of = [&](int i) { return (i >> 1) * 8 + 2 * t + (i & 1); };
-  auto row_of = [&](int tile, int i) { return max(FAST ? rows[tile] + i : rows[tile * 16 + i], 0); };
-  auto load_k = [&](int tile) {
+  const char *kl = (const char *)a.c.k + first * Sh::kRow + t * Sh::kCk + (FAST ? g * Sh::kRow : 0);
+  const char *vl = (const char *)a.c.v + first * Sh::kRow + g * Sh::kCv + (FAST ? 2 * t * Sh::kRow : 0);
+  const float *ksl = I8 ? a.c.ks + first + (FAST ? 2 * t : 0) : nullptr;
+  const float *vsl = I8 ? a.c.vs + first + (FAST ? 2 * t : 0) : nullptr;
+  const unsigned ring = (unsigned)__cvta_generic_to_shared(pool) + warp * (S * Sh::kStage);
+  constexpr int kVat = 64 * Sh::kKb, kSat = kVat + 128 * Sh::kVb;  // a stage: K, V, scales
+  auto pos_of = [&](int i) { return (i >> 1) * 8 + 2 * t + (i & 1); };  // the lane's position i of a tile
+  auto issue = [&](int tile, int stage) {
+    const unsigned d = ring + stage * Sh::kStage;
+    const int base = FAST ? max(rows[tile], 0) : 0;
 #pragma unroll
     for (int r = 0; r < 2; r++) {
-      const char *p = kb + (size_t)row_of(tile, 8 * r + g) * (D * Sh::kEs);
+      const char *p = FAST ? kl + (size_t)base * Sh::kRow + r * 8 * Sh::kRow
+                           : kl + (size_t)max(rows[tile * 16 + 8 * r + g], 0) * Sh::kRow;
 #pragma unroll
-      for (int i = 0; i < Sh::kKb / Sh::kCk; i++) pm_load<Sh::kCk>(&kr[r][i * (Sh::kCk / 4)], p + (i * 4 + t) * Sh::kCk);
+      for (int i = 0; i < Sh::kNk; i++)
+        pm_copy<Sh::kCk>(d + (r * Sh::kNk + i) * 32 * Sh::kCk + lane * Sh::kCk, p + i * 4 * Sh::kCk);
     }
-    if constexpr (I8) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) ksc[i] = a.c.ks[first + row_of(tile, pos_of(i))];
-    }
-  };
-  auto load_v = [&](int tile) {
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      const char *p = vb + (size_t)row_of(tile, pos_of(r)) * (D * Sh::kEs);
+      const int row = FAST ? base : max(rows[tile * 16 + pos_of(r)], 0);
+      const char *p = vl + (size_t)row * Sh::kRow + (FAST ? ((r >> 1) * 8 + (r & 1)) * Sh::kRow : 0);
 #pragma unroll
-      for (int i = 0; i < Sh::kVb / Sh::kCv; i++) pm_load<Sh::kCv>(&vr[r][i * (Sh::kCv / 4)], p + (i * 8 + g) * Sh::kCv);
-    }
-    if constexpr (I8) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) vsc[i] = a.c.vs[first + row_of(tile, pos_of(i))];
+      for (int i = 0; i < Sh::kNv; i++)
+        pm_copy<Sh::kCv>(d + kVat + (r * Sh::kNv + i) * 32 * Sh::kCv + lane * Sh::kCv, p + i * 8 * Sh::kCv);
+      if constexpr (I8) {
+        const unsigned sd = d + kSat + lane * 8 + (r >> 1) * 256;
+        if constexpr (FAST) {
+          if (r % 2 == 0) {
+            pm_copy<8>(sd, ksl + (size_t)row + (r >> 1) * 8);
+            pm_copy<8>(sd + 512, vsl + (size_t)row + (r >> 1) * 8);
+          }
+        } else {
+          pm_copy<4>(sd + (r & 1) * 4, ksl + row);
+          pm_copy<4>(sd + 512 + (r & 1) * 4, vsl + row);
+        }
+      }
     }
   };
+  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
 
   float acc[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; j++)
 #pragma unroll
     for (int i = 0; i < 4; i++) acc[j][i] = 0.0f;
-  float m = -INFINITY, l = 0.0f, vlim = 0x1p-100f;
+  float m = -INFINITY, l = 0.0f, vlim = 0x1p-100f, vinv = 0x1p115f;
 
-  if (warp < ntiles) {
-    load_k(warp);
-    load_v(warp);
+#pragma unroll
+  for (int i = 0; i < S - 1; i++) {
+    if (warp + i * W < ntiles) issue(warp + i * W, i);
+    commit();
   }
-  for (int tile = warp; tile < ntiles; tile += kPmWarps) {
-    const bool more = tile + kPmWarps < ntiles;
+  int stage = 0;
+  for (int tile = warp; tile < ntiles; tile += W) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+    if (tile + (S - 1) * W < ntiles) issue(tile + (S - 1) * W, stage == 0 ? S - 1 : stage - 1);
+    commit();
+    const unsigned src = ring + stage * Sh::kStage;
+    stage = stage == S - 1 ? 0 : stage + 1;
     // scores of 16 positions: two n-tiles of 8
     float c[2][4];
 #pragma unroll
     for (int r = 0; r < 2; r++) {
 #pragma unroll
       for (int i = 0; i < 4; i++) c[r][i] = 0.0f;
+      uint32_t kr[Sh::kKb / 4];
+#pragma unroll
+      for (int i = 0; i < Sh::kNk; i++)
+        pm_read<Sh::kCk>(kr + i * (Sh::kCk / 4), src + (r * Sh::kNk + i) * 32 * Sh::kCk + lane * Sh::kCk);
 #pragma unroll
       for (int k = 0; k < Sh::kSteps; k++) {
-        if constexpr (I8) {
-          const uint32_t x = kr[r][k] ^ 0x80808080u;
+        if constexpr (KIND == PM_I8) {
+          const uint32_t x = kr[k] ^ 0x80808080u;
           mma_f16(c[r], qa[k], codes_f16(x, 0x4140), codes_f16(x, 0x4342));
         } else {
-          mma_bf16(c[r], qa[k], kr[r][2 * k], kr[r][2 * k + 1]);
           const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
-          mma_bf16(c[r], q2, kr[r][2 * k], kr[r][2 * k + 1]);
+          if constexpr (KIND == PM_BF16) {
+            mma_bf16(c[r], qa[k], kr[2 * k], kr[2 * k + 1]);
+            mma_bf16(c[r], q2, kr[2 * k], kr[2 * k + 1]);
+          } else {
+            uint32_t x[3], y[3];
+            split_bf16(__uint_as_float(kr[4 * k]), __uint_as_float(kr[4 * k + 1]), x[0], x[1], x[2]);
+            split_bf16(__uint_as_float(kr[4 * k + 2]), __uint_as_float(kr[4 * k + 3]), y[0], y[1], y[2]);
+            mma_bf16(c[r], q2, x[0], y[0]);
+#pragma unroll
+            for (int i = 2; i >= 0; i--) mma_bf16(c[r], qa[k], x[i], y[i]);
+          }
         }
       }
     }
     float s[4], sv[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      s[i] = (c[i >> 1][i & 1] + c[i >> 1][2 + (i & 1)]) * fs;
-      if constexpr (I8) {
-        s[i] *= ksc[i];
-        sv[i] = vsc[i];
-      }
-    }
-    // positions past the end or without a page
-    bool ok[4];
-    bool whole = c0 + tile * 16 + 16 <= c1;
-    if constexpr (FAST)
-      whole = whole && rows[tile] >= 0;
-    else
-      whole = false;
-    if (!whole) {
+    if constexpr (I8) {
+      uint32_t ks[4], vs[4];
+      pm_read<8>(ks, src + kSat + lane * 8);
+      pm_read<8>(ks + 2, src + kSat + 256 + lane * 8);
+      pm_read<8>(vs, src + kSat + 512 + lane * 8);
+      pm_read<8>(vs + 2, src + kSat + 768 + lane * 8);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        ok[i] = c0 + tile * 16 + pos_of(i) < c1 && rows[FAST ? tile : tile * 16 + pos_of(i)] >= 0;
-        if (!ok[i]) {
+        s[i] = (c[i >> 1][i & 1] + c[i >> 1][2 + (i & 1)]) * fs * __uint_as_float(ks[i]);
+        sv[i] = __uint_as_float(vs[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[i] = (c[i >> 1][i & 1] + c[i >> 1][2 + (i & 1)]) * fs;
+    }
+    // positions past the end or without a page: no score, and a zero value
+    // (0 times what is there might be NaN)
+    unsigned masked = 0;
+    if (!FAST || tile * 16 + 16 > n || rows[tile] < 0) {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (tile * 16 + pos_of(i) >= n || rows[FAST ? tile : tile * 16 + pos_of(i)] < 0) {
+          masked |= 1u << i;
           s[i] = -INFINITY;
           sv[i] = 0.0f;
-          // 0 times what is there might be NaN
-#pragma unroll
-          for (int w = 0; w < kVw; w++) vr[i][w] = 0;
         }
-      }
     }
-    if (more) load_k(tile + kPmWarps);
     if (a.scores && g < nh) {
-      float *out = a.scores + ((size_t)b * a.n_head + h0 + g) * a.max_len;
+      float *out = a.scores + ((size_t)b * a.n_head + h0 + g) * a.max_len + c0 + tile * 16;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int pos = c0 + tile * 16 + pos_of(i);
-        if (pos < c1) out[pos] = s[i];
-      }
+      for (int i = 0; i < 4; i++)
+        if (tile * 16 + pos_of(i) < n) out[pos_of(i)] = s[i];
     }
     float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -299,6 +353,7 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_mma_kernel(AttendArgs a) 
           const float up = __uint_as_float(min((__float_as_uint(vm) & 0x7f800000u) + 0x800000u, 254u << 23));
           f *= vlim / up;
           vlim = up;
+          vinv = 0x1p15f / up;
         }
       }
 #pragma unroll
@@ -315,9 +370,8 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_mma_kernel(AttendArgs a) 
     }
     uint32_t pa[4], pb[4] = {0u, 0u, 0u, 0u};
     if constexpr (I8) {
-      const float f = 0x1p15f / vlim;
 #pragma unroll
-      for (int i = 0; i < 4; i++) p[i] *= sv[i] * f;
+      for (int i = 0; i < 4; i++) p[i] *= sv[i] * vinv;
       split_f16(p[0], p[1], pa[0], pa[1]);
       split_f16(p[2], p[3], pa[2], pa[3]);
     } else {
@@ -325,29 +379,59 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_mma_kernel(AttendArgs a) 
       split_bf16(p[2], p[3], pa[2], pa[3], pb[2]);
     }
 #pragma unroll
-    for (int w = 0; w < kVw; w++) {
-      if constexpr (I8) {
-        const uint32_t v0 = vr[0][w] ^ 0x80808080u, v1 = vr[1][w] ^ 0x80808080u, v2 = vr[2][w] ^ 0x80808080u,
-                       v3 = vr[3][w] ^ 0x80808080u;
-        const uint32_t x = __byte_perm(v0, v1, 0x5140), y = __byte_perm(v2, v3, 0x5140);
-        const uint32_t z = __byte_perm(v0, v1, 0x7362), u = __byte_perm(v2, v3, 0x7362);
-        mma_f16(acc[4 * w], pa, codes_f16(x, 0x4140), codes_f16(y, 0x4140));
-        mma_f16(acc[4 * w + 1], pa, codes_f16(x, 0x4342), codes_f16(y, 0x4342));
-        mma_f16(acc[4 * w + 2], pa, codes_f16(z, 0x4140), codes_f16(u, 0x4140));
-        mma_f16(acc[4 * w + 3], pa, codes_f16(z, 0x4342), codes_f16(u, 0x4342));
-      } else {
-        const uint32_t x0 = __byte_perm(vr[0][w], vr[1][w], 0x5410), x1 = __byte_perm(vr[2][w], vr[3][w], 0x5410);
-        const uint32_t y0 = __byte_perm(vr[0][w], vr[1][w], 0x7632), y1 = __byte_perm(vr[2][w], vr[3][w], 0x7632);
-        mma_bf16(acc[2 * w], pa, x0, x1);
-        mma_bf16(acc[2 * w + 1], pa, y0, y1);
-        mma_bf16(acc[2 * w], pb, x0, x1);
-        mma_bf16(acc[2 * w + 1], pb, y0, y1);
+    for (int i = 0; i < Sh::kNv; i++) {
+      constexpr int kW = Sh::kCv / 4;
+      uint32_t vr[4][kW];
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        pm_read<Sh::kCv>(vr[r], src + kVat + (r * Sh::kNv + i) * 32 * Sh::kCv + lane * Sh::kCv);
+      if constexpr (!I8) {
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int w = 0; w < kW; w++)
+              if (masked >> r & 1u) vr[r][w] = 0u;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < kW; w++) {
+        if constexpr (KIND == PM_I8) {
+          float (*o)[4] = acc + 4 * (i * kW + w);
+          const uint32_t v0 = vr[0][w] ^ 0x80808080u, v1 = vr[1][w] ^ 0x80808080u, v2 = vr[2][w] ^ 0x80808080u,
+                         v3 = vr[3][w] ^ 0x80808080u;
+          const uint32_t x = __byte_perm(v0, v1, 0x5140), y = __byte_perm(v2, v3, 0x5140);
+          const uint32_t z = __byte_perm(v0, v1, 0x7362), u = __byte_perm(v2, v3, 0x7362);
+          mma_f16(o[0], pa, codes_f16(x, 0x4140), codes_f16(y, 0x4140));
+          mma_f16(o[1], pa, codes_f16(x, 0x4342), codes_f16(y, 0x4342));
+          mma_f16(o[2], pa, codes_f16(z, 0x4140), codes_f16(u, 0x4140));
+          mma_f16(o[3], pa, codes_f16(z, 0x4342), codes_f16(u, 0x4342));
+        } else if constexpr (KIND == PM_BF16) {
+          float (*o)[4] = acc + 2 * (i * kW + w);
+          const uint32_t x0 = __byte_perm(vr[0][w], vr[1][w], 0x5410), x1 = __byte_perm(vr[2][w], vr[3][w], 0x5410);
+          const uint32_t y0 = __byte_perm(vr[0][w], vr[1][w], 0x7632), y1 = __byte_perm(vr[2][w], vr[3][w], 0x7632);
+          mma_bf16(o[0], pa, x0, x1);
+          mma_bf16(o[1], pa, y0, y1);
+          mma_bf16(o[0], pb, x0, x1);
+          mma_bf16(o[1], pb, y0, y1);
+        } else {
+          float (&o)[4] = acc[i * kW + w];
+          uint32_t x[3], y[3];
+          split_bf16(__uint_as_float(vr[0][w]), __uint_as_float(vr[1][w]), x[0], x[1], x[2]);
+          split_bf16(__uint_as_float(vr[2][w]), __uint_as_float(vr[3][w]), y[0], y[1], y[2]);
+          mma_bf16(o, pb, x[0], y[0]);
+#pragma unroll
+          for (int k = 2; k >= 0; k--) mma_bf16(o, pa, x[k], y[k]);
+        }
       }
     }
-    if (more) load_v(tile + kPmWarps);
   }
 
-  // join the warps: [warp][head][D sums, M, L]
+  // join the warps: [warp][head][D sums, M, L] in the rings' place
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  float *join = (float *)pool;
+  if constexpr (W > 1) __syncthreads();
+  else __syncwarp();
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
   if (g < nh) {
@@ -363,16 +447,19 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_mma_kernel(AttendArgs a) 
       o[D + 1] = l;
     }
   }
-  __syncthreads();
-  for (int i = tid; i < nh * D; i += kPmWarps * 32) {
+  if constexpr (W > 1)
+    __syncthreads();
+  else
+    __syncwarp();
+  for (int i = tid; i < nh * D; i += W * 32) {
     const int h = i / D, d = i % D;
     const float *o = join + h * (D + 2);
     float M = -INFINITY, L = 0.0f, x = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kPmWarps; w++) M = fmaxf(M, o[w * 8 * (D + 2) + D]);
+    for (int w = 0; w < W; w++) M = fmaxf(M, o[w * 8 * (D + 2) + D]);
     const float mu = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-    for (int w = 0; w < kPmWarps; w++) {
+    for (int w = 0; w < W; w++) {
       const float f = exp2_approx(o[w * 8 * (D + 2) + D] - mu);
       L = fmaf(o[w * 8 * (D + 2) + D + 1], f, L);
       x = fmaf(o[w * 8 * (D + 2) + d], f, x);
@@ -399,7 +486,7 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_mma_kernel(AttendArgs a) 
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  for (int i = tid; i < nh * D; i += kPmWarps * 32) {
+  for (int i = tid; i < nh * D; i += W * 32) {
     const int h = i / D, d = i % D;
     const float *part = a.part + ((size_t)unit * a.splits * 8 + h) * (D + 2);
     float M = -INFINITY, L = 0.0f, x = 0.0f;

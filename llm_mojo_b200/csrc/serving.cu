@@ -68,25 +68,35 @@ llmq_status paged_check(llmq_ctx *ctx, const llmq_paged *p, int layer0, int n_la
   return LLMQ_OK;
 }
 
-// What the kernels of one cache shape have in common.
-template <bool I8, int D>
-cudaError_t launch_attend_mma(const AttendArgs &a, unsigned grid, cudaStream_t s) {
+template <int KIND, int D, int W>
+cudaError_t launch_attend_w(const AttendArgs &a, unsigned grid, cudaStream_t s) {
   const bool fast = a.c.page_size % 16 == 0;
-  const size_t sm = pm_smem(a.chunk, D, fast);
-  if (fast)
-    paged_mma_kernel<I8, D, true><<<grid, kPmWarps * 32, sm, s>>>(a);
-  else
-    paged_mma_kernel<I8, D, false><<<grid, kPmWarps * 32, sm, s>>>(a);
+  const size_t sm = pm_smem<KIND, D, W>(a.chunk, fast);
+  void (*k)(AttendArgs) = fast ? paged_mma_kernel<KIND, D, true, W> : paged_mma_kernel<KIND, D, false, W>;
+  if (sm > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute((const void *)k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+    if (e != cudaSuccess) return e;
+  }
+  k<<<grid, W * 32, sm, s>>>(a);
   return cudaGetLastError();
 }
-cudaError_t launch_attend(const AttendArgs &a, unsigned grid, cudaStream_t s) {
-  const bool i8 = a.c.kind == LLMQ_KV_QUANT8;
+template <int KIND, int D>
+cudaError_t launch_attend_d(const AttendArgs &a, int warps, unsigned grid, cudaStream_t s) {
+  return warps == 1 ? launch_attend_w<KIND, D, 1>(a, grid, s) : launch_attend_w<KIND, D, 4>(a, grid, s);
+}
+template <int KIND>
+cudaError_t launch_attend_k(const AttendArgs &a, int warps, unsigned grid, cudaStream_t s) {
   switch (a.c.head_dim) {
-    case 32: return i8 ? launch_attend_mma<true, 32>(a, grid, s) : launch_attend_mma<false, 32>(a, grid, s);
-    case 64: return i8 ? launch_attend_mma<true, 64>(a, grid, s) : launch_attend_mma<false, 64>(a, grid, s);
-    case 96: return i8 ? launch_attend_mma<true, 96>(a, grid, s) : launch_attend_mma<false, 96>(a, grid, s);
-    default: return i8 ? launch_attend_mma<true, 128>(a, grid, s) : launch_attend_mma<false, 128>(a, grid, s);
+    case 32: return launch_attend_d<KIND, 32>(a, warps, grid, s);
+    case 64: return launch_attend_d<KIND, 64>(a, warps, grid, s);
+    case 96: return launch_attend_d<KIND, 96>(a, warps, grid, s);
+    default: return launch_attend_d<KIND, 128>(a, warps, grid, s);
   }
+}
+cudaError_t launch_attend(const AttendArgs &a, int warps, unsigned grid, cudaStream_t s) {
+  if (a.c.kind == LLMQ_KV_QUANT8) return launch_attend_k<PM_I8>(a, warps, grid, s);
+  if (a.c.kind == LLMQ_KV_BF16) return launch_attend_k<PM_BF16>(a, warps, grid, s);
+  return launch_attend_k<PM_F32>(a, warps, grid, s);
 }
 
 template <typename E, int D>
@@ -243,18 +253,20 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   a.scale2 = (float)(scale * 1.4426950408889634);
   const size_t rows = (size_t)n_seqs * n_head;
   const int D = p->v.head_dim, G = n_head / p->v.n_kv_head;
-  const bool split = p->v.kind != LLMQ_KV_F32;
   a.head_chunks = (G + 7) / 8;
   const long long units = (long long)n_seqs * p->v.n_kv_head * a.head_chunks;
   // chunks so that the longest call's CTAs fill the GPU about twice over
-  const long long want = std::max(1LL, (long long)ctx->num_sms * 8 / units);
+  const int target = getenv("TGT") ? atoi(getenv("TGT")) : 8;
+  const long long want = std::max(1LL, (long long)ctx->num_sms * target / units);
   long long chunk = std::max(64LL, (a.max_len + want - 1) / want);
   chunk = std::max(chunk, (long long)(a.max_len + kMaxSplits - 1) / kMaxSplits);
   a.chunk = (int)std::min((chunk + 63) / 64 * 64, (long long)kMaxChunk);
   a.splits = (a.max_len + a.chunk - 1) / a.chunk;
-  const unsigned g = grid1(split ? units * a.splits : (long long)rows);
+  int warps = a.splits == 1 && units >= ctx->num_sms * 8 ? 1 : 4;
+  if (getenv("WARPS")) warps = atoi(getenv("WARPS"));
+  const unsigned g = grid1(units * a.splits);
   if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many sequences for one call");
-  const size_t parts = split && a.splits > 1 ? (size_t)units * a.splits * 8 * (D + 2) : 0;
+  const size_t parts = a.splits > 1 ? (size_t)units * a.splits * 8 * (D + 2) : 0;
   if (weights_out || parts) {
     ServeWs *ws;
     const size_t floats = parts + (weights_out ? rows * (a.max_len + 2) : 0);
@@ -266,12 +278,7 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
       a.scores = a.stat + rows * 2;
     }
   }
-  if (split) {
-    CK(launch_attend(a, g, ctx->stream));
-  } else {
-    paged_attend_kernel<PgF32><<<g, 256, 0, ctx->stream>>>(a);
-    CKL();
-  }
+  CK(launch_attend(a, warps, g, ctx->stream));
   if (weights_out) {
     const dim3 wg((max_len + 255) / 256, (unsigned)std::min((long long)n_seqs * p->v.n_kv_head, 65535LL));
     paged_weights_kernel<<<wg, 256, 0, ctx->stream>>>(a, max_len, weights, weights_out, weights_stride);
