@@ -140,8 +140,8 @@ struct AttendArgs {
   float *scores;  // [n_seqs][n_head][max_len], for the weights; else null
   float *stat;    // [n_seqs][n_head][2]: the maximum score M and the sum of 2^(score - M)
   // the split over positions (paged_mma.cuh)
-  int chunk, splits, head_chunks;
-  float *part;   // [unit][split][8][D + 2]: sums, then M and L of each head
+  int chunk, splits, head_chunks, unit_heads;
+  float *part;   // [unit][split][unit_heads][D + 2]: sums, then M and L of each head
   int *tickets;  // [unit], zero between launches
 };
 

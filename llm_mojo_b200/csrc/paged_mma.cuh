@@ -17,13 +17,13 @@
 // query head or a few would leave idle.
 //
 // Both products may take dimensions and positions in any order that their
-// two operands share, so a lane reads contiguous bytes of a row as its
-// operand: of K, rows (lane / 4) and + 8, pieces of every run; of V, the
-// four rows whose weights the lane holds, an eighth each. A lane copies
-// (cp.async) the bytes that it will read itself into its own slots of a ring
-// in shared memory, [piece][lane], so that reads have no bank conflicts,
-// nothing waits for another lane, and the copies in flight cost no
-// registers.
+// two operands share. A warp copies its tiles of 16 rows of K and of V
+// (cp.async, 16-byte pieces) into its own ring in shared memory, rows padded
+// by 16 bytes, so that ldmatrix reads them without bank conflicts: K as it
+// lies (a lane's 4 bytes of row lane / 4), V transposed (a pair of rows).
+// For int8 the transposed element is a pair of codes, which one byte permute
+// each turns into two operands. Copies in flight cost no registers, and
+// warps wait for nothing but their own copies.
 #pragma once
 
 #include "paged.cuh"
@@ -42,25 +42,35 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// BYTES (4, 8 or 16) into the lane's slot; 16 bypass L1: the cache is read once.
-template <int BYTES>
-__device__ __forceinline__ void pm_copy(unsigned dst, const void *src) {
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+__device__ __forceinline__ void pm_copy16(unsigned dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-template <int BYTES>
-__device__ __forceinline__ void pm_read(uint32_t *d, unsigned src) {
-  if constexpr (BYTES == 16)
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+__device__ __forceinline__ void pm_copy4(unsigned dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// Four 8x8 matrices of 16-bit elements; lane 8 m + i gives row i of matrix m.
+template <bool TRANS>
+__device__ __forceinline__ void pm_ldmatrix(uint32_t *d, unsigned src) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
                  : "r"(src)
                  : "memory");
-  else if constexpr (BYTES == 8)
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "r"(src) : "memory");
   else
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(d[0]) : "r"(src) : "memory");
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(src)
+                 : "memory");
+}
+__device__ __forceinline__ float2 pm_read2(unsigned src) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(src) : "memory");
+  return v;
+}
+__device__ __forceinline__ float pm_read1(unsigned src) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(src) : "memory");
+  return v;
 }
 
 // Two f16 from two biased codes (code ^ 0x80) in bytes i and j of x: 1024 +
@@ -92,62 +102,73 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t &t0, uint3
   t2 = __byte_perm(__float_as_uint(xs), __float_as_uint(ys), 0x7632);
 }
 
-// How a lane's bytes of a row map to dimensions. K: runs of 4 kCk bytes, a
-// lane's piece t; V: runs of 8 kCv bytes, piece g.
 enum { PM_I8 = 0, PM_BF16 = 1, PM_F32 = 2 };
 template <int KIND, int D>
 struct PmShape {
   static constexpr int kEs = KIND == PM_I8 ? 1 : KIND == PM_BF16 ? 2 : 4;
-  static constexpr int kRow = D * kEs;
-  static constexpr int kKb = kRow / 4, kVb = kRow / 8;  // a lane's bytes of a K / V row
-  static constexpr int kCk = kKb % 16 == 0 ? 16 : 8;
-  static constexpr int kCv = kVb % 16 == 0 ? 16 : (kVb % 8 == 0 ? 8 : 4);
-  static constexpr int kNk = kKb / kCk, kNv = kVb / kCv;  // pieces
-  static constexpr int kSteps = D / 16;
-  // a stage of a warp's ring: two K rows, four V rows and (int8) the scales
-  // of four positions for keys and values, of each lane
-  static constexpr int kStage = 32 * (2 * kKb + 4 * kVb + (KIND == PM_I8 ? 32 : 0));
-  // stages: about 3 KB or more in flight per warp
+  static constexpr int kRow = D * kEs, kNc = kRow / 16;  // bytes and 16-byte pieces of a row
+  static constexpr int kPad = kRow + 16;                 // a row in the ring: an odd number of pieces
+  static constexpr int kSteps = D / 16, kNt = D / 8;
+  // a stage of a warp's ring: 16 rows of K, 16 of V, and (int8) their scales
+  static constexpr int kVat = 16 * kPad, kSat = 32 * kPad, kStage = kSat + (KIND == PM_I8 ? 128 : 0);
+  // stages: one read, the others in flight, 5 KB or more per warp
   static constexpr int kStages = kStage <= 2048 ? 4 : kStage <= 4096 ? 3 : 2;
-  static __device__ __forceinline__ int kdim(int x, int t) {  // dimension of a lane's x-th K element
-    constexpr int E = kCk / kEs;
-    return (x / E * 4 + t) * E + x % E;
+  // Dimension of a lane's element u of the operand of step k: where ldmatrix
+  // puts 4 codes, a pair of bfloat16 twice, or a float32 four times.
+  static __device__ __forceinline__ int kdim(int k, int u, int t) {
+    return 16 * k + (KIND == PM_I8 ? 4 * t + u : KIND == PM_BF16 ? (u >> 1) * 8 + 2 * t + (u & 1) : 4 * u + t);
   }
-  static __device__ __forceinline__ int vdim(int x, int g) {
-    constexpr int E = kCv / kEs;
-    return (x / E * 8 + g) * E + x % E;
+  // Dimension of column c of output tile j.
+  static __device__ __forceinline__ int vdim(int j, int c) {
+    return KIND == PM_I8 ? (j >> 1) * 16 + 2 * c + (j & 1) : 8 * j + c;
   }
 };
 
 // Dynamic shared memory: the rows of the tiles (page_size % 16 == 0) or of
 // every position of a chunk; then the rings, and in their place, at the end,
-// the warps' states.
+// the warps' states, and the join's factors.
+constexpr int kPmJoin = 256;  // chunks whose factors the join holds at a time
 __host__ __device__ inline int pm_rows_bytes(int chunk, bool fast) { return ((fast ? chunk / 16 : chunk) * 4 + 15) / 16 * 16; }
 template <int KIND, int D, int W>
 __host__ __device__ inline size_t pm_smem(int chunk, bool fast) {
   typedef PmShape<KIND, D> Sh;
-  const size_t ring = (size_t)W * Sh::kStages * Sh::kStage, join = (size_t)W * 8 * (D + 2) * 4;
-  return pm_rows_bytes(chunk, fast) + (ring > join ? ring : join);
+  const size_t ring = (size_t)W * Sh::kStages * Sh::kStage, join = (size_t)W * 8 * (D + 2) * 4, fac = 8 * kPmJoin * 4;
+  const size_t most = ring > join ? ring : join;
+  return pm_rows_bytes(chunk, fast) + (most > fac ? most : fac);
 }
 
-// One CTA: one unit (sequence, kv head, up to 8 of its query heads) and one
+// x, y as three bf16 terms in the operand rows of a unit with at most 4
+// heads: rows 0-3 (lanes g < 4) the first, rows 4-7 (the other lanes, which
+// hold the same x, y) the second, rows 8-11 the third.
+__device__ __forceinline__ void split_bf16_rows(float x, float y, bool low, uint32_t &top, uint32_t &bottom) {
+  uint32_t t0, t1, t2;
+  split_bf16(x, y, t0, t1, t2);
+  top = low ? t0 : t1;
+  bottom = low ? t2 : 0u;
+}
+
+// One CTA: one unit (sequence, kv head, up to NH of its query heads) and one
 // chunk of positions, tiles of 16 dealt to the W warps. FAST: page_size is a
-// multiple of 16, a tile lies in one page. The chunks of a unit write their
-// sums to a.part; the last to arrive joins them in chunk order (so the bits
-// do not depend on the order of arrival) and leaves its ticket zero.
+// multiple of 16, a tile lies in one page. NH 4 (bfloat16 and float32): the
+// three terms of 4 heads fill 12 of the 16 rows, one product where 8 heads
+// need two. The chunks of a unit write their sums to a.part; the last to
+// arrive joins them in chunk order (so the bits do not depend on the order
+// of arrival) and leaves its ticket zero.
 // grid n_seqs * n_kv_head * head_chunks * splits.
-template <int KIND, int D, bool FAST, int W>
+template <int KIND, int D, int NH, bool FAST, int W>
 __global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
   typedef PmShape<KIND, D> Sh;
-  constexpr bool I8 = KIND == PM_I8;
-  constexpr int NT = D / 8, S = Sh::kStages;
+  constexpr bool I8 = KIND == PM_I8, TWO = !I8 && NH == 8;  // TWO: the third terms are a second product
+  constexpr int NT = Sh::kNt, S = Sh::kStages, NC = Sh::kNc;
   extern __shared__ __align__(16) char smem[];
   __shared__ int s_last;
+  __shared__ float s_stat[8][2];
   const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
   const int hc = unit % a.head_chunks, kh = unit / a.head_chunks % a.c.n_kv_head;
   const int b = unit / a.head_chunks / a.c.n_kv_head;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int G = a.n_head / a.c.n_kv_head, h0 = kh * G + hc * 8, nh = min(8, G - hc * 8);
+  const int G = a.n_head / a.c.n_kv_head, h0 = kh * G + hc * NH, nh = min(NH, G - hc * NH);
+  const int gh = NH == 4 ? g & 3 : g;  // the lane's head
   const int len = paged_len(a, b), ps = a.c.page_size;
   const int ns = max(1, (len + a.chunk - 1) / a.chunk);
   if (split >= ns) return;
@@ -168,17 +189,19 @@ __global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
   }
 
   // the query's operand, kept for the whole chunk
-  uint32_t qa[Sh::kSteps][4], qb[I8 ? 1 : Sh::kSteps][2];
+  uint32_t qa[Sh::kSteps][4], qb[TWO ? Sh::kSteps : 1][2];
   float fs = a.scale2;
   {
-    float x[D / 4];
-    const float *q = a.q + (size_t)b * a.q_stride + (size_t)(h0 + g) * D;
+    float x[Sh::kSteps][4];
+    const float *q = a.q + (size_t)b * a.q_stride + (size_t)(h0 + gh) * D;
     float mx = 0.0f;
 #pragma unroll
-    for (int i = 0; i < D / 4; i++) {
-      x[i] = g < nh ? q[Sh::kdim(i, t)] : 0.0f;
-      mx = fmaxf(mx, fabsf(x[i]));
-    }
+    for (int k = 0; k < Sh::kSteps; k++)
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        x[k][u] = gh < nh ? q[Sh::kdim(k, u, t)] : 0.0f;
+        mx = fmaxf(mx, fabsf(x[k][u]));
+      }
     if constexpr (I8) {
       // the largest |q| of the head to [2^13, 2^14): the second terms reach 2^-38 of it
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -186,67 +209,57 @@ __global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
       const int e = min(max((int)(__float_as_uint(mx) >> 23), 1), 254) - 127;
       const float up = pow2i(min(13 - e, 126));
 #pragma unroll
-      for (int i = 0; i < D / 4; i++) x[i] *= up;
+      for (int k = 0; k < Sh::kSteps; k++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) x[k][u] *= up;
       fs = a.scale2 * pow2i(max(e - 13, -126));
     }
 #pragma unroll
-    for (int k = 0; k < Sh::kSteps; k++) {
-      if constexpr (I8) {
-        split_f16(x[4 * k], x[4 * k + 1], qa[k][0], qa[k][1]);
-        split_f16(x[4 * k + 2], x[4 * k + 3], qa[k][2], qa[k][3]);
-      } else {
-        split_bf16(x[4 * k], x[4 * k + 1], qa[k][0], qa[k][1], qb[k][0]);
-        split_bf16(x[4 * k + 2], x[4 * k + 3], qa[k][2], qa[k][3], qb[k][1]);
+    for (int k = 0; k < Sh::kSteps; k++)
+#pragma unroll
+      for (int u = 0; u < 4; u += 2) {
+        if constexpr (I8)
+          split_f16(x[k][u], x[k][u + 1], qa[k][u], qa[k][u + 1]);
+        else if constexpr (TWO)
+          split_bf16(x[k][u], x[k][u + 1], qa[k][u], qa[k][u + 1], qb[k][u / 2]);
+        else
+          split_bf16_rows(x[k][u], x[k][u + 1], g < 4, qa[k][u], qa[k][u + 1]);
       }
-    }
   }
   if constexpr (W > 1)
     __syncthreads();
   else
     __syncwarp();
 
-  // the lane's first bytes in the pool, and its slots
   const size_t first = a.c.row(a.layer, 0, kh, 0);
-  const char *kl = (const char *)a.c.k + first * Sh::kRow + t * Sh::kCk + (FAST ? g * Sh::kRow : 0);
-  const char *vl = (const char *)a.c.v + first * Sh::kRow + g * Sh::kCv + (FAST ? 2 * t * Sh::kRow : 0);
-  const float *ksl = I8 ? a.c.ks + first + (FAST ? 2 * t : 0) : nullptr;
-  const float *vsl = I8 ? a.c.vs + first + (FAST ? 2 * t : 0) : nullptr;
+  const char *kl = (const char *)a.c.k + first * Sh::kRow, *vl = (const char *)a.c.v + first * Sh::kRow;
   const unsigned ring = (unsigned)__cvta_generic_to_shared(pool) + warp * (S * Sh::kStage);
-  constexpr int kVat = 64 * Sh::kKb, kSat = kVat + 128 * Sh::kVb;  // a stage: K, V, scales
   auto pos_of = [&](int i) { return (i >> 1) * 8 + 2 * t + (i & 1); };  // the lane's position i of a tile
   auto issue = [&](int tile, int stage) {
     const unsigned d = ring + stage * Sh::kStage;
-    const int base = FAST ? max(rows[tile], 0) : 0;
+    const size_t base = FAST ? (size_t)max(rows[tile], 0) : 0;
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-      const char *p = FAST ? kl + (size_t)base * Sh::kRow + r * 8 * Sh::kRow
-                           : kl + (size_t)max(rows[tile * 16 + 8 * r + g], 0) * Sh::kRow;
-#pragma unroll
-      for (int i = 0; i < Sh::kNk; i++)
-        pm_copy<Sh::kCk>(d + (r * Sh::kNk + i) * 32 * Sh::kCk + lane * Sh::kCk, p + i * 4 * Sh::kCk);
+    for (int i = 0; i < NC / 2; i++) {  // 16 NC pieces of K, and of V, 32 at a time
+      const int p = i * 32 + lane, r = p / NC, c = p % NC;
+      const size_t off = FAST ? base * Sh::kRow + p * 16 : (size_t)max(rows[tile * 16 + r], 0) * Sh::kRow + c * 16;
+      const unsigned at = d + r * Sh::kPad + c * 16;
+      pm_copy16(at, kl + off);
+      pm_copy16(at + Sh::kVat, vl + off);
     }
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int row = FAST ? base : max(rows[tile * 16 + pos_of(r)], 0);
-      const char *p = vl + (size_t)row * Sh::kRow + (FAST ? ((r >> 1) * 8 + (r & 1)) * Sh::kRow : 0);
-#pragma unroll
-      for (int i = 0; i < Sh::kNv; i++)
-        pm_copy<Sh::kCv>(d + kVat + (r * Sh::kNv + i) * 32 * Sh::kCv + lane * Sh::kCv, p + i * 8 * Sh::kCv);
-      if constexpr (I8) {
-        const unsigned sd = d + kSat + lane * 8 + (r >> 1) * 256;
-        if constexpr (FAST) {
-          if (r % 2 == 0) {
-            pm_copy<8>(sd, ksl + (size_t)row + (r >> 1) * 8);
-            pm_copy<8>(sd + 512, vsl + (size_t)row + (r >> 1) * 8);
-          }
-        } else {
-          pm_copy<4>(sd + (r & 1) * 4, ksl + row);
-          pm_copy<4>(sd + 512 + (r & 1) * 4, vsl + row);
-        }
+    if constexpr (I8) {
+      if constexpr (FAST) {
+        if (lane < 8) pm_copy16(d + Sh::kSat + lane * 16, (lane < 4 ? a.c.ks : a.c.vs) + first + base + (lane & 3) * 4);
+      } else {
+        pm_copy4(d + Sh::kSat + lane * 4, (lane < 16 ? a.c.ks : a.c.vs) + first + max(rows[tile * 16 + (lane & 15)], 0));
       }
     }
   };
   auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  // ldmatrix: lane 8 m + i names row i of matrix m. K: matrix = (n-tile, piece), V: (half of the rows, piece)
+  auto matrix_at = [&](int i) {
+    const int mt = 4 * i + (lane >> 3);
+    return (mt / NC * 8 + (lane & 7)) * Sh::kPad + mt % NC * 16;
+  };
 
   float acc[NT][4];
 #pragma unroll
@@ -263,65 +276,73 @@ __global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
   int stage = 0;
   for (int tile = warp; tile < ntiles; tile += W) {
     asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+    __syncwarp();  // every lane's copies of this tile; and every lane is done with the stage that is filled next
     if (tile + (S - 1) * W < ntiles) issue(tile + (S - 1) * W, stage == 0 ? S - 1 : stage - 1);
     commit();
     const unsigned src = ring + stage * Sh::kStage;
     stage = stage == S - 1 ? 0 : stage + 1;
     // scores of 16 positions: two n-tiles of 8
-    float c[2][4];
+    float c[2][4], c2[2][4];
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
+    for (int r = 0; r < 2; r++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) c[r][i] = 0.0f;
-      uint32_t kr[Sh::kKb / 4];
+      for (int i = 0; i < 4; i++) c[r][i] = c2[r][i] = 0.0f;
+    uint32_t kr[2 * NC];
 #pragma unroll
-      for (int i = 0; i < Sh::kNk; i++)
-        pm_read<Sh::kCk>(kr + i * (Sh::kCk / 4), src + (r * Sh::kNk + i) * 32 * Sh::kCk + lane * Sh::kCk);
+    for (int i = 0; i < NC / 2; i++) pm_ldmatrix<false>(kr + 4 * i, src + matrix_at(i));
 #pragma unroll
-      for (int k = 0; k < Sh::kSteps; k++) {
+    for (int k = 0; k < Sh::kSteps; k++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const uint32_t *x = kr + r * NC;
         if constexpr (KIND == PM_I8) {
-          const uint32_t x = kr[k] ^ 0x80808080u;
-          mma_f16(c[r], qa[k], codes_f16(x, 0x4140), codes_f16(x, 0x4342));
+          const uint32_t y = x[k] ^ 0x80808080u;
+          mma_f16(c[r], qa[k], codes_f16(y, 0x4140), codes_f16(y, 0x4342));
+        } else if constexpr (KIND == PM_BF16) {
+          mma_bf16(c[r], qa[k], x[2 * k], x[2 * k + 1]);
+          if constexpr (TWO) {
+            const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
+            mma_bf16(c2[r], q2, x[2 * k], x[2 * k + 1]);
+          }
         } else {
-          const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
-          if constexpr (KIND == PM_BF16) {
-            mma_bf16(c[r], qa[k], kr[2 * k], kr[2 * k + 1]);
-            mma_bf16(c[r], q2, kr[2 * k], kr[2 * k + 1]);
-          } else {
-            uint32_t x[3], y[3];
-            split_bf16(__uint_as_float(kr[4 * k]), __uint_as_float(kr[4 * k + 1]), x[0], x[1], x[2]);
-            split_bf16(__uint_as_float(kr[4 * k + 2]), __uint_as_float(kr[4 * k + 3]), y[0], y[1], y[2]);
-            mma_bf16(c[r], q2, x[0], y[0]);
-#pragma unroll
-            for (int i = 2; i >= 0; i--) mma_bf16(c[r], qa[k], x[i], y[i]);
+          uint32_t y[3], z[3];
+          split_bf16(__uint_as_float(x[4 * k]), __uint_as_float(x[4 * k + 1]), y[0], y[1], y[2]);
+          split_bf16(__uint_as_float(x[4 * k + 2]), __uint_as_float(x[4 * k + 3]), z[0], z[1], z[2]);
+          mma_bf16(c2[r], qa[k], y[2], z[2]);
+          mma_bf16(c2[r], qa[k], y[1], z[1]);
+          mma_bf16(c[r], qa[k], y[0], z[0]);
+          if constexpr (TWO) {
+            const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
+            mma_bf16(c2[r], q2, y[0], z[0]);
           }
         }
       }
-    }
     float s[4], sv[4];
-    if constexpr (I8) {
-      uint32_t ks[4], vs[4];
-      pm_read<8>(ks, src + kSat + lane * 8);
-      pm_read<8>(ks + 2, src + kSat + 256 + lane * 8);
-      pm_read<8>(vs, src + kSat + 512 + lane * 8);
-      pm_read<8>(vs + 2, src + kSat + 768 + lane * 8);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        s[i] = (c[i >> 1][i & 1] + c[i >> 1][2 + (i & 1)]) * fs * __uint_as_float(ks[i]);
-        sv[i] = __uint_as_float(vs[i]);
+    for (int i = 0; i < 4; i++) {
+      const int r = i >> 1, e = i & 1;
+      if constexpr (I8) {
+        s[i] = c[r][e] + c[r][2 + e];
+      } else {
+        s[i] = c[r][e] + (c[r][2 + e] + (c2[r][e] + c2[r][2 + e]));
+        if constexpr (NH == 4) s[i] += __shfl_xor_sync(0xffffffffu, s[i], 16);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; i++) s[i] = (c[i >> 1][i & 1] + c[i >> 1][2 + (i & 1)]) * fs;
+      s[i] *= fs;
+    }
+    if constexpr (I8) {
+      const float2 k0 = pm_read2(src + Sh::kSat + t * 8), k1 = pm_read2(src + Sh::kSat + 32 + t * 8);
+      const float2 v0 = pm_read2(src + Sh::kSat + 64 + t * 8), v1 = pm_read2(src + Sh::kSat + 96 + t * 8);
+      s[0] *= k0.x, s[1] *= k0.y, s[2] *= k1.x, s[3] *= k1.y;
+      sv[0] = v0.x, sv[1] = v0.y, sv[2] = v1.x, sv[3] = v1.y;
     }
     // positions past the end or without a page: no score, and a zero value
     // (0 times what is there might be NaN)
-    unsigned masked = 0;
+    unsigned live = 0xfu;
     if (!FAST || tile * 16 + 16 > n || rows[tile] < 0) {
 #pragma unroll
       for (int i = 0; i < 4; i++)
         if (tile * 16 + pos_of(i) >= n || rows[FAST ? tile : tile * 16 + pos_of(i)] < 0) {
-          masked |= 1u << i;
+          live &= ~(1u << i);
           s[i] = -INFINITY;
           sv[i] = 0.0f;
         }
@@ -369,60 +390,58 @@ __global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
       l += p[i];
     }
     uint32_t pa[4], pb[4] = {0u, 0u, 0u, 0u};
-    if constexpr (I8) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) p[i] *= sv[i] * vinv;
-      split_f16(p[0], p[1], pa[0], pa[1]);
-      split_f16(p[2], p[3], pa[2], pa[3]);
-    } else {
-      split_bf16(p[0], p[1], pa[0], pa[1], pb[0]);
-      split_bf16(p[2], p[3], pa[2], pa[3], pb[2]);
+    for (int i = 0; i < 4; i += 2) {
+      if constexpr (I8)
+        split_f16(p[i] * (sv[i] * vinv), p[i + 1] * (sv[i + 1] * vinv), pa[i], pa[i + 1]);
+      else if constexpr (TWO)
+        split_bf16(p[i], p[i + 1], pa[i], pa[i + 1], pb[i]);
+      else
+        split_bf16_rows(p[i], p[i + 1], g < 4, pa[i], pa[i + 1]);
     }
+    if constexpr (KIND != PM_F32) {
+      // operand registers of the rows 0-7 and 8-15: pieces 2 i and 2 i + 1 of both halves at a time
+      const uint32_t z0 = (live & 1u ? 0xffffu : 0u) | (live & 2u ? 0xffff0000u : 0u);
+      const uint32_t z1 = (live & 4u ? 0xffffu : 0u) | (live & 8u ? 0xffff0000u : 0u);
 #pragma unroll
-    for (int i = 0; i < Sh::kNv; i++) {
-      constexpr int kW = Sh::kCv / 4;
-      uint32_t vr[4][kW];
+      for (int i = 0; i < NC / 2; i++) {
+        uint32_t v[4];  // piece 2 i: rows 0-7, 8-15; piece 2 i + 1: rows 0-7, 8-15
+        pm_ldmatrix<true>(v, src + Sh::kVat + ((lane >> 3 & 1) * 8 + (lane & 7)) * Sh::kPad + (2 * i + (lane >> 4)) * 16);
+        if constexpr (I8) {
 #pragma unroll
-      for (int r = 0; r < 4; r++)
-        pm_read<Sh::kCv>(vr[r], src + kVat + (r * Sh::kNv + i) * 32 * Sh::kCv + lane * Sh::kCv);
-      if constexpr (!I8) {
-        if (masked) {
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-#pragma unroll
-            for (int w = 0; w < kW; w++)
-              if (masked >> r & 1u) vr[r][w] = 0u;
+          for (int j = 0; j < 2; j++) {
+            float (*o)[4] = acc + 4 * i + 2 * j;
+            const uint32_t x = v[2 * j] ^ 0x80808080u, y = v[2 * j + 1] ^ 0x80808080u;
+            mma_f16(o[0], pa, codes_f16(x, 0x4240), codes_f16(y, 0x4240));
+            mma_f16(o[1], pa, codes_f16(x, 0x4341), codes_f16(y, 0x4341));
+          }
+        } else {
+          if (live != 0xfu) {
+            v[0] &= z0, v[1] &= z1, v[2] &= z0, v[3] &= z1;
+          }
+          mma_bf16(acc[2 * i], pa, v[0], v[1]);
+          mma_bf16(acc[2 * i + 1], pa, v[2], v[3]);
+          if constexpr (TWO) {
+            mma_bf16(acc[2 * i], pb, v[0], v[1]);
+            mma_bf16(acc[2 * i + 1], pb, v[2], v[3]);
+          }
         }
       }
+    } else {
 #pragma unroll
-      for (int w = 0; w < kW; w++) {
-        if constexpr (KIND == PM_I8) {
-          float (*o)[4] = acc + 4 * (i * kW + w);
-          const uint32_t v0 = vr[0][w] ^ 0x80808080u, v1 = vr[1][w] ^ 0x80808080u, v2 = vr[2][w] ^ 0x80808080u,
-                         v3 = vr[3][w] ^ 0x80808080u;
-          const uint32_t x = __byte_perm(v0, v1, 0x5140), y = __byte_perm(v2, v3, 0x5140);
-          const uint32_t z = __byte_perm(v0, v1, 0x7362), u = __byte_perm(v2, v3, 0x7362);
-          mma_f16(o[0], pa, codes_f16(x, 0x4140), codes_f16(y, 0x4140));
-          mma_f16(o[1], pa, codes_f16(x, 0x4342), codes_f16(y, 0x4342));
-          mma_f16(o[2], pa, codes_f16(z, 0x4140), codes_f16(u, 0x4140));
-          mma_f16(o[3], pa, codes_f16(z, 0x4342), codes_f16(u, 0x4342));
-        } else if constexpr (KIND == PM_BF16) {
-          float (*o)[4] = acc + 2 * (i * kW + w);
-          const uint32_t x0 = __byte_perm(vr[0][w], vr[1][w], 0x5410), x1 = __byte_perm(vr[2][w], vr[3][w], 0x5410);
-          const uint32_t y0 = __byte_perm(vr[0][w], vr[1][w], 0x7632), y1 = __byte_perm(vr[2][w], vr[3][w], 0x7632);
-          mma_bf16(o[0], pa, x0, x1);
-          mma_bf16(o[1], pa, y0, y1);
-          mma_bf16(o[0], pb, x0, x1);
-          mma_bf16(o[1], pb, y0, y1);
-        } else {
-          float (&o)[4] = acc[i * kW + w];
-          uint32_t x[3], y[3];
-          split_bf16(__uint_as_float(vr[0][w]), __uint_as_float(vr[1][w]), x[0], x[1], x[2]);
-          split_bf16(__uint_as_float(vr[2][w]), __uint_as_float(vr[3][w]), y[0], y[1], y[2]);
-          mma_bf16(o, pb, x[0], y[0]);
+      for (int j = 0; j < NT; j++) {
+        float v[4];
 #pragma unroll
-          for (int k = 2; k >= 0; k--) mma_bf16(o, pa, x[k], y[k]);
+        for (int i = 0; i < 4; i++) {
+          v[i] = pm_read1(src + Sh::kVat + pos_of(i) * Sh::kPad + (8 * j + g) * 4);
+          if (!(live >> i & 1u)) v[i] = 0.0f;
         }
+        uint32_t x[3], y[3];
+        split_bf16(v[0], v[1], x[0], x[1], x[2]);
+        split_bf16(v[2], v[3], y[0], y[1], y[2]);
+        if constexpr (TWO) mma_bf16(acc[j], pb, x[0], y[0]);
+#pragma unroll
+        for (int k = 2; k >= 0; k--) mma_bf16(acc[j], pa, x[k], y[k]);
       }
     }
   }
@@ -430,19 +449,24 @@ __global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
   // join the warps: [warp][head][D sums, M, L] in the rings' place
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   float *join = (float *)pool;
-  if constexpr (W > 1) __syncthreads();
-  else __syncwarp();
+  if constexpr (W > 1)
+    __syncthreads();
+  else
+    __syncwarp();
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
-  if (g < nh) {
-    float *o = join + (warp * 8 + g) * (D + 2);
+  {
+    float *o = join + (warp * 8 + gh) * (D + 2);
     const float f = I8 ? vlim * 0x1p-15f : 1.0f;
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-      o[Sh::vdim(j, 2 * t)] = (acc[j][0] + acc[j][2]) * f;
-      o[Sh::vdim(j, 2 * t + 1)] = (acc[j][1] + acc[j][3]) * f;
-    }
-    if (t == 0) {
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float x = acc[j][e] + acc[j][2 + e];
+        if constexpr (NH == 4) x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (g < nh) o[Sh::vdim(j, 2 * t + e)] = x * f;
+      }
+    if (g < nh && t == 0) {
       o[D] = m;
       o[D + 1] = l;
     }
@@ -471,7 +495,7 @@ __global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
         a.stat[2 * ((size_t)b * a.n_head + h0 + h) + 1] = L;
       }
     } else {
-      float *part = a.part + (((size_t)unit * a.splits + split) * 8 + h) * (D + 2);
+      float *part = a.part + (((size_t)unit * a.splits + split) * NH + h) * (D + 2);
       part[d] = x;
       if (d == 0) {
         part[D] = M;
@@ -486,21 +510,57 @@ __global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  for (int i = tid; i < nh * D; i += W * 32) {
-    const int h = i / D, d = i % D;
-    const float *part = a.part + ((size_t)unit * a.splits * 8 + h) * (D + 2);
-    float M = -INFINITY, L = 0.0f, x = 0.0f;
-    for (int k = 0; k < ns; k++) M = fmaxf(M, __ldcg(part + (size_t)k * 8 * (D + 2) + D));
+  // the unit's chunks: M and L of each head, then the sums, the chunks'
+  // factors 2^(M_k - M) a block of kPmJoin at a time in shared memory
+  const float *part = a.part + (size_t)unit * a.splits * NH * (D + 2);
+  constexpr int kStep = NH * (D + 2);
+  float *fac = (float *)pool;  // [head][kPmJoin]
+  for (int h = warp; h < nh; h += W) {
+    float M = -INFINITY, L = 0.0f;
+    for (int k = lane; k < ns; k += 32) M = fmaxf(M, __ldcg(part + (size_t)k * kStep + h * (D + 2) + D));
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float mu = M == -INFINITY ? 0.0f : M;
-    for (int k = 0; k < ns; k++) {
-      const float *o = part + (size_t)k * 8 * (D + 2);
-      const float f = exp2_approx(__ldcg(o + D) - mu);
-      L = fmaf(__ldcg(o + D + 1), f, L);
-      x = fmaf(__ldcg(o + d), f, x);
+    for (int k = lane; k < ns; k += 32) {
+      const float *o = part + (size_t)k * kStep + h * (D + 2) + D;
+      L = fmaf(__ldcg(o + 1), exp2_approx(__ldcg(o) - mu), L);
     }
-    a.out[(size_t)b * a.out_stride + (size_t)(h0 + h) * D + d] = L == 0.0f ? 0.0f : x / L;
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (lane == 0) {
+      s_stat[h][0] = M;
+      s_stat[h][1] = L;
+    }
+  }
+  constexpr int kOwn = (NH * D + W * 32 - 1) / (W * 32);
+  float x[kOwn];
+#pragma unroll
+  for (int u = 0; u < kOwn; u++) x[u] = 0.0f;
+  for (int k0 = 0; k0 < ns; k0 += kPmJoin) {
+    const int nk = min(kPmJoin, ns - k0);
+    __syncthreads();
+    for (int i = tid; i < nh * nk; i += W * 32) {
+      const int h = i / nk, k = i % nk;
+      const float M = s_stat[h][0];
+      fac[h * kPmJoin + k] = exp2_approx(__ldcg(part + (size_t)(k0 + k) * kStep + h * (D + 2) + D) - (M == -INFINITY ? 0.0f : M));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kOwn; u++) {
+      const int i = u * W * 32 + tid, h = i / D, d = i % D;
+      if (h < nh) {
+        const float *o = part + (size_t)k0 * kStep + h * (D + 2) + d;
+#pragma unroll 8
+        for (int k = 0; k < nk; k++) x[u] = fmaf(__ldcg(o + (size_t)k * kStep), fac[h * kPmJoin + k], x[u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kOwn; u++) {
+    const int i = u * W * 32 + tid, h = i / D, d = i % D;
+    if (h >= nh) continue;
+    const float L = s_stat[h][1];
+    a.out[(size_t)b * a.out_stride + (size_t)(h0 + h) * D + d] = L == 0.0f ? 0.0f : x[u] / L;
     if (a.stat && d == 0) {
-      a.stat[2 * ((size_t)b * a.n_head + h0 + h)] = M;
+      a.stat[2 * ((size_t)b * a.n_head + h0 + h)] = s_stat[h][0];
       a.stat[2 * ((size_t)b * a.n_head + h0 + h) + 1] = L;
     }
   }

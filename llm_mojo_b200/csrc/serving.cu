@@ -68,11 +68,11 @@ llmq_status paged_check(llmq_ctx *ctx, const llmq_paged *p, int layer0, int n_la
   return LLMQ_OK;
 }
 
-template <int KIND, int D, int W>
+template <int KIND, int D, int NH, int W>
 cudaError_t launch_attend_w(const AttendArgs &a, unsigned grid, cudaStream_t s) {
   const bool fast = a.c.page_size % 16 == 0;
   const size_t sm = pm_smem<KIND, D, W>(a.chunk, fast);
-  void (*k)(AttendArgs) = fast ? paged_mma_kernel<KIND, D, true, W> : paged_mma_kernel<KIND, D, false, W>;
+  void (*k)(AttendArgs) = fast ? paged_mma_kernel<KIND, D, NH, true, W> : paged_mma_kernel<KIND, D, NH, false, W>;
   if (sm > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute((const void *)k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
     if (e != cudaSuccess) return e;
@@ -82,7 +82,10 @@ cudaError_t launch_attend_w(const AttendArgs &a, unsigned grid, cudaStream_t s) 
 }
 template <int KIND, int D>
 cudaError_t launch_attend_d(const AttendArgs &a, int warps, unsigned grid, cudaStream_t s) {
-  return warps == 1 ? launch_attend_w<KIND, D, 1>(a, grid, s) : launch_attend_w<KIND, D, 4>(a, grid, s);
+  if (KIND != PM_I8 && a.unit_heads == 4)
+    return warps == 1 ? launch_attend_w<KIND, D, KIND == PM_I8 ? 8 : 4, 1>(a, grid, s)
+                      : launch_attend_w<KIND, D, KIND == PM_I8 ? 8 : 4, 4>(a, grid, s);
+  return warps == 1 ? launch_attend_w<KIND, D, 8, 1>(a, grid, s) : launch_attend_w<KIND, D, 8, 4>(a, grid, s);
 }
 template <int KIND>
 cudaError_t launch_attend_k(const AttendArgs &a, int warps, unsigned grid, cudaStream_t s) {
@@ -253,10 +256,11 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   a.scale2 = (float)(scale * 1.4426950408889634);
   const size_t rows = (size_t)n_seqs * n_head;
   const int D = p->v.head_dim, G = n_head / p->v.n_kv_head;
-  a.head_chunks = (G + 7) / 8;
+  a.unit_heads = p->v.kind != LLMQ_KV_QUANT8 && G <= 4 ? 4 : 8;
+  a.head_chunks = (G + a.unit_heads - 1) / a.unit_heads;
   const long long units = (long long)n_seqs * p->v.n_kv_head * a.head_chunks;
   // chunks so that the longest call's CTAs fill the GPU about twice over
-  const int target = getenv("TGT") ? atoi(getenv("TGT")) : 8;
+  const int target = getenv("TGT") ? atoi(getenv("TGT")) : 5;
   const long long want = std::max(1LL, (long long)ctx->num_sms * target / units);
   long long chunk = std::max(64LL, (a.max_len + want - 1) / want);
   chunk = std::max(chunk, (long long)(a.max_len + kMaxSplits - 1) / kMaxSplits);
@@ -266,7 +270,7 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   if (getenv("WARPS")) warps = atoi(getenv("WARPS"));
   const unsigned g = grid1(units * a.splits);
   if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many sequences for one call");
-  const size_t parts = a.splits > 1 ? (size_t)units * a.splits * 8 * (D + 2) : 0;
+  const size_t parts = a.splits > 1 ? (size_t)units * a.splits * a.unit_heads * (D + 2) : 0;
   if (weights_out || parts) {
     ServeWs *ws;
     const size_t floats = parts + (weights_out ? rows * (a.max_len + 2) : 0);
