@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, int tiles)
   const int row = blockIdx.x / tiles, j0 = blockIdx.x % tiles * kEvPos, tid = threadIdx.x;
   const int h = row % a.c.n_kv_head, b = row / a.c.n_kv_head % a.src.n_seqs;
   const int layer = a.layer0 + row / a.c.n_kv_head / a.src.n_seqs, ps = a.c.page_size;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the selection
   if (tid < kEvPos) {
     const int j = j0 + tid, s = j < a.budget ? a.kept[(size_t)row * a.budget + j] : -1;
     from[tid] = -1;

@@ -137,7 +137,8 @@ struct AttendArgs {
   long long q_stride, out_stride;
   const int *lens;
   float scale2;   // scale * log2(e): scores are exponents of two
-  float *scores;  // [n_seqs][n_head][max_len], for the weights; else null
+  float *scores;  // [n_seqs][n_head][score_stride], for the weights; else null
+  int score_stride;  // max_len to a multiple of 4
   float *stat;    // [n_seqs][n_head][2]: the maximum score M and the sum of 2^(score - M)
   // the split over positions (paged_mma.cuh)
   int chunk, splits, head_chunks, unit_heads;
@@ -157,23 +158,50 @@ __device__ __forceinline__ int paged_len(const AttendArgs &a, int b) {
   return max(0, min(min(a.lens[b], a.max_len), (int)min(cap, (long long)INT_MAX)));
 }
 
+// Four floats from j on, of a row of n; VEC: aligned rows.
+template <bool VEC>
+__device__ __forceinline__ float4 row_load4(const float *p, int j, int n) {
+  if (VEC && j + 3 < n) return *(const float4 *)(p + j);
+  return make_float4(p[j], j + 1 < n ? p[j + 1] : 0.0f, j + 2 < n ? p[j + 2] : 0.0f, j + 3 < n ? p[j + 3] : 0.0f);
+}
+
 // weights_out[b][kv head][j] = weights[b][kv head][j] + sum over the kv
 // head's query heads of their softmax weight of position j (0 past the
-// length) for j < n. grid (ceil(n / 256), n_seqs * n_kv_head), 256 threads.
+// length) for j < n: four positions a thread, the heads' scores (which the
+// attention left in L2) in head order. Launched to overlap the attention's
+// end. grid (ceil(n / 1024), n_seqs * n_kv_head), 256 threads.
+template <bool VEC>
 __global__ void __launch_bounds__(256) paged_weights_kernel(AttendArgs a, int n, const float *win, float *wout,
                                                             long long stride) {
-  const int j = blockIdx.x * 256 + threadIdx.x, G = a.n_head / a.c.n_kv_head;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int j = (blockIdx.x * 256 + threadIdx.x) * 4, G = a.n_head / a.c.n_kv_head;
   if (j >= n) return;
   for (int u = blockIdx.y; u < a.t.n_seqs * a.c.n_kv_head; u += gridDim.y) {
-    const int b = u / a.c.n_kv_head, kh = u % a.c.n_kv_head;
-    float w = win ? win[(size_t)u * stride + j] : 0.0f;
-    if (j < paged_len(a, b))
+    const int b = u / a.c.n_kv_head, kh = u % a.c.n_kv_head, len = paged_len(a, b);
+    if (j >= len && win == wout) continue;
+    float4 w = win ? row_load4<VEC>(win + (size_t)u * stride, j, n) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (j < len) {
+      const size_t r0 = (size_t)b * a.n_head + kh * G;
+#pragma unroll 4
       for (int g = 0; g < G; g++) {
-        const size_t r = (size_t)b * a.n_head + kh * G + g;
-        const float s = a.scores[r * a.max_len + j];
-        if (s != -INFINITY) w += exp2_approx(s - a.stat[2 * r]) / a.stat[2 * r + 1];
+        const float4 s = *(const float4 *)(a.scores + (r0 + g) * a.score_stride + j);
+        const float2 st = *(const float2 *)(a.stat + 2 * (r0 + g));
+        const float M = st.x == -INFINITY ? 0.0f : st.x, inv = st.y > 0.0f ? 1.0f / st.y : st.y;
+        w.x = fmaf(exp2_approx(s.x - M), inv, w.x);
+        if (j + 1 < len) w.y = fmaf(exp2_approx(s.y - M), inv, w.y);
+        if (j + 2 < len) w.z = fmaf(exp2_approx(s.z - M), inv, w.z);
+        if (j + 3 < len) w.w = fmaf(exp2_approx(s.w - M), inv, w.w);
       }
-    wout[(size_t)u * stride + j] = w;
+    }
+    float *o = wout + (size_t)u * stride + j;
+    if (VEC && j + 3 < n) {
+      *(float4 *)o = w;
+    } else {
+      o[0] = w.x;
+      if (j + 1 < n) o[1] = w.y;
+      if (j + 2 < n) o[2] = w.z;
+      if (j + 3 < n) o[3] = w.w;
+    }
   }
 }
 

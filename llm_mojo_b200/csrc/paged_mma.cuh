@@ -74,13 +74,19 @@ __device__ __forceinline__ float pm_read1(unsigned src) {
 }
 
 // Two f16 from two biased codes (code ^ 0x80) in bytes i and j of x: 1024 +
-// byte, less 1152; all exact.
+// byte, less 1152; all exact. For V: its sums nearly cancel, and a bias left
+// in them would cost their low bits.
 __device__ __forceinline__ uint32_t codes_f16(uint32_t x, uint32_t sel) {
   const uint32_t h = __byte_perm(x, 0x64646464u, sel), off = 0x64806480u;
   uint32_t r;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(off));
   return r;
 }
+
+// The same as subnormals, 2^-24 (code + 128). For K: the bias is 128 2^-24
+// times the sum of the query, which the score's accumulator starts from, of
+// the size of the products themselves.
+__device__ __forceinline__ uint32_t codes_sub(uint32_t x, uint32_t sel) { return __byte_perm(x, 0u, sel); }
 
 // x, y as two f16 terms each: hi = (f16 x, f16 y), lo = the rest.
 __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo) {
@@ -102,17 +108,32 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t &t0, uint3
   t2 = __byte_perm(__float_as_uint(xs), __float_as_uint(ys), 0x7632);
 }
 
+// x, y as three bf16 terms in the operand rows of a unit with at most 4
+// heads: rows 0-3 (lanes g < 4) the first, rows 4-7 (the other lanes, which
+// hold the same x, y) the second, rows 8-11 the third.
+__device__ __forceinline__ void split_bf16_rows(float x, float y, bool low, uint32_t &top, uint32_t &bottom) {
+  uint32_t t0, t1, t2;
+  split_bf16(x, y, t0, t1, t2);
+  top = low ? t0 : t1;
+  bottom = low ? t2 : 0u;
+}
+
 enum { PM_I8 = 0, PM_BF16 = 1, PM_F32 = 2 };
-template <int KIND, int D>
+template <int KIND, int D, int W>
 struct PmShape {
   static constexpr int kEs = KIND == PM_I8 ? 1 : KIND == PM_BF16 ? 2 : 4;
   static constexpr int kRow = D * kEs, kNc = kRow / 16;  // bytes and 16-byte pieces of a row
   static constexpr int kPad = kRow + 16;                 // a row in the ring: an odd number of pieces
   static constexpr int kSteps = D / 16, kNt = D / 8;
-  // a stage of a warp's ring: 16 rows of K, 16 of V, and (int8) their scales
-  static constexpr int kVat = 16 * kPad, kSat = 32 * kPad, kStage = kSat + (KIND == PM_I8 ? 128 : 0);
+  // tiles of 16 positions taken together: two while their operands fit in registers
+  static constexpr int kU = kRow <= 128 ? 2 : 1;
+  // a stage of a warp's ring, for each tile: 16 rows of K, 16 of V, and (int8) their scales
+  static constexpr int kVat = 16 * kPad, kSat = 32 * kPad, kTile = kSat + (KIND == PM_I8 ? 128 : 0);
+  static constexpr int kStage = kU * kTile;
   // stages: one read, the others in flight, 5 KB or more per warp
-  static constexpr int kStages = kStage <= 2048 ? 4 : kStage <= 4096 ? 3 : 2;
+  static constexpr int kStages = kStage <= 2560 ? 4 : kStage <= 4096 ? 3 : 2;
+  static constexpr int kBlock = 16 * kU * W;  // positions that the CTA's warps take together
+  static constexpr int kRun = 4096;           // positions whose rows are looked up at a time
   // Dimension of a lane's element u of the operand of step k: where ldmatrix
   // puts 4 codes, a pair of bfloat16 twice, or a float32 four times.
   static __device__ __forceinline__ int kdim(int k, int u, int t) {
@@ -124,27 +145,26 @@ struct PmShape {
   }
 };
 
-// Dynamic shared memory: the rows of the tiles (page_size % 16 == 0) or of
-// every position of a chunk; then the rings, and in their place, at the end,
-// the warps' states, and the join's factors.
-constexpr int kPmJoin = 256;  // chunks whose factors the join holds at a time
-__host__ __device__ inline int pm_rows_bytes(int chunk, bool fast) { return ((fast ? chunk / 16 : chunk) * 4 + 15) / 16 * 16; }
+// Dynamic shared memory: the rows of a run's tiles (page_size % 16 == 0) or
+// of its positions; then the rings, and in their place, at the end, the warps' states, and the join's factors.
+constexpr int kPmJoin = 64;  // partial results whose factors the join holds at a time
 template <int KIND, int D, int W>
-__host__ __device__ inline size_t pm_smem(int chunk, bool fast) {
-  typedef PmShape<KIND, D> Sh;
-  const size_t ring = (size_t)W * Sh::kStages * Sh::kStage, join = (size_t)W * 8 * (D + 2) * 4, fac = 8 * kPmJoin * 4;
-  const size_t most = ring > join ? ring : join;
-  return pm_rows_bytes(chunk, fast) + (most > fac ? most : fac);
+__host__ __device__ constexpr int pm_rows_bytes(bool fast) {
+  return PmShape<KIND, D, W>::kRun / (fast ? 16 : 1) * 4;
+}
+template <int KIND, int D, int W>
+__host__ __device__ constexpr int pm_smem(bool fast) {
+  typedef PmShape<KIND, D, W> Sh;
+  constexpr int ring = W * Sh::kStages * Sh::kStage, join = W * 8 * (D + 2) * 4, fac = 8 * kPmJoin * 4;
+  constexpr int most = ring > join ? ring : join;
+  return pm_rows_bytes<KIND, D, W>(fast) + (most > fac ? most : fac);
 }
 
-// x, y as three bf16 terms in the operand rows of a unit with at most 4
-// heads: rows 0-3 (lanes g < 4) the first, rows 4-7 (the other lanes, which
-// hold the same x, y) the second, rows 8-11 the third.
-__device__ __forceinline__ void split_bf16_rows(float x, float y, bool low, uint32_t &top, uint32_t &bottom) {
-  uint32_t t0, t1, t2;
-  split_bf16(x, y, t0, t1, t2);
-  top = low ? t0 : t1;
-  bottom = low ? t2 : 0u;
+// CTAs of 4 warps per SM that registers are held down for: 96, 128, 168 or
+// 255 a thread, as the accumulators and the query need.
+constexpr int pm_per_sm(int kind, int D, int NH) {
+  const bool two = kind != PM_I8 && NH == 8;
+  return D == 32 ? 5 : D == 64 ? (two ? 3 : 4) : D == 96 ? (two ? 2 : 3) : two || kind == PM_F32 ? 2 : 3;
 }
 
 // One CTA: one unit (sequence, kv head, up to NH of its query heads) and one
@@ -156,104 +176,33 @@ __device__ __forceinline__ void split_bf16_rows(float x, float y, bool low, uint
 // of arrival) and leaves its ticket zero.
 // grid n_seqs * n_kv_head * head_chunks * splits.
 template <int KIND, int D, int NH, bool FAST, int W>
-__global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
-  typedef PmShape<KIND, D> Sh;
+__global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_mma_kernel(AttendArgs a) {
+  typedef PmShape<KIND, D, W> Sh;
   constexpr bool I8 = KIND == PM_I8, TWO = !I8 && NH == 8;  // TWO: the third terms are a second product
-  constexpr int NT = Sh::kNt, S = Sh::kStages, NC = Sh::kNc;
+  constexpr int NT = Sh::kNt, S = Sh::kStages, NC = Sh::kNc, U = Sh::kU;
   extern __shared__ __align__(16) char smem[];
   __shared__ int s_last;
   __shared__ float s_stat[8][2];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
   const int hc = unit % a.head_chunks, kh = unit / a.head_chunks % a.c.n_kv_head;
   const int b = unit / a.head_chunks / a.c.n_kv_head;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int G = a.n_head / a.c.n_kv_head, h0 = kh * G + hc * NH, nh = min(NH, G - hc * NH);
-  const int gh = NH == 4 ? g & 3 : g;  // the lane's head
-  const int len = paged_len(a, b), ps = a.c.page_size;
-  const int ns = max(1, (len + a.chunk - 1) / a.chunk);
+  const int G = a.n_head / a.c.n_kv_head, ps = a.c.page_size, gh = NH == 4 ? g & 3 : g;  // gh: the lane's head
+  const int h0 = kh * G + hc * NH, nh = min(NH, G - hc * NH);
+  const int len = paged_len(a, b), ns = max(1, (len + a.chunk - 1) / a.chunk);
   if (split >= ns) return;
-  const int c0 = split * a.chunk, n = min(len - c0, a.chunk);  // the chunk's positions
-  const int ntiles = (n + 15) / 16;
+  const int p0 = split * a.chunk, p1 = min(len, p0 + a.chunk);  // the chunk's positions
   int *rows = (int *)smem;
-  char *pool = smem + pm_rows_bytes(a.chunk, FAST);
+  char *pool = smem + pm_rows_bytes<KIND, D, W>(FAST);
+  auto sync = [] {
+    if constexpr (W > 1)
+      __syncthreads();
+    else
+      __syncwarp();
+  };
 
-  // rows of the chunk, relative to this layer's and kv head's first; -1: no page
-  for (int i = tid; i < (FAST ? ntiles : ntiles * 16); i += W * 32) {
-    const int j = FAST ? i * 16 : i;
-    int row = -1;
-    if (j < n) {
-      const int pi = (c0 + j) / ps, page = a.t.page(b, pi);
-      if (page >= 0 && page < a.c.n_pages) row = page * (a.c.n_kv_head * ps) + (c0 + j - pi * ps);
-    }
-    rows[i] = row;
-  }
-
-  // the query's operand, kept for the whole chunk
-  uint32_t qa[Sh::kSteps][4], qb[TWO ? Sh::kSteps : 1][2];
-  float fs = a.scale2;
-  {
-    float x[Sh::kSteps][4];
-    const float *q = a.q + (size_t)b * a.q_stride + (size_t)(h0 + gh) * D;
-    float mx = 0.0f;
-#pragma unroll
-    for (int k = 0; k < Sh::kSteps; k++)
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        x[k][u] = gh < nh ? q[Sh::kdim(k, u, t)] : 0.0f;
-        mx = fmaxf(mx, fabsf(x[k][u]));
-      }
-    if constexpr (I8) {
-      // the largest |q| of the head to [2^13, 2^14): the second terms reach 2^-38 of it
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const int e = min(max((int)(__float_as_uint(mx) >> 23), 1), 254) - 127;
-      const float up = pow2i(min(13 - e, 126));
-#pragma unroll
-      for (int k = 0; k < Sh::kSteps; k++)
-#pragma unroll
-        for (int u = 0; u < 4; u++) x[k][u] *= up;
-      fs = a.scale2 * pow2i(max(e - 13, -126));
-    }
-#pragma unroll
-    for (int k = 0; k < Sh::kSteps; k++)
-#pragma unroll
-      for (int u = 0; u < 4; u += 2) {
-        if constexpr (I8)
-          split_f16(x[k][u], x[k][u + 1], qa[k][u], qa[k][u + 1]);
-        else if constexpr (TWO)
-          split_bf16(x[k][u], x[k][u + 1], qa[k][u], qa[k][u + 1], qb[k][u / 2]);
-        else
-          split_bf16_rows(x[k][u], x[k][u + 1], g < 4, qa[k][u], qa[k][u + 1]);
-      }
-  }
-  if constexpr (W > 1)
-    __syncthreads();
-  else
-    __syncwarp();
-
-  const size_t first = a.c.row(a.layer, 0, kh, 0);
-  const char *kl = (const char *)a.c.k + first * Sh::kRow, *vl = (const char *)a.c.v + first * Sh::kRow;
   const unsigned ring = (unsigned)__cvta_generic_to_shared(pool) + warp * (S * Sh::kStage);
   auto pos_of = [&](int i) { return (i >> 1) * 8 + 2 * t + (i & 1); };  // the lane's position i of a tile
-  auto issue = [&](int tile, int stage) {
-    const unsigned d = ring + stage * Sh::kStage;
-    const size_t base = FAST ? (size_t)max(rows[tile], 0) : 0;
-#pragma unroll
-    for (int i = 0; i < NC / 2; i++) {  // 16 NC pieces of K, and of V, 32 at a time
-      const int p = i * 32 + lane, r = p / NC, c = p % NC;
-      const size_t off = FAST ? base * Sh::kRow + p * 16 : (size_t)max(rows[tile * 16 + r], 0) * Sh::kRow + c * 16;
-      const unsigned at = d + r * Sh::kPad + c * 16;
-      pm_copy16(at, kl + off);
-      pm_copy16(at + Sh::kVat, vl + off);
-    }
-    if constexpr (I8) {
-      if constexpr (FAST) {
-        if (lane < 8) pm_copy16(d + Sh::kSat + lane * 16, (lane < 4 ? a.c.ks : a.c.vs) + first + base + (lane & 3) * 4);
-      } else {
-        pm_copy4(d + Sh::kSat + lane * 4, (lane < 16 ? a.c.ks : a.c.vs) + first + max(rows[tile * 16 + (lane & 15)], 0));
-      }
-    }
-  };
   auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
   // ldmatrix: lane 8 m + i names row i of matrix m. K: matrix = (n-tile, piece), V: (half of the rows, piece)
   auto matrix_at = [&](int i) {
@@ -261,310 +210,430 @@ __global__ void __launch_bounds__(W * 32) paged_mma_kernel(AttendArgs a) {
     return (mt / NC * 8 + (lane & 7)) * Sh::kPad + mt % NC * 16;
   };
 
-  float acc[NT][4];
-#pragma unroll
-  for (int j = 0; j < NT; j++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) acc[j][i] = 0.0f;
-  float m = -INFINITY, l = 0.0f, vlim = 0x1p-100f, vinv = 0x1p115f;
-
-#pragma unroll
-  for (int i = 0; i < S - 1; i++) {
-    if (warp + i * W < ntiles) issue(warp + i * W, i);
-    commit();
-  }
-  int stage = 0;
-  for (int tile = warp; tile < ntiles; tile += W) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
-    __syncwarp();  // every lane's copies of this tile; and every lane is done with the stage that is filled next
-    if (tile + (S - 1) * W < ntiles) issue(tile + (S - 1) * W, stage == 0 ? S - 1 : stage - 1);
-    commit();
-    const unsigned src = ring + stage * Sh::kStage;
-    stage = stage == S - 1 ? 0 : stage + 1;
-    // scores of 16 positions: two n-tiles of 8
-    float c[2][4], c2[2][4];
-#pragma unroll
-    for (int r = 0; r < 2; r++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) c[r][i] = c2[r][i] = 0.0f;
-    uint32_t kr[2 * NC];
-#pragma unroll
-    for (int i = 0; i < NC / 2; i++) pm_ldmatrix<false>(kr + 4 * i, src + matrix_at(i));
-#pragma unroll
-    for (int k = 0; k < Sh::kSteps; k++)
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const uint32_t *x = kr + r * NC;
-        if constexpr (KIND == PM_I8) {
-          const uint32_t y = x[k] ^ 0x80808080u;
-          mma_f16(c[r], qa[k], codes_f16(y, 0x4140), codes_f16(y, 0x4342));
-        } else if constexpr (KIND == PM_BF16) {
-          mma_bf16(c[r], qa[k], x[2 * k], x[2 * k + 1]);
-          if constexpr (TWO) {
-            const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
-            mma_bf16(c2[r], q2, x[2 * k], x[2 * k + 1]);
-          }
-        } else {
-          uint32_t y[3], z[3];
-          split_bf16(__uint_as_float(x[4 * k]), __uint_as_float(x[4 * k + 1]), y[0], y[1], y[2]);
-          split_bf16(__uint_as_float(x[4 * k + 2]), __uint_as_float(x[4 * k + 3]), z[0], z[1], z[2]);
-          mma_bf16(c2[r], qa[k], y[2], z[2]);
-          mma_bf16(c2[r], qa[k], y[1], z[1]);
-          mma_bf16(c[r], qa[k], y[0], z[0]);
-          if constexpr (TWO) {
-            const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
-            mma_bf16(c2[r], q2, y[0], z[0]);
-          }
-        }
-      }
-    float s[4], sv[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int r = i >> 1, e = i & 1;
-      if constexpr (I8) {
-        s[i] = c[r][e] + c[r][2 + e];
-      } else {
-        s[i] = c[r][e] + (c[r][2 + e] + (c2[r][e] + c2[r][2 + e]));
-        if constexpr (NH == 4) s[i] += __shfl_xor_sync(0xffffffffu, s[i], 16);
-      }
-      s[i] *= fs;
-    }
-    if constexpr (I8) {
-      const float2 k0 = pm_read2(src + Sh::kSat + t * 8), k1 = pm_read2(src + Sh::kSat + 32 + t * 8);
-      const float2 v0 = pm_read2(src + Sh::kSat + 64 + t * 8), v1 = pm_read2(src + Sh::kSat + 96 + t * 8);
-      s[0] *= k0.x, s[1] *= k0.y, s[2] *= k1.x, s[3] *= k1.y;
-      sv[0] = v0.x, sv[1] = v0.y, sv[2] = v1.x, sv[3] = v1.y;
-    }
-    // positions past the end or without a page: no score, and a zero value
-    // (0 times what is there might be NaN)
-    unsigned live = 0xfu;
-    if (!FAST || tile * 16 + 16 > n || rows[tile] < 0) {
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (tile * 16 + pos_of(i) >= n || rows[FAST ? tile : tile * 16 + pos_of(i)] < 0) {
-          live &= ~(1u << i);
-          s[i] = -INFINITY;
-          sv[i] = 0.0f;
-        }
-    }
-    if (a.scores && g < nh) {
-      float *out = a.scores + ((size_t)b * a.n_head + h0 + g) * a.max_len + c0 + tile * 16;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (tile * 16 + pos_of(i) < n) out[pos_of(i)] = s[i];
-    }
-    float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    bool grow = mx > m;
-    float vm = 0.0f;
-    if constexpr (I8) {
-      vm = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-      grow = grow || vm > vlim;
-    }
-    if (__any_sync(0xffffffffu, grow)) {
-      const float mn = fmaxf(m, mx);
-      float f = m == -INFINITY ? 0.0f : exp2_approx(m - mn);
-      l *= f;
-      m = mn;
-      if constexpr (I8) {
-        // vlim: a power of two not below any value scale so far
-        for (int o = 16; o > 0; o >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
-        if (vm > vlim) {
-          const float up = __uint_as_float(min((__float_as_uint(vm) & 0x7f800000u) + 0x800000u, 254u << 23));
-          f *= vlim / up;
-          vlim = up;
-          vinv = 0x1p15f / up;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NT; j++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[j][i] *= f;
-    }
-    const float mu = m == -INFINITY ? 0.0f : m;
-    float p[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      p[i] = exp2_approx(s[i] - mu);
-      l += p[i];
-    }
-    uint32_t pa[4], pb[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      if constexpr (I8)
-        split_f16(p[i] * (sv[i] * vinv), p[i + 1] * (sv[i + 1] * vinv), pa[i], pa[i + 1]);
-      else if constexpr (TWO)
-        split_bf16(p[i], p[i + 1], pa[i], pa[i + 1], pb[i]);
-      else
-        split_bf16_rows(p[i], p[i + 1], g < 4, pa[i], pa[i + 1]);
-    }
-    if constexpr (KIND != PM_F32) {
-      // operand registers of the rows 0-7 and 8-15: pieces 2 i and 2 i + 1 of both halves at a time
-      const uint32_t z0 = (live & 1u ? 0xffffu : 0u) | (live & 2u ? 0xffff0000u : 0u);
-      const uint32_t z1 = (live & 4u ? 0xffffu : 0u) | (live & 8u ? 0xffff0000u : 0u);
-#pragma unroll
-      for (int i = 0; i < NC / 2; i++) {
-        uint32_t v[4];  // piece 2 i: rows 0-7, 8-15; piece 2 i + 1: rows 0-7, 8-15
-        pm_ldmatrix<true>(v, src + Sh::kVat + ((lane >> 3 & 1) * 8 + (lane & 7)) * Sh::kPad + (2 * i + (lane >> 4)) * 16);
-        if constexpr (I8) {
-#pragma unroll
-          for (int j = 0; j < 2; j++) {
-            float (*o)[4] = acc + 4 * i + 2 * j;
-            const uint32_t x = v[2 * j] ^ 0x80808080u, y = v[2 * j + 1] ^ 0x80808080u;
-            mma_f16(o[0], pa, codes_f16(x, 0x4240), codes_f16(y, 0x4240));
-            mma_f16(o[1], pa, codes_f16(x, 0x4341), codes_f16(y, 0x4341));
-          }
-        } else {
-          if (live != 0xfu) {
-            v[0] &= z0, v[1] &= z1, v[2] &= z0, v[3] &= z1;
-          }
-          mma_bf16(acc[2 * i], pa, v[0], v[1]);
-          mma_bf16(acc[2 * i + 1], pa, v[2], v[3]);
-          if constexpr (TWO) {
-            mma_bf16(acc[2 * i], pb, v[0], v[1]);
-            mma_bf16(acc[2 * i + 1], pb, v[2], v[3]);
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NT; j++) {
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          v[i] = pm_read1(src + Sh::kVat + pos_of(i) * Sh::kPad + (8 * j + g) * 4);
-          if (!(live >> i & 1u)) v[i] = 0.0f;
-        }
-        uint32_t x[3], y[3];
-        split_bf16(v[0], v[1], x[0], x[1], x[2]);
-        split_bf16(v[2], v[3], y[0], y[1], y[2]);
-        if constexpr (TWO) mma_bf16(acc[j], pb, x[0], y[0]);
-#pragma unroll
-        for (int k = 2; k >= 0; k--) mma_bf16(acc[j], pa, x[k], y[k]);
-      }
-    }
-  }
-
-  // join the warps: [warp][head][D sums, M, L] in the rings' place
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  float *join = (float *)pool;
-  if constexpr (W > 1)
-    __syncthreads();
-  else
-    __syncwarp();
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
   {
-    float *o = join + (warp * 8 + gh) * (D + 2);
-    const float f = I8 ? vlim * 0x1p-15f : 1.0f;
+    // the query's operand, kept for the whole chunk
+    uint32_t qa[Sh::kSteps][4], qb[TWO ? Sh::kSteps : 1][2];
+    float fs = a.scale2, cb0 = 0.0f, cb1 = 0.0f;  // int8: where the scores' two rows start
+    {
+      float x[Sh::kSteps][4];
+      const float *q = a.q + (size_t)b * a.q_stride + (size_t)(h0 + gh) * D;
+      float mx = 0.0f;
+#pragma unroll
+      for (int k = 0; k < Sh::kSteps; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          x[k][e] = gh < nh ? q[Sh::kdim(k, e, t)] : 0.0f;
+          mx = fmaxf(mx, fabsf(x[k][e]));
+        }
+      if constexpr (I8) {
+        // the largest |q| of the head to [2^13, 2^14): the second terms reach 2^-38 of it
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const int e = min(max((int)(__float_as_uint(mx) >> 23), 1), 254) - 127;
+        const float up = pow2i(min(13 - e, 126));
+#pragma unroll
+        for (int k = 0; k < Sh::kSteps; k++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) x[k][i] *= up;
+        fs = a.scale2 * pow2i(max(e - 13, -126)) * 0x1p24f;
+      }
+#pragma unroll
+      for (int k = 0; k < Sh::kSteps; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          if constexpr (I8) {
+            split_f16(x[k][e], x[k][e + 1], qa[k][e], qa[k][e + 1]);
+            const float2 hi = __half22float2(*(const __half2 *)&qa[k][e]);
+            const float2 lo = __half22float2(*(const __half2 *)&qa[k][e + 1]);
+            cb0 += hi.x + hi.y;
+            cb1 += lo.x + lo.y;
+          } else if constexpr (TWO) {
+            split_bf16(x[k][e], x[k][e + 1], qa[k][e], qa[k][e + 1], qb[k][e / 2]);
+          } else {
+            split_bf16_rows(x[k][e], x[k][e + 1], g < 4, qa[k][e], qa[k][e + 1]);
+          }
+        }
+      if constexpr (I8) {
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          cb0 += __shfl_xor_sync(0xffffffffu, cb0, o);
+          cb1 += __shfl_xor_sync(0xffffffffu, cb1, o);
+        }
+        cb0 *= -0x1p-17f;
+        cb1 *= -0x1p-17f;
+      }
+    }
+
+    const size_t first = a.c.row(a.layer, 0, kh, 0);
+    const char *kl = (const char *)a.c.k + first * Sh::kRow, *vl = (const char *)a.c.v + first * Sh::kRow;
+    // int8 scales: a lane's piece of a tile's 16 + 16 (FAST), or of its positions
+    const float *scl = I8 ? (FAST ? (lane < 4 ? a.c.ks : a.c.vs) + first + (lane & 3) * 4
+                                  : (lane < 16 ? a.c.ks : a.c.vs) + first)
+                          : nullptr;
+    float acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; j++)
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        float x = acc[j][e] + acc[j][2 + e];
-        if constexpr (NH == 4) x += __shfl_xor_sync(0xffffffffu, x, 16);
-        if (g < nh) o[Sh::vdim(j, 2 * t + e)] = x * f;
+      for (int i = 0; i < 4; i++) acc[j][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f, vlim = 0x1p-100f, vinv = 0x1p115f;
+
+    for (int c0 = p0; c0 < p1; c0 += Sh::kRun) {
+      const int n = min(p1 - c0, Sh::kRun), ntiles = (n + 15) / 16;  // the run
+      // its rows, relative to this layer's and kv head's first; -1: no page
+      bool hole = false;
+      if (c0 > p0) sync();
+      for (int i = tid; i < (FAST ? ntiles : ntiles * 16); i += W * 32) {
+        const int j = FAST ? i * 16 : i;
+        int row = -1;
+        if (j < n) {
+          const int pi = (c0 + j) / ps, page = a.t.page(b, pi);
+          if (page >= 0 && page < a.c.n_pages)
+            row = page * (a.c.n_kv_head * ps) + (c0 + j - pi * ps);
+          else
+            hole = true;
+        }
+        rows[i] = row;
       }
-    if (g < nh && t == 0) {
-      o[D] = m;
-      o[D + 1] = l;
-    }
-  }
-  if constexpr (W > 1)
-    __syncthreads();
-  else
-    __syncwarp();
-  for (int i = tid; i < nh * D; i += W * 32) {
-    const int h = i / D, d = i % D;
-    const float *o = join + h * (D + 2);
-    float M = -INFINITY, L = 0.0f, x = 0.0f;
+      if constexpr (W > 1)
+        hole = __syncthreads_or(hole);
+      else
+        hole = __any_sync(0xffffffffu, hole);
+
+      auto issue = [&](int tile0, int stage) {  // tiles tile0 .. tile0 + U - 1, as far as there are
 #pragma unroll
-    for (int w = 0; w < W; w++) M = fmaxf(M, o[w * 8 * (D + 2) + D]);
-    const float mu = M == -INFINITY ? 0.0f : M;
+        for (int v = 0; v < U; v++) {
+          const int tile = U == 1 ? tile0 : min(tile0 + v, ntiles - 1);
+          const unsigned d = ring + stage * Sh::kStage + v * Sh::kTile;
+          const size_t at0 = FAST ? (size_t)max(rows[tile], 0) : 0;
 #pragma unroll
-    for (int w = 0; w < W; w++) {
-      const float f = exp2_approx(o[w * 8 * (D + 2) + D] - mu);
-      L = fmaf(o[w * 8 * (D + 2) + D + 1], f, L);
-      x = fmaf(o[w * 8 * (D + 2) + d], f, x);
+          for (int i = 0; i < NC / 2; i++) {  // 16 NC pieces of K, and of V, 32 at a time
+            const int p = i * 32 + lane, r = p / NC, c = p % NC;
+            const size_t off = FAST ? at0 * Sh::kRow + p * 16 : (size_t)max(rows[tile * 16 + r], 0) * Sh::kRow + c * 16;
+            const unsigned at = d + r * Sh::kPad + c * 16;
+            pm_copy16(at, kl + off);
+            pm_copy16(at + Sh::kVat, vl + off);
+          }
+          if constexpr (I8) {
+            if constexpr (FAST) {
+              if (lane < 8) pm_copy16(d + Sh::kSat + lane * 16, scl + at0);
+            } else {
+              pm_copy4(d + Sh::kSat + lane * 4, scl + max(rows[tile * 16 + (lane & 15)], 0));
+            }
+          }
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < S - 1; i++) {
+        if ((warp + i * W) * U < ntiles) issue((warp + i * W) * U, i);
+        commit();
+      }
+      int stage = 0;
+      for (int tile = warp * U; tile < ntiles; tile += W * U) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+        __syncwarp();  // every lane's copies of this tile; and every lane is done with the stage that is filled next
+        if (tile + (S - 1) * W * U < ntiles) issue(tile + (S - 1) * W * U, stage == 0 ? S - 1 : stage - 1);
+        commit();
+        const unsigned src = ring + stage * Sh::kStage;
+        stage = stage == S - 1 ? 0 : stage + 1;
+        float s[U][4], sv[U][4];
+#pragma unroll
+        for (int v = 0; v < U; v++) {
+          // scores of 16 positions: two n-tiles of 8
+          float c[2][4], c2[2][4];
+#pragma unroll
+          for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              c[r][i] = i < 2 ? cb0 : cb1;
+              c2[r][i] = 0.0f;
+            }
+          uint32_t kr[2 * NC];
+#pragma unroll
+          for (int i = 0; i < NC / 2; i++) pm_ldmatrix<false>(kr + 4 * i, src + v * Sh::kTile + matrix_at(i));
+#pragma unroll
+          for (int k = 0; k < Sh::kSteps; k++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+              const uint32_t *x = kr + r * NC;
+              if constexpr (KIND == PM_I8) {
+                const uint32_t y = x[k] ^ 0x80808080u;
+                mma_f16(c[r], qa[k], codes_sub(y, 0x4140), codes_sub(y, 0x4342));
+              } else if constexpr (KIND == PM_BF16) {
+                mma_bf16(c[r], qa[k], x[2 * k], x[2 * k + 1]);
+                if constexpr (TWO) {
+                  const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
+                  mma_bf16(c2[r], q2, x[2 * k], x[2 * k + 1]);
+                }
+              } else {
+                uint32_t y[3], z[3];
+                split_bf16(__uint_as_float(x[4 * k]), __uint_as_float(x[4 * k + 1]), y[0], y[1], y[2]);
+                split_bf16(__uint_as_float(x[4 * k + 2]), __uint_as_float(x[4 * k + 3]), z[0], z[1], z[2]);
+                mma_bf16(c2[r], qa[k], y[2], z[2]);
+                mma_bf16(c2[r], qa[k], y[1], z[1]);
+                mma_bf16(c[r], qa[k], y[0], z[0]);
+                if constexpr (TWO) {
+                  const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
+                  mma_bf16(c2[r], q2, y[0], z[0]);
+                }
+              }
+            }
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int r = i >> 1, e = i & 1;
+            if constexpr (I8) {
+              s[v][i] = c[r][e] + c[r][2 + e];
+            } else {
+              s[v][i] = c[r][e] + (c[r][2 + e] + (KIND == PM_F32 || TWO ? c2[r][e] + c2[r][2 + e] : 0.0f));
+              if constexpr (NH == 4) s[v][i] += __shfl_xor_sync(0xffffffffu, s[v][i], 16);
+            }
+            s[v][i] *= fs;
+          }
+          if constexpr (I8) {
+            const unsigned at = src + v * Sh::kTile + Sh::kSat + t * 8;
+            const float2 x0 = pm_read2(at), x1 = pm_read2(at + 32), v0 = pm_read2(at + 64), v1 = pm_read2(at + 96);
+            s[v][0] *= x0.x, s[v][1] *= x0.y, s[v][2] *= x1.x, s[v][3] *= x1.y;
+            sv[v][0] = v0.x, sv[v][1] = v0.y, sv[v][2] = v1.x, sv[v][3] = v1.y;
+          }
+        }
+        // positions past the end or without a page: no score, and a zero value
+        // (0 times what is there might be NaN)
+        unsigned live = ~0u;
+        if (hole || (tile + U) * 16 > n) {
+#pragma unroll
+          for (int v = 0; v < U; v++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int j = (tile + v) * 16 + pos_of(i);
+              if (j >= n || rows[FAST ? tile + v : j] < 0) {
+                live &= ~(1u << (4 * v + i));
+                s[v][i] = -INFINITY;
+                sv[v][i] = 0.0f;
+              }
+            }
+        }
+        if (a.scores && g < nh) {
+          float *out = a.scores + ((size_t)b * a.n_head + h0 + g) * a.score_stride + c0 + tile * 16;
+#pragma unroll
+          for (int v = 0; v < U; v++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if ((tile + v) * 16 + pos_of(i) < n) out[v * 16 + pos_of(i)] = s[v][i];
+        }
+        float mx = s[0][0], vm = 0.0f;
+#pragma unroll
+        for (int v = 0; v < U; v++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            mx = fmaxf(mx, s[v][i]);
+            if constexpr (I8) vm = fmaxf(vm, sv[v][i]);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (__any_sync(0xffffffffu, mx > m || (I8 && vm > vlim))) {
+          const float mn = fmaxf(m, mx);
+          float f = m == -INFINITY ? 0.0f : exp2_approx(m - mn);
+          l *= f;
+          m = mn;
+          if constexpr (I8) {
+            // vlim: a power of two not below any value scale so far
+            for (int o = 16; o > 0; o >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+            if (vm > vlim) {
+              const float up = __uint_as_float(min((__float_as_uint(vm) & 0x7f800000u) + 0x800000u, 254u << 23));
+              f *= vlim / up;
+              vlim = up;
+              vinv = 0x1p15f / up;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[j][i] *= f;
+        }
+        const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int v = 0; v < U; v++) {
+          const unsigned vat = src + v * Sh::kTile + Sh::kVat;
+          float p[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            p[i] = exp2_approx(s[v][i] - mu);
+            l += p[i];
+          }
+          uint32_t pa[4], pb[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            if constexpr (I8)
+              split_f16(p[i] * (sv[v][i] * vinv), p[i + 1] * (sv[v][i + 1] * vinv), pa[i], pa[i + 1]);
+            else if constexpr (TWO)
+              split_bf16(p[i], p[i + 1], pa[i], pa[i + 1], pb[i]);
+            else
+              split_bf16_rows(p[i], p[i + 1], g < 4, pa[i], pa[i + 1]);
+          }
+          if constexpr (KIND != PM_F32) {
+            // operand registers of the rows 0-7 and 8-15: pieces 2 i and 2 i + 1 of both halves at a time
+#pragma unroll
+            for (int i = 0; i < NC / 2; i++) {
+              uint32_t w[4];  // piece 2 i: rows 0-7, 8-15; piece 2 i + 1: rows 0-7, 8-15
+              pm_ldmatrix<true>(w, vat + ((lane >> 3 & 1) * 8 + (lane & 7)) * Sh::kPad + (2 * i + (lane >> 4)) * 16);
+              if constexpr (I8) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                  float (*o)[4] = acc + 4 * i + 2 * j;
+                  const uint32_t x = w[2 * j] ^ 0x80808080u, y = w[2 * j + 1] ^ 0x80808080u;
+                  mma_f16(o[0], pa, codes_f16(x, 0x4240), codes_f16(y, 0x4240));
+                  mma_f16(o[1], pa, codes_f16(x, 0x4341), codes_f16(y, 0x4341));
+                }
+              } else {
+                if (live != ~0u) {
+                  const unsigned f = live >> (4 * v);
+                  const uint32_t z0 = (f & 1u ? 0xffffu : 0u) | (f & 2u ? 0xffff0000u : 0u);
+                  const uint32_t z1 = (f & 4u ? 0xffffu : 0u) | (f & 8u ? 0xffff0000u : 0u);
+                  w[0] &= z0, w[1] &= z1, w[2] &= z0, w[3] &= z1;
+                }
+                mma_bf16(acc[2 * i], pa, w[0], w[1]);
+                mma_bf16(acc[2 * i + 1], pa, w[2], w[3]);
+                if constexpr (TWO) {
+                  mma_bf16(acc[2 * i], pb, w[0], w[1]);
+                  mma_bf16(acc[2 * i + 1], pb, w[2], w[3]);
+                }
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+              float w[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                w[i] = pm_read1(vat + pos_of(i) * Sh::kPad + (8 * j + g) * 4);
+                if (!(live >> (4 * v + i) & 1u)) w[i] = 0.0f;
+              }
+              uint32_t x[3], y[3];
+              split_bf16(w[0], w[1], x[0], x[1], x[2]);
+              split_bf16(w[2], w[3], y[0], y[1], y[2]);
+              if constexpr (TWO) mma_bf16(acc[j], pb, x[0], y[0]);
+#pragma unroll
+              for (int k = 2; k >= 0; k--) mma_bf16(acc[j], pa, x[k], y[k]);
+            }
+          }
+        }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    if (ns == 1) {
-      a.out[(size_t)b * a.out_stride + (size_t)(h0 + h) * D + d] = L == 0.0f ? 0.0f : x / L;
+
+    // join the warps: [warp][head][D sums, M, L] in the rings' place
+    float *join = (float *)pool;
+    sync();
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    {
+      float *o = join + (warp * 8 + gh) * (D + 2);
+      const float f = I8 ? vlim * 0x1p-15f : 1.0f;
+#pragma unroll
+      for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float x = acc[j][e] + acc[j][2 + e];
+          if constexpr (NH == 4) x += __shfl_xor_sync(0xffffffffu, x, 16);
+          if (g < nh) o[Sh::vdim(j, 2 * t + e)] = x * f;
+        }
+      if (g < nh && t == 0) {
+        o[D] = m;
+        o[D + 1] = l;
+      }
+    }
+    sync();
+    constexpr int kStep = NH * (D + 2);  // floats of a partial result
+    for (int i = tid; i < nh * D; i += W * 32) {
+      const int h = i / D, d = i % D;
+      const float *o = join + h * (D + 2);
+      float M = -INFINITY, L = 0.0f, x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; w++) M = fmaxf(M, o[w * 8 * (D + 2) + D]);
+      const float mu = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+      for (int w = 0; w < W; w++) {
+        const float f = exp2_approx(o[w * 8 * (D + 2) + D] - mu);
+        L = fmaf(o[w * 8 * (D + 2) + D + 1], f, L);
+        x = fmaf(o[w * 8 * (D + 2) + d], f, x);
+      }
+      if (ns == 1) {
+        a.out[(size_t)b * a.out_stride + (size_t)(h0 + h) * D + d] = L == 0.0f ? 0.0f : x / L;
+        if (a.stat && d == 0) {
+          a.stat[2 * ((size_t)b * a.n_head + h0 + h)] = M;
+          a.stat[2 * ((size_t)b * a.n_head + h0 + h) + 1] = L;
+        }
+      } else {
+        float *part = a.part + ((size_t)unit * a.splits + split) * kStep + h * (D + 2);
+        part[d] = x;
+        if (d == 0) {
+          part[D] = M;
+          part[D + 1] = L;
+        }
+      }
+    }
+    if (ns == 1) return;
+    __threadfence();
+    sync();
+    if (tid == 0) s_last = atomicAdd(&a.tickets[unit], 1) == ns - 1;
+    sync();
+    if (!s_last) return;
+    __threadfence();
+    // M and L of each head, then the sums, the parts' factors 2^(M_k - M) a
+    // block of kPmJoin at a time in shared memory
+    const float *part = a.part + (size_t)unit * a.splits * kStep;
+    auto part_of = [&](int k) { return part + (size_t)k * kStep; };
+    float *fac = (float *)pool;  // [head][kPmJoin]
+    for (int h = warp; h < nh; h += W) {
+      float M = -INFINITY, L = 0.0f;
+      for (int k = lane; k < ns; k += 32) M = fmaxf(M, __ldcg(part_of(k) + h * (D + 2) + D));
+      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      const float mu = M == -INFINITY ? 0.0f : M;
+      for (int k = lane; k < ns; k += 32) {
+        const float *o = part_of(k) + h * (D + 2) + D;
+        L = fmaf(__ldcg(o + 1), exp2_approx(__ldcg(o) - mu), L);
+      }
+      for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      if (lane == 0) {
+        s_stat[h][0] = M;
+        s_stat[h][1] = L;
+      }
+    }
+    constexpr int kOwn = (NH * D + W * 32 - 1) / (W * 32);
+    float x[kOwn];
+#pragma unroll
+    for (int e = 0; e < kOwn; e++) x[e] = 0.0f;
+    for (int b0 = 0; b0 < ns; b0 += kPmJoin) {
+      const int nk = min(kPmJoin, ns - b0);
+      sync();
+      for (int i = tid; i < nh * nk; i += W * 32) {
+        const int h = i / nk, k = i % nk;
+        const float M = s_stat[h][0];
+        fac[h * kPmJoin + k] = exp2_approx(__ldcg(part_of(b0 + k) + h * (D + 2) + D) - (M == -INFINITY ? 0.0f : M));
+      }
+      sync();
+#pragma unroll
+      for (int e = 0; e < kOwn; e++) {
+        const int i = e * W * 32 + tid, h = i / D, d = i % D;
+        if (h < nh) {
+#pragma unroll 8
+          for (int k = 0; k < nk; k++)
+            x[e] = fmaf(__ldcg(part_of(b0 + k) + h * (D + 2) + d), fac[h * kPmJoin + k], x[e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kOwn; e++) {
+      const int i = e * W * 32 + tid, h = i / D, d = i % D;
+      if (h >= nh) continue;
+      const float L = s_stat[h][1];
+      a.out[(size_t)b * a.out_stride + (size_t)(h0 + h) * D + d] = L == 0.0f ? 0.0f : x[e] / L;
       if (a.stat && d == 0) {
-        a.stat[2 * ((size_t)b * a.n_head + h0 + h)] = M;
+        a.stat[2 * ((size_t)b * a.n_head + h0 + h)] = s_stat[h][0];
         a.stat[2 * ((size_t)b * a.n_head + h0 + h) + 1] = L;
       }
-    } else {
-      float *part = a.part + (((size_t)unit * a.splits + split) * NH + h) * (D + 2);
-      part[d] = x;
-      if (d == 0) {
-        part[D] = M;
-        part[D + 1] = L;
-      }
     }
+    if (tid == 0) a.tickets[unit] = 0;
   }
-  if (ns == 1) return;
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) s_last = atomicAdd(&a.tickets[unit], 1) == ns - 1;
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  // the unit's chunks: M and L of each head, then the sums, the chunks'
-  // factors 2^(M_k - M) a block of kPmJoin at a time in shared memory
-  const float *part = a.part + (size_t)unit * a.splits * NH * (D + 2);
-  constexpr int kStep = NH * (D + 2);
-  float *fac = (float *)pool;  // [head][kPmJoin]
-  for (int h = warp; h < nh; h += W) {
-    float M = -INFINITY, L = 0.0f;
-    for (int k = lane; k < ns; k += 32) M = fmaxf(M, __ldcg(part + (size_t)k * kStep + h * (D + 2) + D));
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float mu = M == -INFINITY ? 0.0f : M;
-    for (int k = lane; k < ns; k += 32) {
-      const float *o = part + (size_t)k * kStep + h * (D + 2) + D;
-      L = fmaf(__ldcg(o + 1), exp2_approx(__ldcg(o) - mu), L);
-    }
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if (lane == 0) {
-      s_stat[h][0] = M;
-      s_stat[h][1] = L;
-    }
-  }
-  constexpr int kOwn = (NH * D + W * 32 - 1) / (W * 32);
-  float x[kOwn];
-#pragma unroll
-  for (int u = 0; u < kOwn; u++) x[u] = 0.0f;
-  for (int k0 = 0; k0 < ns; k0 += kPmJoin) {
-    const int nk = min(kPmJoin, ns - k0);
-    __syncthreads();
-    for (int i = tid; i < nh * nk; i += W * 32) {
-      const int h = i / nk, k = i % nk;
-      const float M = s_stat[h][0];
-      fac[h * kPmJoin + k] = exp2_approx(__ldcg(part + (size_t)(k0 + k) * kStep + h * (D + 2) + D) - (M == -INFINITY ? 0.0f : M));
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kOwn; u++) {
-      const int i = u * W * 32 + tid, h = i / D, d = i % D;
-      if (h < nh) {
-        const float *o = part + (size_t)k0 * kStep + h * (D + 2) + d;
-#pragma unroll 8
-        for (int k = 0; k < nk; k++) x[u] = fmaf(__ldcg(o + (size_t)k * kStep), fac[h * kPmJoin + k], x[u]);
-      }
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kOwn; u++) {
-    const int i = u * W * 32 + tid, h = i / D, d = i % D;
-    if (h >= nh) continue;
-    const float L = s_stat[h][1];
-    a.out[(size_t)b * a.out_stride + (size_t)(h0 + h) * D + d] = L == 0.0f ? 0.0f : x[u] / L;
-    if (a.stat && d == 0) {
-      a.stat[2 * ((size_t)b * a.n_head + h0 + h)] = s_stat[h][0];
-      a.stat[2 * ((size_t)b * a.n_head + h0 + h) + 1] = L;
-    }
-  }
-  if (tid == 0) a.tickets[unit] = 0;
 }
 
 }  // namespace llmq

@@ -2,6 +2,7 @@
 // and eviction, and the rules on logits (include/llmq.h).
 #include <algorithm>
 #include <climits>
+#include <mutex>
 
 #include "context.cuh"
 #include "evict.cuh"
@@ -56,6 +57,9 @@ llmq_status serve_ws(llmq_ctx *ctx, size_t bytes, size_t tickets, ServeWs **out)
   return LLMQ_OK;
 }
 
+constexpr int kMaxDevices = 64;
+constexpr int kMaxJoin = 128;  // chunks of one unit, which its last CTA joins
+
 int elem_bytes(int kind) { return kind == LLMQ_KV_F32 ? 4 : kind == LLMQ_KV_BF16 ? 2 : 1; }
 
 // What store, attend and evict all check.
@@ -68,38 +72,56 @@ llmq_status paged_check(llmq_ctx *ctx, const llmq_paged *p, int layer0, int n_la
   return LLMQ_OK;
 }
 
-template <int KIND, int D, int NH, int W>
-cudaError_t launch_attend_w(const AttendArgs &a, unsigned grid, cudaStream_t s) {
-  const bool fast = a.c.page_size % 16 == 0;
-  const size_t sm = pm_smem<KIND, D, W>(a.chunk, fast);
-  void (*k)(AttendArgs) = fast ? paged_mma_kernel<KIND, D, NH, true, W> : paged_mma_kernel<KIND, D, NH, false, W>;
-  if (sm > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute((const void *)k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
-    if (e != cudaSuccess) return e;
-  }
-  k<<<grid, W * 32, sm, s>>>(a);
-  return cudaGetLastError();
+// A kernel with its shared memory and how many of its CTAs an SM holds
+// (asked for once per device).
+struct AttendKernel {
+  void (*fn)(AttendArgs) = nullptr;
+  int threads = 0, smem = 0, block = 0, per_sm[kMaxDevices] = {};
+};
+template <int KIND, int D, int NH, bool FAST, int W>
+AttendKernel *attend_kernel_w() {
+  static AttendKernel k = [] {
+    AttendKernel x;
+    x.fn = paged_mma_kernel<KIND, D, NH, FAST, W>;
+    x.threads = W * 32;
+    x.smem = pm_smem<KIND, D, W>(FAST);
+    x.block = PmShape<KIND, D, W>::kBlock;
+    return x;
+  }();
+  return &k;
 }
-template <int KIND, int D>
-cudaError_t launch_attend_d(const AttendArgs &a, int warps, unsigned grid, cudaStream_t s) {
-  if (KIND != PM_I8 && a.unit_heads == 4)
-    return warps == 1 ? launch_attend_w<KIND, D, KIND == PM_I8 ? 8 : 4, 1>(a, grid, s)
-                      : launch_attend_w<KIND, D, KIND == PM_I8 ? 8 : 4, 4>(a, grid, s);
-  return warps == 1 ? launch_attend_w<KIND, D, 8, 1>(a, grid, s) : launch_attend_w<KIND, D, 8, 4>(a, grid, s);
+template <int KIND, int D, int NH>
+AttendKernel *attend_kernel_n(bool fast, int warps) {
+  if (warps == 1) return fast ? attend_kernel_w<KIND, D, NH, true, 1>() : attend_kernel_w<KIND, D, NH, false, 1>();
+  if (warps == 2) return fast ? attend_kernel_w<KIND, D, NH, true, 2>() : attend_kernel_w<KIND, D, NH, false, 2>();
+  return fast ? attend_kernel_w<KIND, D, NH, true, 4>() : attend_kernel_w<KIND, D, NH, false, 4>();
 }
 template <int KIND>
-cudaError_t launch_attend_k(const AttendArgs &a, int warps, unsigned grid, cudaStream_t s) {
-  switch (a.c.head_dim) {
-    case 32: return launch_attend_d<KIND, 32>(a, warps, grid, s);
-    case 64: return launch_attend_d<KIND, 64>(a, warps, grid, s);
-    case 96: return launch_attend_d<KIND, 96>(a, warps, grid, s);
-    default: return launch_attend_d<KIND, 128>(a, warps, grid, s);
+AttendKernel *attend_kernel_k(int D, int heads, bool fast, int warps) {
+  constexpr int N = KIND == PM_I8 ? 8 : 4;  // int8 units have 8 heads
+  switch (D) {
+    case 32: return heads == 4 ? attend_kernel_n<KIND, 32, N>(fast, warps) : attend_kernel_n<KIND, 32, 8>(fast, warps);
+    case 64: return heads == 4 ? attend_kernel_n<KIND, 64, N>(fast, warps) : attend_kernel_n<KIND, 64, 8>(fast, warps);
+    case 96: return heads == 4 ? attend_kernel_n<KIND, 96, N>(fast, warps) : attend_kernel_n<KIND, 96, 8>(fast, warps);
+    default: return heads == 4 ? attend_kernel_n<KIND, 128, N>(fast, warps) : attend_kernel_n<KIND, 128, 8>(fast, warps);
   }
 }
-cudaError_t launch_attend(const AttendArgs &a, int warps, unsigned grid, cudaStream_t s) {
-  if (a.c.kind == LLMQ_KV_QUANT8) return launch_attend_k<PM_I8>(a, warps, grid, s);
-  if (a.c.kind == LLMQ_KV_BF16) return launch_attend_k<PM_BF16>(a, warps, grid, s);
-  return launch_attend_k<PM_F32>(a, warps, grid, s);
+// The kernel for a call, ready to launch on ctx's device.
+llmq_status attend_kernel(llmq_ctx *ctx, const AttendArgs &a, int warps, AttendKernel **out) {
+  const bool fast = a.c.page_size % 16 == 0;
+  AttendKernel *k = a.c.kind == LLMQ_KV_QUANT8 ? attend_kernel_k<PM_I8>(a.c.head_dim, a.unit_heads, fast, warps)
+                    : a.c.kind == LLMQ_KV_BF16 ? attend_kernel_k<PM_BF16>(a.c.head_dim, a.unit_heads, fast, warps)
+                                               : attend_kernel_k<PM_F32>(a.c.head_dim, a.unit_heads, fast, warps);
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  int &n = k->per_sm[ctx->device % kMaxDevices];
+  if (!n) {
+    CK(cudaFuncSetAttribute((const void *)k->fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k->smem));
+    CK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k->fn, k->threads, k->smem));
+    if (n <= 0) return fail(ctx, LLMQ_ERR_UNSUPPORTED, "the attention kernel does not fit on this device");
+  }
+  *out = k;
+  return LLMQ_OK;
 }
 
 template <typename E, int D>
@@ -128,22 +150,35 @@ cudaError_t launch_store(const StoreArgs &a, bool vec, unsigned grid, cudaStream
   return cudaGetLastError();
 }
 
-cudaError_t launch_move(const EvictArgs &a, int tiles, unsigned grid, cudaStream_t s) {
-  switch (a.c.head_dim * elem_bytes(a.c.kind) / 16) {
-    case 2: evict_move_kernel<2><<<grid, 256, 0, s>>>(a, tiles); break;
-    case 4: evict_move_kernel<4><<<grid, 256, 0, s>>>(a, tiles); break;
-    case 6: evict_move_kernel<6><<<grid, 256, 0, s>>>(a, tiles); break;
-    case 8: evict_move_kernel<8><<<grid, 256, 0, s>>>(a, tiles); break;
-    case 12: evict_move_kernel<12><<<grid, 256, 0, s>>>(a, tiles); break;
-    case 16: evict_move_kernel<16><<<grid, 256, 0, s>>>(a, tiles); break;
-    case 24: evict_move_kernel<24><<<grid, 256, 0, s>>>(a, tiles); break;
-    default: evict_move_kernel<32><<<grid, 256, 0, s>>>(a, tiles);
-  }
-  return cudaGetLastError();
+// A launch that may start while the kernel before it on the stream ends; its
+// own first step waits for that kernel (griddepcontrol.wait).
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*k)(P...), dim3 grid, unsigned threads, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k, static_cast<P>(args)...);
 }
 
-constexpr int kMaxSplits = 256;  // chunks of one unit that its last CTA joins
-constexpr int kMaxChunk = 4096;  // positions whose rows fit in shared memory without asking for more
+cudaError_t launch_move(const EvictArgs &a, int tiles, unsigned grid, cudaStream_t s) {
+  auto go = [&](void (*k)(EvictArgs, int)) { return launch_after(k, dim3(grid), 256, s, a, tiles); };
+  switch (a.c.head_dim * elem_bytes(a.c.kind) / 16) {
+    case 2: return go(evict_move_kernel<2>);
+    case 4: return go(evict_move_kernel<4>);
+    case 6: return go(evict_move_kernel<6>);
+    case 8: return go(evict_move_kernel<8>);
+    case 12: return go(evict_move_kernel<12>);
+    case 16: return go(evict_move_kernel<16>);
+    case 24: return go(evict_move_kernel<24>);
+    default: return go(evict_move_kernel<32>);
+  }
+}
 
 // Blocks of a one-dimensional grid, or 0 when there would be too many.
 unsigned grid1(long long n) { return n > 0 && n <= INT_MAX ? (unsigned)n : 0u; }
@@ -248,6 +283,7 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   a.layer = layer;
   a.n_head = n_head;
   a.max_len = (int)std::min((long long)max_len, (long long)table_cols * p->v.page_size);
+  a.score_stride = (int)(((long long)a.max_len + 3) / 4 * 4);
   a.q = q;
   a.out = out;
   a.q_stride = q_stride;
@@ -259,34 +295,37 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   a.unit_heads = p->v.kind != LLMQ_KV_QUANT8 && G <= 4 ? 4 : 8;
   a.head_chunks = (G + a.unit_heads - 1) / a.unit_heads;
   const long long units = (long long)n_seqs * p->v.n_kv_head * a.head_chunks;
-  // chunks so that the longest call's CTAs fill the GPU about twice over
-  const int target = getenv("TGT") ? atoi(getenv("TGT")) : 5;
-  const long long want = std::max(1LL, (long long)ctx->num_sms * target / units);
-  long long chunk = std::max(64LL, (a.max_len + want - 1) / want);
-  chunk = std::max(chunk, (long long)(a.max_len + kMaxSplits - 1) / kMaxSplits);
-  a.chunk = (int)std::min((chunk + 63) / 64 * 64, (long long)kMaxChunk);
-  a.splits = (a.max_len + a.chunk - 1) / a.chunk;
-  int warps = a.splits == 1 && units >= ctx->num_sms * 8 ? 1 : 4;
+  int warps = a.max_len <= 512 && units >= ctx->num_sms * 4 ? 1 : 4;
   if (getenv("WARPS")) warps = atoi(getenv("WARPS"));
+  AttendKernel *k;
+  if ((st = attend_kernel(ctx, a, warps, &k)) != LLMQ_OK) return st;
+  // Chunks: one wave of resident CTAs if every sequence were the longest,
+  // in whole blocks, at most kMaxJoin of a unit
+  const long long wave = (long long)ctx->num_sms * k->per_sm[ctx->device % kMaxDevices];
+  const double waves = getenv("WAVES") ? atof(getenv("WAVES")) : n_seqs == 1 ? 1.0 : 1.5;
+  const long long fit = std::min((long long)kMaxJoin, std::max(1LL, (long long)(waves * wave / units)));
+  const int minb = getenv("MINB") ? atoi(getenv("MINB")) : 2;
+  long long blocks = (a.max_len + k->block - 1) / k->block;
+  a.chunk = (int)std::max((long long)minb, (blocks + fit - 1) / fit) * k->block;
+  a.splits = (a.max_len + a.chunk - 1) / a.chunk;
   const unsigned g = grid1(units * a.splits);
   if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many sequences for one call");
-  const size_t parts = a.splits > 1 ? (size_t)units * a.splits * a.unit_heads * (D + 2) : 0;
-  if (weights_out || parts) {
-    ServeWs *ws;
-    const size_t floats = parts + (weights_out ? rows * (a.max_len + 2) : 0);
-    if ((st = serve_ws(ctx, floats * 4, parts ? (size_t)units : 0, &ws)) != LLMQ_OK) return st;
-    a.part = (float *)ws->buf;
-    a.tickets = ws->tickets;
-    if (weights_out) {
-      a.stat = a.part + parts;
-      a.scores = a.stat + rows * 2;
-    }
-  }
-  CK(launch_attend(a, warps, g, ctx->stream));
+  ServeWs *ws;
+  const size_t parts = a.splits > 1 ? (size_t)g * a.unit_heads * (D + 2) : 0, floats = parts + (weights_out ? rows * (a.score_stride + 2) + 4 : 0);
+  if ((st = serve_ws(ctx, floats * 4, a.splits > 1 ? (size_t)units : 0, &ws)) != LLMQ_OK) return st;
+  a.part = (float *)ws->buf;
+  a.tickets = ws->tickets;
   if (weights_out) {
-    const dim3 wg((max_len + 255) / 256, (unsigned)std::min((long long)n_seqs * p->v.n_kv_head, 65535LL));
-    paged_weights_kernel<<<wg, 256, 0, ctx->stream>>>(a, max_len, weights, weights_out, weights_stride);
-    CKL();
+    a.scores = a.part + (parts + 3) / 4 * 4;  // 16-byte aligned rows
+    a.stat = a.scores + rows * a.score_stride;
+  }
+  k->fn<<<g, k->threads, k->smem, ctx->stream>>>(a);
+  CKL();
+  if (weights_out) {
+    const dim3 wg((max_len + 1023) / 1024, (unsigned)std::min((long long)n_seqs * p->v.n_kv_head, 65535LL));
+    const bool vec = ((uintptr_t)weights | (uintptr_t)weights_out) % 16 == 0 && weights_stride % 4 == 0;
+    CK(launch_after(vec ? paged_weights_kernel<true> : paged_weights_kernel<false>, wg, 256, ctx->stream, a, max_len,
+                    weights, weights_out, weights_stride));
   }
   return LLMQ_OK;
 }
