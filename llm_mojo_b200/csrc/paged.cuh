@@ -135,6 +135,7 @@ struct AttendArgs {
   const float *q;
   float *out;
   long long q_stride, out_stride;
+  bool q_vec;  // rows of q are 16-byte aligned
   const int *lens;
   float scale2;   // scale * log2(e): scores are exponents of two
   float *scores;  // [n_seqs][n_head][score_stride], for the weights; else null

@@ -35,6 +35,19 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The first product of a sum, from c on.
+__device__ __forceinline__ void mma_f16_from(float (&d)[4], float c0, float c2, const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%11,%11};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c2));
+}
+__device__ __forceinline__ void mma_bf16_from0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -147,7 +160,7 @@ struct PmShape {
 
 // Dynamic shared memory: the rows of a run's tiles (page_size % 16 == 0) or
 // of its positions; then the rings, and in their place, at the end, the warps' states, and the join's factors.
-constexpr int kPmJoin = 64;  // partial results whose factors the join holds at a time
+constexpr int kPmJoin = 128;  // chunks of a unit at most
 template <int KIND, int D, int W>
 __host__ __device__ constexpr int pm_rows_bytes(bool fast) {
   return PmShape<KIND, D, W>::kRun / (fast ? 16 : 1) * 4;
@@ -155,7 +168,8 @@ __host__ __device__ constexpr int pm_rows_bytes(bool fast) {
 template <int KIND, int D, int W>
 __host__ __device__ constexpr int pm_smem(bool fast) {
   typedef PmShape<KIND, D, W> Sh;
-  constexpr int ring = W * Sh::kStages * Sh::kStage, join = W * 8 * (D + 2) * 4, fac = 8 * kPmJoin * 4;
+  constexpr int ring = W * Sh::kStages * Sh::kStage, join = W * 8 * (D + 4) * 4;
+  constexpr int fac = (8 * kPmJoin + (8 * D > W * 32 ? 8 * D : W * 32)) * 4;
   constexpr int most = ring > join ? ring : join;
   return pm_rows_bytes<KIND, D, W>(fast) + (most > fac ? most : fac);
 }
@@ -204,27 +218,53 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
   const unsigned ring = (unsigned)__cvta_generic_to_shared(pool) + warp * (S * Sh::kStage);
   auto pos_of = [&](int i) { return (i >> 1) * 8 + 2 * t + (i & 1); };  // the lane's position i of a tile
   auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  // Where the lane's i-th piece of a tile's K (or V) goes: piece 32 i + lane.
+  const int piece0 = lane / NC * Sh::kPad + lane % NC * 16;
+  auto piece_at = [&](int i) {
+    if constexpr (32 % NC == 0) return piece0 + i * (32 / NC) * Sh::kPad;
+    const int p = 32 * i + lane;
+    return p / NC * Sh::kPad + p % NC * 16;
+  };
   // ldmatrix: lane 8 m + i names row i of matrix m. K: matrix = (n-tile, piece), V: (half of the rows, piece)
+  const int matrix0 = (NC == 2 ? (lane >> 4) * 8 + (lane & 7) : lane & 7) * Sh::kPad + (NC == 2 ? lane >> 3 & 1 : lane >> 3) * 16;
   auto matrix_at = [&](int i) {
+    if constexpr (NC == 2) return matrix0;
+    if constexpr (NC % 4 == 0) return matrix0 + 4 * i / NC * 8 * Sh::kPad + 4 * i % NC * 16;
     const int mt = 4 * i + (lane >> 3);
     return (mt / NC * 8 + (lane & 7)) * Sh::kPad + mt % NC * 16;
   };
+  const int vmatrix0 = Sh::kVat + ((lane >> 3 & 1) * 8 + (lane & 7)) * Sh::kPad + (lane >> 4) * 16;
 
   {
     // the query's operand, kept for the whole chunk
     uint32_t qa[Sh::kSteps][4], qb[TWO ? Sh::kSteps : 1][2];
-    float fs = a.scale2, cb0 = 0.0f, cb1 = 0.0f;  // int8: where the scores' two rows start
+    float fs = a.scale2, cb = 0.0f;  // cb: where int8's scores start
     {
       float x[Sh::kSteps][4];
       const float *q = a.q + (size_t)b * a.q_stride + (size_t)(h0 + gh) * D;
       float mx = 0.0f;
+      const bool vec = a.q_vec;
 #pragma unroll
-      for (int k = 0; k < Sh::kSteps; k++)
+      for (int k = 0; k < Sh::kSteps; k++) {
+        // int8: 4 dimensions in a row, bfloat16: 2 and 2
+        if (KIND != PM_F32 && vec) {
+          float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (gh < nh) {
+            if constexpr (I8) {
+              y = *(const float4 *)(q + Sh::kdim(k, 0, t));
+            } else {
+              const float2 y0 = *(const float2 *)(q + Sh::kdim(k, 0, t)), y1 = *(const float2 *)(q + Sh::kdim(k, 2, t));
+              y = make_float4(y0.x, y0.y, y1.x, y1.y);
+            }
+          }
+          x[k][0] = y.x, x[k][1] = y.y, x[k][2] = y.z, x[k][3] = y.w;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          x[k][e] = gh < nh ? q[Sh::kdim(k, e, t)] : 0.0f;
-          mx = fmaxf(mx, fabsf(x[k][e]));
+          for (int e = 0; e < 4; e++) x[k][e] = gh < nh ? q[Sh::kdim(k, e, t)] : 0.0f;
         }
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[k][e]));
+      }
       if constexpr (I8) {
         // the largest |q| of the head to [2^13, 2^14): the second terms reach 2^-38 of it
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -245,8 +285,7 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
             split_f16(x[k][e], x[k][e + 1], qa[k][e], qa[k][e + 1]);
             const float2 hi = __half22float2(*(const __half2 *)&qa[k][e]);
             const float2 lo = __half22float2(*(const __half2 *)&qa[k][e + 1]);
-            cb0 += hi.x + hi.y;
-            cb1 += lo.x + lo.y;
+            cb += (hi.x + lo.x) + (hi.y + lo.y);
           } else if constexpr (TWO) {
             split_bf16(x[k][e], x[k][e + 1], qa[k][e], qa[k][e + 1], qb[k][e / 2]);
           } else {
@@ -254,18 +293,15 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
           }
         }
       if constexpr (I8) {
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          cb0 += __shfl_xor_sync(0xffffffffu, cb0, o);
-          cb1 += __shfl_xor_sync(0xffffffffu, cb1, o);
-        }
-        cb0 *= -0x1p-17f;
-        cb1 *= -0x1p-17f;
+        cb += __shfl_xor_sync(0xffffffffu, cb, 1);
+        cb += __shfl_xor_sync(0xffffffffu, cb, 2);
+        cb *= -0x1p-17f;
       }
     }
 
     const size_t first = a.c.row(a.layer, 0, kh, 0);
-    const char *kl = (const char *)a.c.k + first * Sh::kRow, *vl = (const char *)a.c.v + first * Sh::kRow;
+    const char *kl = (const char *)a.c.k + first * Sh::kRow + (FAST ? lane * 16 : 0);
+    const char *vl = (const char *)a.c.v + first * Sh::kRow + (FAST ? lane * 16 : 0);
     // int8 scales: a lane's piece of a tile's 16 + 16 (FAST), or of its positions
     const float *scl = I8 ? (FAST ? (lane < 4 ? a.c.ks : a.c.vs) + first + (lane & 3) * 4
                                   : (lane < 16 ? a.c.ks : a.c.vs) + first)
@@ -305,13 +341,18 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
           const int tile = U == 1 ? tile0 : min(tile0 + v, ntiles - 1);
           const unsigned d = ring + stage * Sh::kStage + v * Sh::kTile;
           const size_t at0 = FAST ? (size_t)max(rows[tile], 0) : 0;
+          const char *kt = kl + at0 * Sh::kRow, *vt = vl + at0 * Sh::kRow;
 #pragma unroll
           for (int i = 0; i < NC / 2; i++) {  // 16 NC pieces of K, and of V, 32 at a time
-            const int p = i * 32 + lane, r = p / NC, c = p % NC;
-            const size_t off = FAST ? at0 * Sh::kRow + p * 16 : (size_t)max(rows[tile * 16 + r], 0) * Sh::kRow + c * 16;
-            const unsigned at = d + r * Sh::kPad + c * 16;
-            pm_copy16(at, kl + off);
-            pm_copy16(at + Sh::kVat, vl + off);
+            if constexpr (FAST) {
+              pm_copy16(d + piece_at(i), kt + i * 512);
+              pm_copy16(d + piece_at(i) + Sh::kVat, vt + i * 512);
+            } else {
+              const int p = 32 * i + lane;
+              const size_t off = (size_t)max(rows[tile * 16 + p / NC], 0) * Sh::kRow + p % NC * 16;
+              pm_copy16(d + piece_at(i), kl + off);
+              pm_copy16(d + piece_at(i) + Sh::kVat, vl + off);
+            }
           }
           if constexpr (I8) {
             if constexpr (FAST) {
@@ -340,13 +381,6 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
         for (int v = 0; v < U; v++) {
           // scores of 16 positions: two n-tiles of 8
           float c[2][4], c2[2][4];
-#pragma unroll
-          for (int r = 0; r < 2; r++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              c[r][i] = i < 2 ? cb0 : cb1;
-              c2[r][i] = 0.0f;
-            }
           uint32_t kr[2 * NC];
 #pragma unroll
           for (int i = 0; i < NC / 2; i++) pm_ldmatrix<false>(kr + 4 * i, src + v * Sh::kTile + matrix_at(i));
@@ -357,20 +391,31 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
               const uint32_t *x = kr + r * NC;
               if constexpr (KIND == PM_I8) {
                 const uint32_t y = x[k] ^ 0x80808080u;
-                mma_f16(c[r], qa[k], codes_sub(y, 0x4140), codes_sub(y, 0x4342));
+                if (k == 0)
+                  mma_f16_from(c[r], cb, 0.0f, qa[k], codes_sub(y, 0x4140), codes_sub(y, 0x4342));
+                else
+                  mma_f16(c[r], qa[k], codes_sub(y, 0x4140), codes_sub(y, 0x4342));
               } else if constexpr (KIND == PM_BF16) {
-                mma_bf16(c[r], qa[k], x[2 * k], x[2 * k + 1]);
-                if constexpr (TWO) {
-                  const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
-                  mma_bf16(c2[r], q2, x[2 * k], x[2 * k + 1]);
+                const uint32_t q2[4] = {qb[TWO ? k : 0][0], 0u, qb[TWO ? k : 0][1], 0u};
+                if (k == 0) {
+                  mma_bf16_from0(c[r], qa[k], x[0], x[1]);
+                  if constexpr (TWO) mma_bf16_from0(c2[r], q2, x[0], x[1]);
+                } else {
+                  mma_bf16(c[r], qa[k], x[2 * k], x[2 * k + 1]);
+                  if constexpr (TWO) mma_bf16(c2[r], q2, x[2 * k], x[2 * k + 1]);
                 }
               } else {
                 uint32_t y[3], z[3];
                 split_bf16(__uint_as_float(x[4 * k]), __uint_as_float(x[4 * k + 1]), y[0], y[1], y[2]);
                 split_bf16(__uint_as_float(x[4 * k + 2]), __uint_as_float(x[4 * k + 3]), z[0], z[1], z[2]);
-                mma_bf16(c2[r], qa[k], y[2], z[2]);
+                if (k == 0) {
+                  mma_bf16_from0(c2[r], qa[k], y[2], z[2]);
+                  mma_bf16_from0(c[r], qa[k], y[0], z[0]);
+                } else {
+                  mma_bf16(c2[r], qa[k], y[2], z[2]);
+                  mma_bf16(c[r], qa[k], y[0], z[0]);
+                }
                 mma_bf16(c2[r], qa[k], y[1], z[1]);
-                mma_bf16(c[r], qa[k], y[0], z[0]);
                 if constexpr (TWO) {
                   const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
                   mma_bf16(c2[r], q2, y[0], z[0]);
@@ -452,7 +497,6 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
         const float mu = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int v = 0; v < U; v++) {
-          const unsigned vat = src + v * Sh::kTile + Sh::kVat;
           float p[4];
 #pragma unroll
           for (int i = 0; i < 4; i++) {
@@ -474,7 +518,7 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
 #pragma unroll
             for (int i = 0; i < NC / 2; i++) {
               uint32_t w[4];  // piece 2 i: rows 0-7, 8-15; piece 2 i + 1: rows 0-7, 8-15
-              pm_ldmatrix<true>(w, vat + ((lane >> 3 & 1) * 8 + (lane & 7)) * Sh::kPad + (2 * i + (lane >> 4)) * 16);
+              pm_ldmatrix<true>(w, src + v * Sh::kTile + vmatrix0 + 32 * i);
               if constexpr (I8) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
@@ -504,7 +548,7 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
               float w[4];
 #pragma unroll
               for (int i = 0; i < 4; i++) {
-                w[i] = pm_read1(vat + pos_of(i) * Sh::kPad + (8 * j + g) * 4);
+                w[i] = pm_read1(src + v * Sh::kTile + Sh::kVat + pos_of(i) * Sh::kPad + (8 * j + g) * 4);
                 if (!(live >> (4 * v + i) & 1u)) w[i] = 0.0f;
               }
               uint32_t x[3], y[3];
@@ -520,41 +564,57 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
 
-    // join the warps: [warp][head][D sums, M, L] in the rings' place
+    // join the warps: [warp][head][D sums, M, L, -, -] in the rings' place
+    constexpr int kJ = D + 4;
     float *join = (float *)pool;
     sync();
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     {
-      float *o = join + (warp * 8 + gh) * (D + 2);
+      float *o = join + (warp * 8 + gh) * kJ;
       const float f = I8 ? vlim * 0x1p-15f : 1.0f;
+      float x[NT][2];
 #pragma unroll
       for (int j = 0; j < NT; j++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          float x = acc[j][e] + acc[j][2 + e];
-          if constexpr (NH == 4) x += __shfl_xor_sync(0xffffffffu, x, 16);
-          if (g < nh) o[Sh::vdim(j, 2 * t + e)] = x * f;
+          x[j][e] = acc[j][e] + acc[j][2 + e];
+          if constexpr (NH == 4) x[j][e] += __shfl_xor_sync(0xffffffffu, x[j][e], 16);
+          x[j][e] *= f;
         }
-      if (g < nh && t == 0) {
-        o[D] = m;
-        o[D + 1] = l;
+      if (g < nh) {
+        if constexpr (I8) {
+#pragma unroll
+          for (int j = 0; j < NT; j += 2)
+            *(float4 *)(o + Sh::vdim(j, 2 * t)) = make_float4(x[j][0], x[j + 1][0], x[j][1], x[j + 1][1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < NT; j++) *(float2 *)(o + Sh::vdim(j, 2 * t)) = make_float2(x[j][0], x[j][1]);
+        }
+        if (t == 0) {
+          o[D] = m;
+          o[D + 1] = l;
+        }
       }
     }
     sync();
     constexpr int kStep = NH * (D + 2);  // floats of a partial result
     for (int i = tid; i < nh * D; i += W * 32) {
       const int h = i / D, d = i % D;
-      const float *o = join + h * (D + 2);
+      const float *o = join + h * kJ;
       float M = -INFINITY, L = 0.0f, x = 0.0f;
+      if constexpr (W == 1) {
+        M = o[D], L = o[D + 1], x = o[d];
+      } else {
 #pragma unroll
-      for (int w = 0; w < W; w++) M = fmaxf(M, o[w * 8 * (D + 2) + D]);
-      const float mu = M == -INFINITY ? 0.0f : M;
+        for (int w = 0; w < W; w++) M = fmaxf(M, o[w * 8 * kJ + D]);
+        const float mu = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-      for (int w = 0; w < W; w++) {
-        const float f = exp2_approx(o[w * 8 * (D + 2) + D] - mu);
-        L = fmaf(o[w * 8 * (D + 2) + D + 1], f, L);
-        x = fmaf(o[w * 8 * (D + 2) + d], f, x);
+        for (int w = 0; w < W; w++) {
+          const float f = exp2_approx(o[w * 8 * kJ + D] - mu);
+          L = fmaf(o[w * 8 * kJ + D + 1], f, L);
+          x = fmaf(o[w * 8 * kJ + d], f, x);
+        }
       }
       if (ns == 1) {
         a.out[(size_t)b * a.out_stride + (size_t)(h0 + h) * D + d] = L == 0.0f ? 0.0f : x / L;
@@ -578,19 +638,29 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
     sync();
     if (!s_last) return;
     __threadfence();
-    // M and L of each head, then the sums, the parts' factors 2^(M_k - M) a
-    // block of kPmJoin at a time in shared memory
+    // M, L and the parts' factors 2^(M_k - M) of each head; then the sums, the
+    // parts dealt to as many groups of threads as there are, joined in order
     const float *part = a.part + (size_t)unit * a.splits * kStep;
-    auto part_of = [&](int k) { return part + (size_t)k * kStep; };
-    float *fac = (float *)pool;  // [head][kPmJoin]
+    float *fac = (float *)pool, *sums = fac + 8 * kPmJoin;  // [head][kPmJoin]; [group][nh * D]
     for (int h = warp; h < nh; h += W) {
-      float M = -INFINITY, L = 0.0f;
-      for (int k = lane; k < ns; k += 32) M = fmaxf(M, __ldcg(part_of(k) + h * (D + 2) + D));
+      constexpr int kN = kPmJoin / 32;
+      float mk[kN], lk[kN], M = -INFINITY, L = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kN; i++) {
+        const int k = i * 32 + lane;
+        const float *o = part + (size_t)k * kStep + h * (D + 2) + D;
+        mk[i] = k < ns ? __ldcg(o) : -INFINITY;
+        lk[i] = k < ns ? __ldcg(o + 1) : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < kN; i++) M = fmaxf(M, mk[i]);
       for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
       const float mu = M == -INFINITY ? 0.0f : M;
-      for (int k = lane; k < ns; k += 32) {
-        const float *o = part_of(k) + h * (D + 2) + D;
-        L = fmaf(__ldcg(o + 1), exp2_approx(__ldcg(o) - mu), L);
+#pragma unroll
+      for (int i = 0; i < kN; i++) {
+        const float f = exp2_approx(mk[i] - mu);
+        L = fmaf(lk[i], f, L);
+        fac[h * kPmJoin + i * 32 + lane] = f;
       }
       for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
       if (lane == 0) {
@@ -598,35 +668,29 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
         s_stat[h][1] = L;
       }
     }
-    constexpr int kOwn = (NH * D + W * 32 - 1) / (W * 32);
-    float x[kOwn];
+    sync();
+    const int no = nh * D, groups = max(1, W * 32 / no);
+    for (int i = tid; i < no * groups; i += W * 32) {
+      const int grp = i / no, o = i % no, h = o / D;
+      const float *src = part + h * (D + 2) + o % D, *f = fac + h * kPmJoin;
+      float x = 0.0f;
+      for (int k0 = grp; k0 < ns; k0 += 8 * groups) {
+        float y[8];
 #pragma unroll
-    for (int e = 0; e < kOwn; e++) x[e] = 0.0f;
-    for (int b0 = 0; b0 < ns; b0 += kPmJoin) {
-      const int nk = min(kPmJoin, ns - b0);
-      sync();
-      for (int i = tid; i < nh * nk; i += W * 32) {
-        const int h = i / nk, k = i % nk;
-        const float M = s_stat[h][0];
-        fac[h * kPmJoin + k] = exp2_approx(__ldcg(part_of(b0 + k) + h * (D + 2) + D) - (M == -INFINITY ? 0.0f : M));
-      }
-      sync();
+        for (int j = 0; j < 8; j++) y[j] = k0 + j * groups < ns ? __ldcg(src + (size_t)(k0 + j * groups) * kStep) : 0.0f;
 #pragma unroll
-      for (int e = 0; e < kOwn; e++) {
-        const int i = e * W * 32 + tid, h = i / D, d = i % D;
-        if (h < nh) {
-#pragma unroll 8
-          for (int k = 0; k < nk; k++)
-            x[e] = fmaf(__ldcg(part_of(b0 + k) + h * (D + 2) + d), fac[h * kPmJoin + k], x[e]);
-        }
+        for (int j = 0; j < 8; j++)
+          if (k0 + j * groups < ns) x = fmaf(y[j], f[k0 + j * groups], x);
       }
+      sums[i] = x;
     }
-#pragma unroll
-    for (int e = 0; e < kOwn; e++) {
-      const int i = e * W * 32 + tid, h = i / D, d = i % D;
-      if (h >= nh) continue;
+    sync();
+    for (int i = tid; i < no; i += W * 32) {
+      const int h = i / D, d = i % D;
+      float x = sums[i];
+      for (int grp = 1; grp < groups; grp++) x += sums[grp * no + i];
       const float L = s_stat[h][1];
-      a.out[(size_t)b * a.out_stride + (size_t)(h0 + h) * D + d] = L == 0.0f ? 0.0f : x[e] / L;
+      a.out[(size_t)b * a.out_stride + (size_t)(h0 + h) * D + d] = L == 0.0f ? 0.0f : x / L;
       if (a.stat && d == 0) {
         a.stat[2 * ((size_t)b * a.n_head + h0 + h)] = s_stat[h][0];
         a.stat[2 * ((size_t)b * a.n_head + h0 + h) + 1] = L;

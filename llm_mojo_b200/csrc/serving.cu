@@ -58,7 +58,6 @@ llmq_status serve_ws(llmq_ctx *ctx, size_t bytes, size_t tickets, ServeWs **out)
 }
 
 constexpr int kMaxDevices = 64;
-constexpr int kMaxJoin = 128;  // chunks of one unit, which its last CTA joins
 
 int elem_bytes(int kind) { return kind == LLMQ_KV_F32 ? 4 : kind == LLMQ_KV_BF16 ? 2 : 1; }
 
@@ -288,6 +287,7 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   a.out = out;
   a.q_stride = q_stride;
   a.out_stride = out_stride;
+  a.q_vec = (uintptr_t)q % 16 == 0 && q_stride % 4 == 0;
   a.lens = lens;
   a.scale2 = (float)(scale * 1.4426950408889634);
   const size_t rows = (size_t)n_seqs * n_head;
@@ -295,15 +295,19 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   a.unit_heads = p->v.kind != LLMQ_KV_QUANT8 && G <= 4 ? 4 : 8;
   a.head_chunks = (G + a.unit_heads - 1) / a.unit_heads;
   const long long units = (long long)n_seqs * p->v.n_kv_head * a.head_chunks;
-  int warps = a.max_len <= 512 && units >= ctx->num_sms * 4 ? 1 : 4;
+  // Fewer warps a CTA for many units of short sequences, whose prologues and
+  // joins then cost less than idle warps do (int8, 64 dimensions, us with 1 /
+  // 2 / 4 warps: 3072 units x <=256 positions 22 / 25 / 33, 1536 x <=256 21 /
+  // 17 / 19, 576 x <=256 12 / 12 / 9)
+  int warps = units >= ctx->num_sms * 16 && a.max_len <= 256 ? 1 : units >= ctx->num_sms * 8 ? 2 : 4;
   if (getenv("WARPS")) warps = atoi(getenv("WARPS"));
   AttendKernel *k;
   if ((st = attend_kernel(ctx, a, warps, &k)) != LLMQ_OK) return st;
   // Chunks: one wave of resident CTAs if every sequence were the longest,
-  // in whole blocks, at most kMaxJoin of a unit
+  // in whole blocks, at most kPmJoin of a unit
   const long long wave = (long long)ctx->num_sms * k->per_sm[ctx->device % kMaxDevices];
-  const double waves = getenv("WAVES") ? atof(getenv("WAVES")) : n_seqs == 1 ? 1.0 : 1.5;
-  const long long fit = std::min((long long)kMaxJoin, std::max(1LL, (long long)(waves * wave / units)));
+  const double waves = getenv("WAVES") ? atof(getenv("WAVES")) : n_seqs == 1 ? 1.0 : 2.0;
+  const long long fit = std::min((long long)kPmJoin, std::max(1LL, (long long)(waves * wave / units)));
   const int minb = getenv("MINB") ? atoi(getenv("MINB")) : 2;
   long long blocks = (a.max_len + k->block - 1) / k->block;
   a.chunk = (int)std::max((long long)minb, (blocks + fit - 1) / fit) * k->block;
