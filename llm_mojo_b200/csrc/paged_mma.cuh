@@ -1,29 +1,30 @@
 // paged_mma.cuh -- attention of one new token over a paged cache on the
 // tensor cores, split over positions and joined.
 //
-// One pass over the cache: scores S = Q K^T, running maximum M and sum L of
-// 2^(s - M), and O = P V, as m16n8k16 products with float32 accumulators,
-// from registers to registers: the score tile's accumulator layout is the
-// operand layout of P. The rows of the 16-row operand hold up to 8 query
-// heads of one kv head, twice: a float32 factor x enters as a sum of 16-bit
-// terms, so that products keep float32's accuracy,
-//   int8:     x 2^e = f16 + f16: rows 0-7 the first term, rows 8-15 the
-//             second (22 bits; codes are exact in f16),
-//   bfloat16: x = bf16 + bf16 + bf16 by truncation (all 24 bits): rows 0-7
-//             and 8-15 the first two, a second product the third,
+// One pass over the cache: scores S^T = K Q^T, running maximum M and sum L
+// of 2^(s - M), and O^T = V^T P^T, as m16n8k16 products with float32
+// accumulators. Positions, and then dimensions, are the 16 rows; the 8
+// columns are up to 4 query heads of one kv head, two terms each: a float32
+// factor x enters as a sum of 16-bit terms, so that products keep float32's
+// accuracy,
+//   int8:     x 2^e = f16 + f16 (22 bits; codes are exact in f16),
+//   bfloat16: x = bf16 + bf16 + bf16 by truncation (all 24 bits), the third
+//             terms as 8 more columns,
 //   float32:  both factors in three bf16 terms, the products of weight
-//             2^-24 and above,
-// and a head's result is the sum of its rows. The terms sit in rows that one
-// query head or a few would leave idle.
+//             2^-24 and above.
+// A lane's accumulators are the terms of one head, so they add up in place,
+// and few query heads still fill the columns with what accuracy needs. P goes
+// from the accumulators' layout to the operand's by one transposing move per
+// 8x8 block.
 //
-// Both products may take dimensions and positions in any order that their
-// two operands share. A warp copies its tiles of 16 rows of K and of V
-// (cp.async, 16-byte pieces) into its own ring in shared memory, rows padded
-// by 16 bytes, so that ldmatrix reads them without bank conflicts: K as it
-// lies (a lane's 4 bytes of row lane / 4), V transposed (a pair of rows).
-// For int8 the transposed element is a pair of codes, which one byte permute
-// each turns into two operands. Copies in flight cost no registers, and
-// warps wait for nothing but their own copies.
+// Both products may take dimensions in any order that their two operands
+// share. A warp copies its tiles of 16 rows of K and of V (cp.async, 16-byte
+// pieces) into its own ring in shared memory, rows padded by 16 bytes, so
+// that ldmatrix reads them without bank conflicts: K as it lies (a lane's 4
+// bytes of row lane / 4), V transposed (a pair of rows). For int8 the
+// transposed element is a pair of codes, which one byte permute each turns
+// into two operands. Copies in flight cost no registers, and warps wait for
+// nothing but their own copies.
 #pragma once
 
 #include "paged.cuh"
@@ -35,12 +36,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The first product of a sum, from c on.
-__device__ __forceinline__ void mma_f16_from(float (&d)[4], float c0, float c2, const uint32_t (&a)[4], uint32_t b0,
-                                             uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%11,%11};"
+// The first product of a sum, from c in the even columns and 0 in the odd.
+__device__ __forceinline__ void mma_f16_from(float (&d)[4], float c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c2));
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c), "f"(0.0f));
 }
 __device__ __forceinline__ void mma_bf16_from0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -75,10 +75,12 @@ __device__ __forceinline__ void pm_ldmatrix(uint32_t *d, unsigned src) {
                  : "r"(src)
                  : "memory");
 }
-__device__ __forceinline__ float2 pm_read2(unsigned src) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(src) : "memory");
-  return v;
+// The transpose of an 8x8 matrix of 16-bit elements, lane (g, t) holding row
+// g's elements 2t, 2t + 1.
+__device__ __forceinline__ uint32_t pm_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ float pm_read1(unsigned src) {
   float v;
@@ -110,7 +112,8 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32
   lo = *(const uint32_t *)&l;
 }
 
-// x, y as three bf16 terms each by truncation, exact: 8 + 8 + 8 bits.
+// x, y as three bf16 terms each by truncation, exact: 8 + 8 + 8 bits. t0 =
+// (first of x, first of y), and so on.
 __device__ __forceinline__ void split_bf16(float x, float y, uint32_t &t0, uint32_t &t1, uint32_t &t2) {
   const uint32_t x0 = __float_as_uint(x) & 0xffff0000u, y0 = __float_as_uint(y) & 0xffff0000u;
   const float xr = x - __uint_as_float(x0), yr = y - __uint_as_float(y0);
@@ -121,14 +124,13 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t &t0, uint3
   t2 = __byte_perm(__float_as_uint(xs), __float_as_uint(ys), 0x7632);
 }
 
-// x, y as three bf16 terms in the operand rows of a unit with at most 4
-// heads: rows 0-3 (lanes g < 4) the first, rows 4-7 (the other lanes, which
-// hold the same x, y) the second, rows 8-11 the third.
-__device__ __forceinline__ void split_bf16_rows(float x, float y, bool low, uint32_t &top, uint32_t &bottom) {
-  uint32_t t0, t1, t2;
-  split_bf16(x, y, t0, t1, t2);
-  top = low ? t0 : t1;
-  bottom = low ? t2 : 0u;
+// One x: (first, second) and (third, 0).
+__device__ __forceinline__ void split_bf16_one(float x, uint32_t &t01, uint32_t &t2) {
+  const uint32_t x0 = __float_as_uint(x) & 0xffff0000u;
+  const float r = x - __uint_as_float(x0);
+  const uint32_t x1 = __float_as_uint(r) & 0xffff0000u;
+  t01 = (x0 >> 16) | x1;
+  t2 = __float_as_uint(r - __uint_as_float(x1)) >> 16;
 }
 
 enum { PM_I8 = 0, PM_BF16 = 1, PM_F32 = 2 };
@@ -137,7 +139,7 @@ struct PmShape {
   static constexpr int kEs = KIND == PM_I8 ? 1 : KIND == PM_BF16 ? 2 : 4;
   static constexpr int kRow = D * kEs, kNc = kRow / 16;  // bytes and 16-byte pieces of a row
   static constexpr int kPad = kRow + 16;                 // a row in the ring: an odd number of pieces
-  static constexpr int kSteps = D / 16, kNt = D / 8;
+  static constexpr int kSteps = D / 16;  // steps of the scores; and tiles of dimensions of the output
   // tiles of 16 positions taken together: two while their operands fit in registers
   static constexpr int kU = kRow <= 128 ? 2 : 1;
   // a stage of a warp's ring, for each tile: 16 rows of K, 16 of V, and (int8) their scales
@@ -152,9 +154,9 @@ struct PmShape {
   static __device__ __forceinline__ int kdim(int k, int u, int t) {
     return 16 * k + (KIND == PM_I8 ? 4 * t + u : KIND == PM_BF16 ? (u >> 1) * 8 + 2 * t + (u & 1) : 4 * u + t);
   }
-  // Dimension of column c of output tile j.
-  static __device__ __forceinline__ int vdim(int j, int c) {
-    return KIND == PM_I8 ? (j >> 1) * 16 + 2 * c + (j & 1) : 8 * j + c;
+  // Dimension of row g (half 0) or g + 8 (half 1) of output tile j.
+  static __device__ __forceinline__ int vdim(int j, int half, int g) {
+    return 16 * j + (KIND == PM_I8 ? 2 * g + half : 8 * half + g);
   }
 };
 
@@ -176,24 +178,21 @@ __host__ __device__ constexpr int pm_smem(bool fast) {
 
 // CTAs of 4 warps per SM that registers are held down for: 96, 128, 168 or
 // 255 a thread, as the accumulators and the query need.
-constexpr int pm_per_sm(int kind, int D, int NH) {
-  const bool two = kind != PM_I8 && NH == 8;
-  return D == 32 ? 5 : D == 64 ? (two ? 3 : 4) : D == 96 ? (two ? 2 : 3) : two || kind == PM_F32 ? 2 : 3;
+constexpr int pm_per_sm(int kind, int D, int HT) {
+  return D == 32 ? 5 : D == 64 ? (kind == PM_I8 && HT == 1 ? 5 : 4) : HT == 2 ? 2 : 3;
 }
 
-// One CTA: one unit (sequence, kv head, up to NH of its query heads) and one
-// chunk of positions, tiles of 16 dealt to the W warps. FAST: page_size is a
-// multiple of 16, a tile lies in one page. NH 4 (bfloat16 and float32): the
-// three terms of 4 heads fill 12 of the 16 rows, one product where 8 heads
-// need two. The chunks of a unit write their sums to a.part; the last to
-// arrive joins them in chunk order (so the bits do not depend on the order
-// of arrival) and leaves its ticket zero.
-// grid n_seqs * n_kv_head * head_chunks * splits.
-template <int KIND, int D, int NH, bool FAST, int W>
-__global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_mma_kernel(AttendArgs a) {
+// One CTA: one unit (sequence, kv head, up to 4 HT of its query heads) and
+// one chunk of positions, tiles of 16 dealt to the W warps, U at a time.
+// FAST: page_size is a multiple of 16, a tile lies in one page. The chunks of
+// a unit write their sums to a.part; the last to arrive joins them in chunk
+// order (so the bits do not depend on the order of arrival) and leaves its
+// ticket zero. grid n_seqs * n_kv_head * head_chunks * splits.
+template <int KIND, int D, int HT, bool FAST, int W>
+__global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_mma_kernel(AttendArgs a) {
   typedef PmShape<KIND, D, W> Sh;
-  constexpr bool I8 = KIND == PM_I8, TWO = !I8 && NH == 8;  // TWO: the third terms are a second product
-  constexpr int NT = Sh::kNt, S = Sh::kStages, NC = Sh::kNc, U = Sh::kU;
+  constexpr bool I8 = KIND == PM_I8;
+  constexpr int NT = Sh::kSteps, S = Sh::kStages, NC = Sh::kNc, U = Sh::kU, NH = 4 * HT;
   extern __shared__ __align__(16) char smem[];
   __shared__ int s_last;
   __shared__ float s_stat[8][2];
@@ -201,7 +200,7 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
   const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
   const int hc = unit % a.head_chunks, kh = unit / a.head_chunks % a.c.n_kv_head;
   const int b = unit / a.head_chunks / a.c.n_kv_head;
-  const int G = a.n_head / a.c.n_kv_head, ps = a.c.page_size, gh = NH == 4 ? g & 3 : g;  // gh: the lane's head
+  const int G = a.n_head / a.c.n_kv_head, ps = a.c.page_size;
   const int h0 = kh * G + hc * NH, nh = min(NH, G - hc * NH);
   const int len = paged_len(a, b), ns = max(1, (len + a.chunk - 1) / a.chunk);
   if (split >= ns) return;
@@ -216,7 +215,9 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
   };
 
   const unsigned ring = (unsigned)__cvta_generic_to_shared(pool) + warp * (S * Sh::kStage);
-  auto pos_of = [&](int i) { return (i >> 1) * 8 + 2 * t + (i & 1); };  // the lane's position i of a tile
+  // of a tile: the lane's scores are positions g and g + 8 of head t, its
+  // operands of V positions 2t, 2t + 1, 8 + 2t and 9 + 2t
+  auto vpos = [&](int i) { return (i >> 1) * 8 + 2 * t + (i & 1); };
   auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
   // Where the lane's i-th piece of a tile's K (or V) goes: piece 32 i + lane.
   const int piece0 = lane / NC * Sh::kPad + lane % NC * 16;
@@ -233,23 +234,28 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
     const int mt = 4 * i + (lane >> 3);
     return (mt / NC * 8 + (lane & 7)) * Sh::kPad + mt % NC * 16;
   };
-  const int vmatrix0 = Sh::kVat + ((lane >> 3 & 1) * 8 + (lane & 7)) * Sh::kPad + (lane >> 4) * 16;
+  // V, the four matrices of one product's tile: int8 (piece, half of the rows), bfloat16 (half of the rows, piece)
+  const int half = I8 ? lane >> 3 & 1 : lane >> 4, vpiece = I8 ? lane >> 4 : lane >> 3 & 1;
+  const int vmatrix0 = Sh::kVat + (half * 8 + (lane & 7)) * Sh::kPad + vpiece * 16;
 
   {
-    // the query's operand, kept for the whole chunk
-    uint32_t qa[Sh::kSteps][4], qb[TWO ? Sh::kSteps : 1][2];
-    float fs = a.scale2, cb = 0.0f;  // cb: where int8's scores start
-    {
-      float x[Sh::kSteps][4];
-      const float *q = a.q + (size_t)b * a.q_stride + (size_t)(h0 + gh) * D;
-      float mx = 0.0f;
+    // the query's operand, kept for the whole chunk: column g is a term of
+    // head g / 2, the first or the second (int8, bfloat16), qb the third of
+    // bfloat16 in the even columns
+    uint32_t qa[HT][NT][2], qb[HT][I8 ? 1 : NT][2];
+    float fs[HT], cb[HT];  // of the lane's own head t: the scores' factor, and (int8) where they start
+#pragma unroll
+    for (int ht = 0; ht < HT; ht++) {
+      const int h = ht * 4 + (g >> 1);
+      const float *q = a.q + (size_t)b * a.q_stride + (size_t)(h0 + h) * D;
+      float x[NT][4], mx = 0.0f;
       const bool vec = a.q_vec;
 #pragma unroll
-      for (int k = 0; k < Sh::kSteps; k++) {
+      for (int k = 0; k < NT; k++) {
         // int8: 4 dimensions in a row, bfloat16: 2 and 2
         if (KIND != PM_F32 && vec) {
           float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (gh < nh) {
+          if (h < nh) {
             if constexpr (I8) {
               y = *(const float4 *)(q + Sh::kdim(k, 0, t));
             } else {
@@ -260,42 +266,45 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
           x[k][0] = y.x, x[k][1] = y.y, x[k][2] = y.z, x[k][3] = y.w;
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[k][e] = gh < nh ? q[Sh::kdim(k, e, t)] : 0.0f;
+          for (int e = 0; e < 4; e++) x[k][e] = h < nh ? q[Sh::kdim(k, e, t)] : 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[k][e]));
       }
+      fs[ht] = a.scale2;
+      cb[ht] = 0.0f;
       if constexpr (I8) {
         // the largest |q| of the head to [2^13, 2^14): the second terms reach 2^-38 of it
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const int e = min(max((int)(__float_as_uint(mx) >> 23), 1), 254) - 127;
-        const float up = pow2i(min(13 - e, 126));
+        const float up = pow2i(min(13 - e, 126)), down = a.scale2 * pow2i(max(e - 13, -126)) * 0x1p24f;
+        float sum = 0.0f;  // of the column's term
 #pragma unroll
-        for (int k = 0; k < Sh::kSteps; k++)
+        for (int k = 0; k < NT; k++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) x[k][i] *= up;
-        fs = a.scale2 * pow2i(max(e - 13, -126)) * 0x1p24f;
-      }
-#pragma unroll
-      for (int k = 0; k < Sh::kSteps; k++)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          if constexpr (I8) {
-            split_f16(x[k][e], x[k][e + 1], qa[k][e], qa[k][e + 1]);
-            const float2 hi = __half22float2(*(const __half2 *)&qa[k][e]);
-            const float2 lo = __half22float2(*(const __half2 *)&qa[k][e + 1]);
-            cb += (hi.x + lo.x) + (hi.y + lo.y);
-          } else if constexpr (TWO) {
-            split_bf16(x[k][e], x[k][e + 1], qa[k][e], qa[k][e + 1], qb[k][e / 2]);
-          } else {
-            split_bf16_rows(x[k][e], x[k][e + 1], g < 4, qa[k][e], qa[k][e + 1]);
+          for (int i = 0; i < 4; i += 2) {
+            uint32_t hi, lo;
+            split_f16(x[k][i] * up, x[k][i + 1] * up, hi, lo);
+            qa[ht][k][i / 2] = g & 1 ? lo : hi;
+            const float2 f = __half22float2(*(const __half2 *)&qa[ht][k][i / 2]);
+            sum += f.x + f.y;
           }
-        }
-      if constexpr (I8) {
-        cb += __shfl_xor_sync(0xffffffffu, cb, 1);
-        cb += __shfl_xor_sync(0xffffffffu, cb, 2);
-        cb *= -0x1p-17f;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);  // both terms
+        cb[ht] = -0x1p-17f * __shfl_sync(0xffffffffu, sum, 8 * t);
+        fs[ht] = __shfl_sync(0xffffffffu, down, 8 * t);
+      } else {
+#pragma unroll
+        for (int k = 0; k < NT; k++)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            uint32_t t0, t1, t2;
+            split_bf16(x[k][i], x[k][i + 1], t0, t1, t2);
+            qa[ht][k][i / 2] = g & 1 ? t1 : t0;
+            qb[ht][k][i / 2] = g & 1 ? 0u : t2;
+          }
       }
     }
 
@@ -306,12 +315,16 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
     const float *scl = I8 ? (FAST ? (lane < 4 ? a.c.ks : a.c.vs) + first + (lane & 3) * 4
                                   : (lane < 16 ? a.c.ks : a.c.vs) + first)
                           : nullptr;
-    float acc[NT][4];
+    float acc[HT][NT][4], m[HT], l[HT], vlim = 0x1p-100f, vinv = 0x1p115f;
 #pragma unroll
-    for (int j = 0; j < NT; j++)
+    for (int ht = 0; ht < HT; ht++) {
+      m[ht] = -INFINITY;
+      l[ht] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; i++) acc[j][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f, vlim = 0x1p-100f, vinv = 0x1p115f;
+      for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[ht][j][i] = 0.0f;
+    }
 
     for (int c0 = p0; c0 < p1; c0 += Sh::kRun) {
       const int n = min(p1 - c0, Sh::kRun), ntiles = (n + 15) / 16;  // the run
@@ -376,187 +389,226 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
         commit();
         const unsigned src = ring + stage * Sh::kStage;
         stage = stage == S - 1 ? 0 : stage + 1;
-        float s[U][4], sv[U][4];
+        float s[HT][U][2], sv[U][2];
 #pragma unroll
         for (int v = 0; v < U; v++) {
-          // scores of 16 positions: two n-tiles of 8
-          float c[2][4], c2[2][4];
-          uint32_t kr[2 * NC];
+          uint32_t kr[2 * NC];  // [rows 0-7, 8-15][piece]
 #pragma unroll
           for (int i = 0; i < NC / 2; i++) pm_ldmatrix<false>(kr + 4 * i, src + v * Sh::kTile + matrix_at(i));
+          float c[HT][4], c2[HT][4];
 #pragma unroll
-          for (int k = 0; k < Sh::kSteps; k++)
+          for (int k = 0; k < NT; k++) {
+            if constexpr (I8) {
+              const uint32_t x = kr[k] ^ 0x80808080u, y = kr[NC + k] ^ 0x80808080u;
+              const uint32_t f[4] = {codes_sub(x, 0x4140), codes_sub(y, 0x4140), codes_sub(x, 0x4342), codes_sub(y, 0x4342)};
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-              const uint32_t *x = kr + r * NC;
-              if constexpr (KIND == PM_I8) {
-                const uint32_t y = x[k] ^ 0x80808080u;
+              for (int ht = 0; ht < HT; ht++) {
                 if (k == 0)
-                  mma_f16_from(c[r], cb, 0.0f, qa[k], codes_sub(y, 0x4140), codes_sub(y, 0x4342));
+                  mma_f16_from(c[ht], cb[ht], f, qa[ht][k][0], qa[ht][k][1]);
                 else
-                  mma_f16(c[r], qa[k], codes_sub(y, 0x4140), codes_sub(y, 0x4342));
-              } else if constexpr (KIND == PM_BF16) {
-                const uint32_t q2[4] = {qb[TWO ? k : 0][0], 0u, qb[TWO ? k : 0][1], 0u};
+                  mma_f16(c[ht], f, qa[ht][k][0], qa[ht][k][1]);
+              }
+            } else if constexpr (KIND == PM_BF16) {
+              const uint32_t f[4] = {kr[2 * k], kr[NC + 2 * k], kr[2 * k + 1], kr[NC + 2 * k + 1]};
+#pragma unroll
+              for (int ht = 0; ht < HT; ht++) {
                 if (k == 0) {
-                  mma_bf16_from0(c[r], qa[k], x[0], x[1]);
-                  if constexpr (TWO) mma_bf16_from0(c2[r], q2, x[0], x[1]);
+                  mma_bf16_from0(c[ht], f, qa[ht][k][0], qa[ht][k][1]);
+                  mma_bf16_from0(c2[ht], f, qb[ht][k][0], qb[ht][k][1]);
                 } else {
-                  mma_bf16(c[r], qa[k], x[2 * k], x[2 * k + 1]);
-                  if constexpr (TWO) mma_bf16(c2[r], q2, x[2 * k], x[2 * k + 1]);
-                }
-              } else {
-                uint32_t y[3], z[3];
-                split_bf16(__uint_as_float(x[4 * k]), __uint_as_float(x[4 * k + 1]), y[0], y[1], y[2]);
-                split_bf16(__uint_as_float(x[4 * k + 2]), __uint_as_float(x[4 * k + 3]), z[0], z[1], z[2]);
-                if (k == 0) {
-                  mma_bf16_from0(c2[r], qa[k], y[2], z[2]);
-                  mma_bf16_from0(c[r], qa[k], y[0], z[0]);
-                } else {
-                  mma_bf16(c2[r], qa[k], y[2], z[2]);
-                  mma_bf16(c[r], qa[k], y[0], z[0]);
-                }
-                mma_bf16(c2[r], qa[k], y[1], z[1]);
-                if constexpr (TWO) {
-                  const uint32_t q2[4] = {qb[k][0], 0u, qb[k][1], 0u};
-                  mma_bf16(c2[r], q2, y[0], z[0]);
+                  mma_bf16(c[ht], f, qa[ht][k][0], qa[ht][k][1]);
+                  mma_bf16(c2[ht], f, qb[ht][k][0], qb[ht][k][1]);
                 }
               }
-            }
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int r = i >> 1, e = i & 1;
-            if constexpr (I8) {
-              s[v][i] = c[r][e] + c[r][2 + e];
             } else {
-              s[v][i] = c[r][e] + (c[r][2 + e] + (KIND == PM_F32 || TWO ? c2[r][e] + c2[r][2 + e] : 0.0f));
-              if constexpr (NH == 4) s[v][i] += __shfl_xor_sync(0xffffffffu, s[v][i], 16);
+              uint32_t f[3][4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) {  // operand register i: rows 8 (i & 1) on, elements 2 (i / 2), + 1
+                const uint32_t *x = kr + (i & 1) * NC + 4 * k + (i >> 1) * 2;
+                split_bf16(__uint_as_float(x[0]), __uint_as_float(x[1]), f[0][i], f[1][i], f[2][i]);
+              }
+#pragma unroll
+              for (int ht = 0; ht < HT; ht++) {
+                if (k == 0) {
+                  mma_bf16_from0(c2[ht], f[2], qa[ht][k][0], qa[ht][k][1]);
+                  mma_bf16_from0(c[ht], f[0], qa[ht][k][0], qa[ht][k][1]);
+                } else {
+                  mma_bf16(c2[ht], f[2], qa[ht][k][0], qa[ht][k][1]);
+                  mma_bf16(c[ht], f[0], qa[ht][k][0], qa[ht][k][1]);
+                }
+                mma_bf16(c2[ht], f[1], qa[ht][k][0], qa[ht][k][1]);
+                mma_bf16(c2[ht], f[0], qb[ht][k][0], qb[ht][k][1]);
+              }
             }
-            s[v][i] *= fs;
           }
+          float ks[2] = {1.0f, 1.0f};
           if constexpr (I8) {
-            const unsigned at = src + v * Sh::kTile + Sh::kSat + t * 8;
-            const float2 x0 = pm_read2(at), x1 = pm_read2(at + 32), v0 = pm_read2(at + 64), v1 = pm_read2(at + 96);
-            s[v][0] *= x0.x, s[v][1] *= x0.y, s[v][2] *= x1.x, s[v][3] *= x1.y;
-            sv[v][0] = v0.x, sv[v][1] = v0.y, sv[v][2] = v1.x, sv[v][3] = v1.y;
+            const unsigned at = src + v * Sh::kTile + Sh::kSat + g * 4;
+            ks[0] = pm_read1(at), ks[1] = pm_read1(at + 32);
+            sv[v][0] = pm_read1(at + 64), sv[v][1] = pm_read1(at + 96);
           }
+#pragma unroll
+          for (int ht = 0; ht < HT; ht++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              float y = c[ht][2 * i] + c[ht][2 * i + 1];
+              if constexpr (!I8) y = c[ht][2 * i] + (c[ht][2 * i + 1] + (c2[ht][2 * i] + c2[ht][2 * i + 1]));
+              s[ht][v][i] = y * fs[ht];
+              if constexpr (I8) s[ht][v][i] *= ks[i];
+            }
         }
         // positions past the end or without a page: no score, and a zero value
         // (0 times what is there might be NaN)
-        unsigned live = ~0u;
-        if (hole || (tile + U) * 16 > n) {
+        const bool part_live = hole || (tile + U) * 16 > n;
+        if (part_live) {
 #pragma unroll
           for (int v = 0; v < U; v++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const int j = (tile + v) * 16 + pos_of(i);
+            for (int i = 0; i < 2; i++) {
+              const int j = (tile + v) * 16 + g + 8 * i;
               if (j >= n || rows[FAST ? tile + v : j] < 0) {
-                live &= ~(1u << (4 * v + i));
-                s[v][i] = -INFINITY;
                 sv[v][i] = 0.0f;
+#pragma unroll
+                for (int ht = 0; ht < HT; ht++) s[ht][v][i] = -INFINITY;
               }
             }
         }
-        if (a.scores && g < nh) {
-          float *out = a.scores + ((size_t)b * a.n_head + h0 + g) * a.score_stride + c0 + tile * 16;
+        if (a.scores) {
+#pragma unroll
+          for (int ht = 0; ht < HT; ht++)
+            if (ht * 4 + t < nh) {
+              float *out = a.scores + ((size_t)b * a.n_head + h0 + ht * 4 + t) * a.score_stride + c0 + tile * 16 + g;
+#pragma unroll
+              for (int v = 0; v < U; v++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                  if ((tile + v) * 16 + g + 8 * i < n) out[v * 16 + 8 * i] = s[ht][v][i];
+            }
+        }
+        float mx[HT], vm = 0.0f;
+        bool grow = false;
+#pragma unroll
+        for (int ht = 0; ht < HT; ht++) {
+          mx[ht] = s[ht][0][0];
 #pragma unroll
           for (int v = 0; v < U; v++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              if ((tile + v) * 16 + pos_of(i) < n) out[v * 16 + pos_of(i)] = s[v][i];
+            for (int i = 0; i < 2; i++) mx[ht] = fmaxf(mx[ht], s[ht][v][i]);
+          grow = grow || mx[ht] > m[ht];
         }
-        float mx = s[0][0], vm = 0.0f;
+        if constexpr (I8) {
 #pragma unroll
-        for (int v = 0; v < U; v++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            mx = fmaxf(mx, s[v][i]);
-            if constexpr (I8) vm = fmaxf(vm, sv[v][i]);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        if (__any_sync(0xffffffffu, mx > m || (I8 && vm > vlim))) {
-          const float mn = fmaxf(m, mx);
-          float f = m == -INFINITY ? 0.0f : exp2_approx(m - mn);
-          l *= f;
-          m = mn;
+          for (int v = 0; v < U; v++) vm = fmaxf(vm, fmaxf(sv[v][0], sv[v][1]));
+          grow = grow || vm > vlim;
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+          float fv = 1.0f;
           if constexpr (I8) {
             // vlim: a power of two not below any value scale so far
-            for (int o = 16; o > 0; o >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+            for (int o = 16; o > 2; o >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
             if (vm > vlim) {
               const float up = __uint_as_float(min((__float_as_uint(vm) & 0x7f800000u) + 0x800000u, 254u << 23));
-              f *= vlim / up;
+              fv = vlim / up;
               vlim = up;
               vinv = 0x1p15f / up;
             }
           }
 #pragma unroll
-          for (int j = 0; j < NT; j++)
+          for (int ht = 0; ht < HT; ht++) {
+            for (int o = 16; o > 2; o >>= 1) mx[ht] = fmaxf(mx[ht], __shfl_xor_sync(0xffffffffu, mx[ht], o));
+            const float mn = fmaxf(m[ht], mx[ht]);
+            const float f = m[ht] == -INFINITY ? 0.0f : exp2_approx(m[ht] - mn);
+            l[ht] *= f;
+            m[ht] = mn;
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[j][i] *= f;
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) acc[ht][j][i] *= f * fv;
+          }
         }
-        const float mu = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int v = 0; v < U; v++) {
-          float p[4];
+          uint32_t pa[HT][2], pb[HT][2];  // P's operands: positions 2t, 2t + 1, and 8 more; the third terms
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            p[i] = exp2_approx(s[v][i] - mu);
-            l += p[i];
+          for (int ht = 0; ht < HT; ht++) {
+            const float mu = m[ht] == -INFINITY ? 0.0f : m[ht];
+            float p[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              p[i] = exp2_approx(s[ht][v][i] - mu);
+              l[ht] += p[i];
+            }
+            if constexpr (I8) {
+              uint32_t hi, lo;
+              split_f16(p[0] * (sv[v][0] * vinv), p[1] * (sv[v][1] * vinv), hi, lo);
+              pa[ht][0] = pm_transpose(__byte_perm(hi, lo, 0x5410));
+              pa[ht][1] = pm_transpose(__byte_perm(hi, lo, 0x7632));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2; i++) {
+                split_bf16_one(p[i], pa[ht][i], pb[ht][i]);
+                pa[ht][i] = pm_transpose(pa[ht][i]);
+                pb[ht][i] = pm_transpose(pb[ht][i]);
+              }
+            }
           }
-          uint32_t pa[4], pb[4] = {0u, 0u, 0u, 0u};
+          bool ok[4] = {true, true, true, true};  // the lane's operand positions of V
+          if (!I8 && part_live) {
 #pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            if constexpr (I8)
-              split_f16(p[i] * (sv[v][i] * vinv), p[i + 1] * (sv[v][i + 1] * vinv), pa[i], pa[i + 1]);
-            else if constexpr (TWO)
-              split_bf16(p[i], p[i + 1], pa[i], pa[i + 1], pb[i]);
-            else
-              split_bf16_rows(p[i], p[i + 1], g < 4, pa[i], pa[i + 1]);
+            for (int i = 0; i < 4; i++) {
+              const int j = (tile + v) * 16 + vpos(i);
+              ok[i] = j < n && rows[FAST ? tile + v : j] >= 0;
+            }
           }
-          if constexpr (KIND != PM_F32) {
-            // operand registers of the rows 0-7 and 8-15: pieces 2 i and 2 i + 1 of both halves at a time
+          if constexpr (I8) {
 #pragma unroll
-            for (int i = 0; i < NC / 2; i++) {
-              uint32_t w[4];  // piece 2 i: rows 0-7, 8-15; piece 2 i + 1: rows 0-7, 8-15
-              pm_ldmatrix<true>(w, src + v * Sh::kTile + vmatrix0 + 32 * i);
-              if constexpr (I8) {
+            for (int j = 0; j < NT; j += 2) {
+              uint32_t w[4];  // piece j: rows 0-7, 8-15; piece j + 1: rows 0-7, 8-15
+              pm_ldmatrix<true>(w, src + v * Sh::kTile + vmatrix0 + 16 * j);
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                  float (*o)[4] = acc + 4 * i + 2 * j;
-                  const uint32_t x = w[2 * j] ^ 0x80808080u, y = w[2 * j + 1] ^ 0x80808080u;
-                  mma_f16(o[0], pa, codes_f16(x, 0x4240), codes_f16(y, 0x4240));
-                  mma_f16(o[1], pa, codes_f16(x, 0x4341), codes_f16(y, 0x4341));
-                }
-              } else {
-                if (live != ~0u) {
-                  const unsigned f = live >> (4 * v);
-                  const uint32_t z0 = (f & 1u ? 0xffffu : 0u) | (f & 2u ? 0xffff0000u : 0u);
-                  const uint32_t z1 = (f & 4u ? 0xffffu : 0u) | (f & 8u ? 0xffff0000u : 0u);
-                  w[0] &= z0, w[1] &= z1, w[2] &= z0, w[3] &= z1;
-                }
-                mma_bf16(acc[2 * i], pa, w[0], w[1]);
-                mma_bf16(acc[2 * i + 1], pa, w[2], w[3]);
-                if constexpr (TWO) {
-                  mma_bf16(acc[2 * i], pb, w[0], w[1]);
-                  mma_bf16(acc[2 * i + 1], pb, w[2], w[3]);
-                }
+              for (int e = 0; e < 2; e++) {
+                const uint32_t x = w[2 * e] ^ 0x80808080u, y = w[2 * e + 1] ^ 0x80808080u;
+                const uint32_t f[4] = {codes_f16(x, 0x4240), codes_f16(x, 0x4341), codes_f16(y, 0x4240), codes_f16(y, 0x4341)};
+#pragma unroll
+                for (int ht = 0; ht < HT; ht++) mma_f16(acc[ht][j + e], f, pa[ht][0], pa[ht][1]);
               }
             }
           } else {
 #pragma unroll
             for (int j = 0; j < NT; j++) {
-              float w[4];
+              if constexpr (KIND == PM_BF16) {
+                uint32_t w[4];  // rows 0-7 of pieces 2 j, 2 j + 1; rows 8-15
+                pm_ldmatrix<true>(w, src + v * Sh::kTile + vmatrix0 + 32 * j);
+                if (part_live) {
+                  const uint32_t z0 = (ok[0] ? 0xffffu : 0u) | (ok[1] ? 0xffff0000u : 0u);
+                  const uint32_t z1 = (ok[2] ? 0xffffu : 0u) | (ok[3] ? 0xffff0000u : 0u);
+                  w[0] &= z0, w[1] &= z0, w[2] &= z1, w[3] &= z1;
+                }
 #pragma unroll
-              for (int i = 0; i < 4; i++) {
-                w[i] = pm_read1(src + v * Sh::kTile + Sh::kVat + pos_of(i) * Sh::kPad + (8 * j + g) * 4);
-                if (!(live >> (4 * v + i) & 1u)) w[i] = 0.0f;
+                for (int ht = 0; ht < HT; ht++) {
+                  mma_bf16(acc[ht][j], w, pa[ht][0], pa[ht][1]);
+                  mma_bf16(acc[ht][j], w, pb[ht][0], pb[ht][1]);
+                }
+              } else {
+                uint32_t f[3][4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {  // operand register i: dimensions 8 (i & 1) on, positions 8 (i / 2) on
+                  float y[2];
+#pragma unroll
+                  for (int e = 0; e < 2; e++) {
+                    const int r = (i >> 1) * 2 + e;
+                    y[e] = pm_read1(src + v * Sh::kTile + Sh::kVat + vpos(r) * Sh::kPad + (16 * j + 8 * (i & 1) + g) * 4);
+                    if (!ok[r]) y[e] = 0.0f;
+                  }
+                  split_bf16(y[0], y[1], f[0][i], f[1][i], f[2][i]);
+                }
+#pragma unroll
+                for (int ht = 0; ht < HT; ht++) {
+                  mma_bf16(acc[ht][j], f[0], pb[ht][0], pb[ht][1]);
+#pragma unroll
+                  for (int k = 2; k >= 0; k--) mma_bf16(acc[ht][j], f[k], pa[ht][0], pa[ht][1]);
+                }
               }
-              uint32_t x[3], y[3];
-              split_bf16(w[0], w[1], x[0], x[1], x[2]);
-              split_bf16(w[2], w[3], y[0], y[1], y[2]);
-              if constexpr (TWO) mma_bf16(acc[j], pb, x[0], y[0]);
-#pragma unroll
-              for (int k = 2; k >= 0; k--) mma_bf16(acc[j], pa, x[k], y[k]);
             }
           }
         }
@@ -568,33 +620,25 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
     constexpr int kJ = D + 4;
     float *join = (float *)pool;
     sync();
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    {
-      float *o = join + (warp * 8 + gh) * kJ;
+#pragma unroll
+    for (int ht = 0; ht < HT; ht++) {
+      for (int o = 4; o < 32; o <<= 1) l[ht] += __shfl_xor_sync(0xffffffffu, l[ht], o);
+      if (ht * 4 + t >= nh) continue;
+      float *o = join + (warp * NH + ht * 4 + t) * kJ;
       const float f = I8 ? vlim * 0x1p-15f : 1.0f;
-      float x[NT][2];
 #pragma unroll
-      for (int j = 0; j < NT; j++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          x[j][e] = acc[j][e] + acc[j][2 + e];
-          if constexpr (NH == 4) x[j][e] += __shfl_xor_sync(0xffffffffu, x[j][e], 16);
-          x[j][e] *= f;
-        }
-      if (g < nh) {
+      for (int j = 0; j < NT; j++) {
+        const float x = (acc[ht][j][0] + acc[ht][j][1]) * f, y = (acc[ht][j][2] + acc[ht][j][3]) * f;
         if constexpr (I8) {
-#pragma unroll
-          for (int j = 0; j < NT; j += 2)
-            *(float4 *)(o + Sh::vdim(j, 2 * t)) = make_float4(x[j][0], x[j + 1][0], x[j][1], x[j + 1][1]);
+          *(float2 *)(o + Sh::vdim(j, 0, g)) = make_float2(x, y);
         } else {
-#pragma unroll
-          for (int j = 0; j < NT; j++) *(float2 *)(o + Sh::vdim(j, 2 * t)) = make_float2(x[j][0], x[j][1]);
+          o[Sh::vdim(j, 0, g)] = x;
+          o[Sh::vdim(j, 1, g)] = y;
         }
-        if (t == 0) {
-          o[D] = m;
-          o[D + 1] = l;
-        }
+      }
+      if (g == 0) {
+        o[D] = m[ht];
+        o[D + 1] = l[ht];
       }
     }
     sync();
@@ -607,13 +651,13 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, NH) * 4 / W) paged_
         M = o[D], L = o[D + 1], x = o[d];
       } else {
 #pragma unroll
-        for (int w = 0; w < W; w++) M = fmaxf(M, o[w * 8 * kJ + D]);
+        for (int w = 0; w < W; w++) M = fmaxf(M, o[w * NH * kJ + D]);
         const float mu = M == -INFINITY ? 0.0f : M;
 #pragma unroll
         for (int w = 0; w < W; w++) {
-          const float f = exp2_approx(o[w * 8 * kJ + D] - mu);
-          L = fmaf(o[w * 8 * kJ + D + 1], f, L);
-          x = fmaf(o[w * 8 * kJ + d], f, x);
+          const float f = exp2_approx(o[w * NH * kJ + D] - mu);
+          L = fmaf(o[w * NH * kJ + D + 1], f, L);
+          x = fmaf(o[w * NH * kJ + d], f, x);
         }
       }
       if (ns == 1) {

@@ -77,11 +77,11 @@ struct AttendKernel {
   void (*fn)(AttendArgs) = nullptr;
   int threads = 0, smem = 0, block = 0, per_sm[kMaxDevices] = {};
 };
-template <int KIND, int D, int NH, bool FAST, int W>
+template <int KIND, int D, int HT, bool FAST, int W>
 AttendKernel *attend_kernel_w() {
   static AttendKernel k = [] {
     AttendKernel x;
-    x.fn = paged_mma_kernel<KIND, D, NH, FAST, W>;
+    x.fn = paged_mma_kernel<KIND, D, HT, FAST, W>;
     x.threads = W * 32;
     x.smem = pm_smem<KIND, D, W>(FAST);
     x.block = PmShape<KIND, D, W>::kBlock;
@@ -89,20 +89,23 @@ AttendKernel *attend_kernel_w() {
   }();
   return &k;
 }
-template <int KIND, int D, int NH>
-AttendKernel *attend_kernel_n(bool fast, int warps) {
-  if (warps == 1) return fast ? attend_kernel_w<KIND, D, NH, true, 1>() : attend_kernel_w<KIND, D, NH, false, 1>();
-  if (warps == 2) return fast ? attend_kernel_w<KIND, D, NH, true, 2>() : attend_kernel_w<KIND, D, NH, false, 2>();
-  return fast ? attend_kernel_w<KIND, D, NH, true, 4>() : attend_kernel_w<KIND, D, NH, false, 4>();
+template <int KIND, int D, int HT>
+AttendKernel *attend_kernel_h(bool fast, int warps) {
+  if (warps == 1) return fast ? attend_kernel_w<KIND, D, HT, true, 1>() : attend_kernel_w<KIND, D, HT, false, 1>();
+  if (warps == 2) return fast ? attend_kernel_w<KIND, D, HT, true, 2>() : attend_kernel_w<KIND, D, HT, false, 2>();
+  return fast ? attend_kernel_w<KIND, D, HT, true, 4>() : attend_kernel_w<KIND, D, HT, false, 4>();
+}
+template <int KIND, int D>
+AttendKernel *attend_kernel_d(int heads, bool fast, int warps) {
+  return heads == 4 ? attend_kernel_h<KIND, D, 1>(fast, warps) : attend_kernel_h<KIND, D, 2>(fast, warps);
 }
 template <int KIND>
 AttendKernel *attend_kernel_k(int D, int heads, bool fast, int warps) {
-  constexpr int N = KIND == PM_I8 ? 8 : 4;  // int8 units have 8 heads
   switch (D) {
-    case 32: return heads == 4 ? attend_kernel_n<KIND, 32, N>(fast, warps) : attend_kernel_n<KIND, 32, 8>(fast, warps);
-    case 64: return heads == 4 ? attend_kernel_n<KIND, 64, N>(fast, warps) : attend_kernel_n<KIND, 64, 8>(fast, warps);
-    case 96: return heads == 4 ? attend_kernel_n<KIND, 96, N>(fast, warps) : attend_kernel_n<KIND, 96, 8>(fast, warps);
-    default: return heads == 4 ? attend_kernel_n<KIND, 128, N>(fast, warps) : attend_kernel_n<KIND, 128, 8>(fast, warps);
+    case 32: return attend_kernel_d<KIND, 32>(heads, fast, warps);
+    case 64: return attend_kernel_d<KIND, 64>(heads, fast, warps);
+    case 96: return attend_kernel_d<KIND, 96>(heads, fast, warps);
+    default: return attend_kernel_d<KIND, 128>(heads, fast, warps);
   }
 }
 // The kernel for a call, ready to launch on ctx's device.
@@ -292,7 +295,7 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   a.scale2 = (float)(scale * 1.4426950408889634);
   const size_t rows = (size_t)n_seqs * n_head;
   const int D = p->v.head_dim, G = n_head / p->v.n_kv_head;
-  a.unit_heads = p->v.kind != LLMQ_KV_QUANT8 && G <= 4 ? 4 : 8;
+  a.unit_heads = G <= 4 ? 4 : 8;
   a.head_chunks = (G + a.unit_heads - 1) / a.unit_heads;
   const long long units = (long long)n_seqs * p->v.n_kv_head * a.head_chunks;
   // Fewer warps a CTA for many units of short sequences, whose prologues and
