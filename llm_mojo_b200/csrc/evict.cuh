@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(EvictArgs a) {
   __shared__ int wsum[32];
   __shared__ int s_bin, s_need;
   const int row = blockIdx.x, b = row / a.c.n_kv_head % a.src.n_seqs, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int len = evict_len(a, b), n = min(len, a.budget);
   const float *w = a.w + row * a.w_stride;
   float *wout = a.wout + row * a.wout_stride;

@@ -82,6 +82,7 @@ constexpr int kStoreItems = 4;
 template <typename E, int D, bool VEC>
 __global__ void __launch_bounds__(256) paged_store_kernel(StoreArgs a) {
   constexpr int LG = D == 96 ? 32 : D / 4, kPer = 256 / LG;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x % LG, nh = a.c.n_kv_head;
   const long long i0 = ((long long)blockIdx.x * kPer + threadIdx.x / LG) * kStoreItems;
   const long long items = (long long)a.n_rows * nh * 2;
@@ -143,7 +144,7 @@ struct AttendArgs {
   float *stat;    // [n_seqs][n_head][2]: the maximum score M and the sum of 2^(score - M)
   // the split over positions (paged_mma.cuh)
   int chunk, splits, head_chunks, unit_heads;
-  float *part;   // [unit][split][unit_heads][D + 2]: sums, then M and L of each head
+  float *part;   // [unit][split][unit_heads][D + 4]: sums, then M and L of each head
   int *tickets;  // [unit], zero between launches
 };
 

@@ -171,7 +171,7 @@ template <int KIND, int D, int W>
 __host__ __device__ constexpr int pm_smem(bool fast) {
   typedef PmShape<KIND, D, W> Sh;
   constexpr int ring = W * Sh::kStages * Sh::kStage, join = W * 8 * (D + 4) * 4;
-  constexpr int fac = (8 * kPmJoin + (8 * D > W * 32 ? 8 * D : W * 32)) * 4;
+  constexpr int fac = (8 * kPmJoin + (8 * D > W * 128 ? 8 * D : W * 128)) * 4;
   constexpr int most = ring > join ? ring : join;
   return pm_rows_bytes<KIND, D, W>(fast) + (most > fac ? most : fac);
 }
@@ -202,6 +202,35 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
   const int b = unit / a.head_chunks / a.c.n_kv_head;
   const int G = a.n_head / a.c.n_kv_head, ps = a.c.page_size;
   const int h0 = kh * G + hc * NH, nh = min(NH, G - hc * NH);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // the query's rows, as they are: column g of the operand is a term of head g / 2
+  float xq[HT][NT][4];
+#pragma unroll
+  for (int ht = 0; ht < HT; ht++) {
+    const int h = ht * 4 + (g >> 1);
+    const float *q = a.q + (size_t)b * a.q_stride + (size_t)(h0 + h) * D;
+#pragma unroll
+    for (int k = 0; k < NT; k++) {
+      float(&x)[4] = xq[ht][k];
+      // int8: 4 dimensions in a row, bfloat16: 2 and 2
+      if (KIND != PM_F32 && a.q_vec) {
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (h < nh) {
+          if constexpr (I8) {
+            y = *(const float4 *)(q + Sh::kdim(k, 0, t));
+          } else {
+            const float2 y0 = *(const float2 *)(q + Sh::kdim(k, 0, t)), y1 = *(const float2 *)(q + Sh::kdim(k, 2, t));
+            y = make_float4(y0.x, y0.y, y1.x, y1.y);
+          }
+        }
+        x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = h < nh ? q[Sh::kdim(k, e, t)] : 0.0f;
+      }
+    }
+  }
+
   const int len = paged_len(a, b), ns = max(1, (len + a.chunk - 1) / a.chunk);
   if (split >= ns) return;
   const int p0 = split * a.chunk, p1 = min(len, p0 + a.chunk);  // the chunk's positions
@@ -238,83 +267,121 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
   const int half = I8 ? lane >> 3 & 1 : lane >> 4, vpiece = I8 ? lane >> 4 : lane >> 3 & 1;
   const int vmatrix0 = Sh::kVat + (half * 8 + (lane & 7)) * Sh::kPad + vpiece * 16;
 
-  {
-    // the query's operand, kept for the whole chunk: column g is a term of
-    // head g / 2, the first or the second (int8, bfloat16), qb the third of
-    // bfloat16 in the even columns
-    uint32_t qa[HT][NT][2], qb[HT][I8 ? 1 : NT][2];
-    float fs[HT], cb[HT];  // of the lane's own head t: the scores' factor, and (int8) where they start
+  const size_t first = a.c.row(a.layer, 0, kh, 0);
+  const char *kl = (const char *)a.c.k + first * Sh::kRow + (FAST ? lane * 16 : 0);
+  const char *vl = (const char *)a.c.v + first * Sh::kRow + (FAST ? lane * 16 : 0);
+  // int8 scales: a lane's piece of a tile's 16 + 16 (FAST), or of its positions
+  const float *scl = I8 ? (FAST ? (lane < 4 ? a.c.ks : a.c.vs) + first + (lane & 3) * 4
+                                : (lane < 16 ? a.c.ks : a.c.vs) + first)
+                        : nullptr;
+  int c0 = p0, n, ntiles;  // the run of positions whose rows are at hand
+  bool hole;               // whether any of them has no page
+  auto issue = [&](int tile0, int stage) {  // tiles tile0 .. tile0 + U - 1, as far as there are
 #pragma unroll
-    for (int ht = 0; ht < HT; ht++) {
-      const int h = ht * 4 + (g >> 1);
-      const float *q = a.q + (size_t)b * a.q_stride + (size_t)(h0 + h) * D;
-      float x[NT][4], mx = 0.0f;
-      const bool vec = a.q_vec;
+    for (int v = 0; v < U; v++) {
+      const int tile = U == 1 ? tile0 : min(tile0 + v, ntiles - 1);
+      const unsigned d = ring + stage * Sh::kStage + v * Sh::kTile;
+      const size_t at0 = FAST ? (size_t)max(rows[tile], 0) : 0;
+      const char *kt = kl + at0 * Sh::kRow, *vt = vl + at0 * Sh::kRow;
 #pragma unroll
-      for (int k = 0; k < NT; k++) {
-        // int8: 4 dimensions in a row, bfloat16: 2 and 2
-        if (KIND != PM_F32 && vec) {
-          float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (h < nh) {
-            if constexpr (I8) {
-              y = *(const float4 *)(q + Sh::kdim(k, 0, t));
-            } else {
-              const float2 y0 = *(const float2 *)(q + Sh::kdim(k, 0, t)), y1 = *(const float2 *)(q + Sh::kdim(k, 2, t));
-              y = make_float4(y0.x, y0.y, y1.x, y1.y);
-            }
-          }
-          x[k][0] = y.x, x[k][1] = y.y, x[k][2] = y.z, x[k][3] = y.w;
+      for (int i = 0; i < NC / 2; i++) {  // 16 NC pieces of K, and of V, 32 at a time
+        if constexpr (FAST) {
+          pm_copy16(d + piece_at(i), kt + i * 512);
+          pm_copy16(d + piece_at(i) + Sh::kVat, vt + i * 512);
         } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++) x[k][e] = h < nh ? q[Sh::kdim(k, e, t)] : 0.0f;
+          const int p = 32 * i + lane;
+          const size_t off = (size_t)max(rows[tile * 16 + p / NC], 0) * Sh::kRow + p % NC * 16;
+          pm_copy16(d + piece_at(i), kl + off);
+          pm_copy16(d + piece_at(i) + Sh::kVat, vl + off);
         }
-#pragma unroll
-        for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[k][e]));
       }
-      fs[ht] = a.scale2;
-      cb[ht] = 0.0f;
       if constexpr (I8) {
-        // the largest |q| of the head to [2^13, 2^14): the second terms reach 2^-38 of it
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const int e = min(max((int)(__float_as_uint(mx) >> 23), 1), 254) - 127;
-        const float up = pow2i(min(13 - e, 126)), down = a.scale2 * pow2i(max(e - 13, -126)) * 0x1p24f;
-        float sum = 0.0f;  // of the column's term
-#pragma unroll
-        for (int k = 0; k < NT; k++)
-#pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            uint32_t hi, lo;
-            split_f16(x[k][i] * up, x[k][i + 1] * up, hi, lo);
-            qa[ht][k][i / 2] = g & 1 ? lo : hi;
-            const float2 f = __half22float2(*(const __half2 *)&qa[ht][k][i / 2]);
-            sum += f.x + f.y;
-          }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);  // both terms
-        cb[ht] = -0x1p-17f * __shfl_sync(0xffffffffu, sum, 8 * t);
-        fs[ht] = __shfl_sync(0xffffffffu, down, 8 * t);
-      } else {
-#pragma unroll
-        for (int k = 0; k < NT; k++)
-#pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            uint32_t t0, t1, t2;
-            split_bf16(x[k][i], x[k][i + 1], t0, t1, t2);
-            qa[ht][k][i / 2] = g & 1 ? t1 : t0;
-            qb[ht][k][i / 2] = g & 1 ? 0u : t2;
-          }
+        if constexpr (FAST) {
+          if (lane < 8) pm_copy16(d + Sh::kSat + lane * 16, scl + at0);
+        } else {
+          pm_copy4(d + Sh::kSat + lane * 4, scl + max(rows[tile * 16 + (lane & 15)], 0));
+        }
       }
     }
+  };
+  // the run from c0 on: its rows, relative to this layer's and kv head's
+  // first, -1: no page; and the first copies
+  auto open_run = [&] {
+    n = min(p1 - c0, Sh::kRun), ntiles = (n + 15) / 16;
+    hole = false;
+    for (int i = tid; i < (FAST ? ntiles : ntiles * 16); i += W * 32) {
+      const int j = FAST ? i * 16 : i;
+      int row = -1;
+      if (j < n) {
+        const int pi = (c0 + j) / ps, page = a.t.page(b, pi);
+        if (page >= 0 && page < a.c.n_pages)
+          row = page * (a.c.n_kv_head * ps) + (c0 + j - pi * ps);
+        else
+          hole = true;
+      }
+      rows[i] = row;
+    }
+    if constexpr (W > 1)
+      hole = __syncthreads_or(hole);
+    else
+      hole = __any_sync(0xffffffffu, hole);
+#pragma unroll
+    for (int i = 0; i < S - 1; i++) {
+      if ((warp + i * W) * U < ntiles) issue((warp + i * W) * U, i);
+      commit();
+    }
+  };
+  open_run();
 
-    const size_t first = a.c.row(a.layer, 0, kh, 0);
-    const char *kl = (const char *)a.c.k + first * Sh::kRow + (FAST ? lane * 16 : 0);
-    const char *vl = (const char *)a.c.v + first * Sh::kRow + (FAST ? lane * 16 : 0);
-    // int8 scales: a lane's piece of a tile's 16 + 16 (FAST), or of its positions
-    const float *scl = I8 ? (FAST ? (lane < 4 ? a.c.ks : a.c.vs) + first + (lane & 3) * 4
-                                  : (lane < 16 ? a.c.ks : a.c.vs) + first)
-                          : nullptr;
+  // the query's operand, kept for the whole chunk: the first or the second
+  // term (int8, bfloat16), qb the third of bfloat16 in the even columns
+  uint32_t qa[HT][NT][2], qb[HT][I8 ? 1 : NT][2];
+  float fs[HT], cb[HT];  // of the lane's own head t: the scores' factor, and (int8) where they start
+#pragma unroll
+  for (int ht = 0; ht < HT; ht++) {
+    fs[ht] = a.scale2;
+    cb[ht] = 0.0f;
+    if constexpr (I8) {
+      // the largest |q| of the head to [2^13, 2^14): the second terms reach 2^-38 of it
+      float mx = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NT; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mx = fmaxf(mx, fabsf(xq[ht][k][i]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const int e = min(max((int)(__float_as_uint(mx) >> 23), 1), 254) - 127;
+      const float up = pow2i(min(13 - e, 126)), down = a.scale2 * pow2i(max(e - 13, -126)) * 0x1p24f;
+      float sum = 0.0f;  // of the column's term
+#pragma unroll
+      for (int k = 0; k < NT; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          uint32_t hi, lo;
+          split_f16(xq[ht][k][i] * up, xq[ht][k][i + 1] * up, hi, lo);
+          qa[ht][k][i / 2] = g & 1 ? lo : hi;
+          const float2 f = __half22float2(*(const __half2 *)&qa[ht][k][i / 2]);
+          sum += f.x + f.y;
+        }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);  // both terms
+      cb[ht] = -0x1p-17f * __shfl_sync(0xffffffffu, sum, 8 * t);
+      fs[ht] = __shfl_sync(0xffffffffu, down, 8 * t);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NT; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          uint32_t t0, t1, t2;
+          split_bf16(xq[ht][k][i], xq[ht][k][i + 1], t0, t1, t2);
+          qa[ht][k][i / 2] = g & 1 ? t1 : t0;
+          qb[ht][k][i / 2] = g & 1 ? 0u : t2;
+        }
+    }
+  }
+
+  {
     float acc[HT][NT][4], m[HT], l[HT], vlim = 0x1p-100f, vinv = 0x1p115f;
 #pragma unroll
     for (int ht = 0; ht < HT; ht++) {
@@ -326,61 +393,7 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
         for (int i = 0; i < 4; i++) acc[ht][j][i] = 0.0f;
     }
 
-    for (int c0 = p0; c0 < p1; c0 += Sh::kRun) {
-      const int n = min(p1 - c0, Sh::kRun), ntiles = (n + 15) / 16;  // the run
-      // its rows, relative to this layer's and kv head's first; -1: no page
-      bool hole = false;
-      if (c0 > p0) sync();
-      for (int i = tid; i < (FAST ? ntiles : ntiles * 16); i += W * 32) {
-        const int j = FAST ? i * 16 : i;
-        int row = -1;
-        if (j < n) {
-          const int pi = (c0 + j) / ps, page = a.t.page(b, pi);
-          if (page >= 0 && page < a.c.n_pages)
-            row = page * (a.c.n_kv_head * ps) + (c0 + j - pi * ps);
-          else
-            hole = true;
-        }
-        rows[i] = row;
-      }
-      if constexpr (W > 1)
-        hole = __syncthreads_or(hole);
-      else
-        hole = __any_sync(0xffffffffu, hole);
-
-      auto issue = [&](int tile0, int stage) {  // tiles tile0 .. tile0 + U - 1, as far as there are
-#pragma unroll
-        for (int v = 0; v < U; v++) {
-          const int tile = U == 1 ? tile0 : min(tile0 + v, ntiles - 1);
-          const unsigned d = ring + stage * Sh::kStage + v * Sh::kTile;
-          const size_t at0 = FAST ? (size_t)max(rows[tile], 0) : 0;
-          const char *kt = kl + at0 * Sh::kRow, *vt = vl + at0 * Sh::kRow;
-#pragma unroll
-          for (int i = 0; i < NC / 2; i++) {  // 16 NC pieces of K, and of V, 32 at a time
-            if constexpr (FAST) {
-              pm_copy16(d + piece_at(i), kt + i * 512);
-              pm_copy16(d + piece_at(i) + Sh::kVat, vt + i * 512);
-            } else {
-              const int p = 32 * i + lane;
-              const size_t off = (size_t)max(rows[tile * 16 + p / NC], 0) * Sh::kRow + p % NC * 16;
-              pm_copy16(d + piece_at(i), kl + off);
-              pm_copy16(d + piece_at(i) + Sh::kVat, vl + off);
-            }
-          }
-          if constexpr (I8) {
-            if constexpr (FAST) {
-              if (lane < 8) pm_copy16(d + Sh::kSat + lane * 16, scl + at0);
-            } else {
-              pm_copy4(d + Sh::kSat + lane * 4, scl + max(rows[tile * 16 + (lane & 15)], 0));
-            }
-          }
-        }
-      };
-#pragma unroll
-      for (int i = 0; i < S - 1; i++) {
-        if ((warp + i * W) * U < ntiles) issue((warp + i * W) * U, i);
-        commit();
-      }
+    for (;;) {
       int stage = 0;
       for (int tile = warp * U; tile < ntiles; tile += W * U) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
@@ -614,6 +627,10 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
+      c0 += Sh::kRun;
+      if (c0 >= p1) break;
+      sync();
+      open_run();
     }
 
     // join the warps: [warp][head][D sums, M, L, -, -] in the rings' place
@@ -642,7 +659,7 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
       }
     }
     sync();
-    constexpr int kStep = NH * (D + 2);  // floats of a partial result
+    constexpr int kStep = NH * kJ;  // floats of a partial result, laid out the same
     for (int i = tid; i < nh * D; i += W * 32) {
       const int h = i / D, d = i % D;
       const float *o = join + h * kJ;
@@ -667,7 +684,7 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
           a.stat[2 * ((size_t)b * a.n_head + h0 + h) + 1] = L;
         }
       } else {
-        float *part = a.part + ((size_t)unit * a.splits + split) * kStep + h * (D + 2);
+        float *part = a.part + ((size_t)unit * a.splits + split) * kStep + h * kJ;
         part[d] = x;
         if (d == 0) {
           part[D] = M;
@@ -692,7 +709,7 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
 #pragma unroll
       for (int i = 0; i < kN; i++) {
         const int k = i * 32 + lane;
-        const float *o = part + (size_t)k * kStep + h * (D + 2) + D;
+        const float *o = part + (size_t)k * kStep + h * kJ + D;
         mk[i] = k < ns ? __ldcg(o) : -INFINITY;
         lk[i] = k < ns ? __ldcg(o + 1) : 0.0f;
       }
@@ -713,26 +730,30 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
       }
     }
     sync();
-    const int no = nh * D, groups = max(1, W * 32 / no);
+    const int no = nh * D / 4, groups = max(1, W * 32 / no);  // four dimensions a thread
     for (int i = tid; i < no * groups; i += W * 32) {
-      const int grp = i / no, o = i % no, h = o / D;
-      const float *src = part + h * (D + 2) + o % D, *f = fac + h * kPmJoin;
-      float x = 0.0f;
+      const int grp = i / no, o = i % no * 4, h = o / D;
+      const float *src = part + h * kJ + o % D, *f = fac + h * kPmJoin;
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int k0 = grp; k0 < ns; k0 += 8 * groups) {
-        float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) y[j] = k0 + j * groups < ns ? __ldcg(src + (size_t)(k0 + j * groups) * kStep) : 0.0f;
+        float4 y[8];
 #pragma unroll
         for (int j = 0; j < 8; j++)
-          if (k0 + j * groups < ns) x = fmaf(y[j], f[k0 + j * groups], x);
+          if (k0 + j * groups < ns) y[j] = __ldcg((const float4 *)(src + (size_t)(k0 + j * groups) * kStep));
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (k0 + j * groups < ns) {
+            const float w = f[k0 + j * groups];
+            x.x = fmaf(y[j].x, w, x.x), x.y = fmaf(y[j].y, w, x.y), x.z = fmaf(y[j].z, w, x.z), x.w = fmaf(y[j].w, w, x.w);
+          }
       }
-      sums[i] = x;
+      *(float4 *)(sums + grp * nh * D + o) = x;
     }
     sync();
-    for (int i = tid; i < no; i += W * 32) {
+    for (int i = tid; i < nh * D; i += W * 32) {
       const int h = i / D, d = i % D;
       float x = sums[i];
-      for (int grp = 1; grp < groups; grp++) x += sums[grp * no + i];
+      for (int grp = 1; grp < groups; grp++) x += sums[grp * nh * D + i];
       const float L = s_stat[h][1];
       a.out[(size_t)b * a.out_stride + (size_t)(h0 + h) * D + d] = L == 0.0f ? 0.0f : x / L;
       if (a.stat && d == 0) {

@@ -71,6 +71,23 @@ llmq_status paged_check(llmq_ctx *ctx, const llmq_paged *p, int layer0, int n_la
   return LLMQ_OK;
 }
 
+// A launch that may begin while the kernel before it on the stream ends; its
+// own first step waits for that kernel (griddepcontrol.wait).
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*k)(P...), dim3 grid, unsigned threads, cudaStream_t s, size_t smem, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k, static_cast<P>(args)...);
+}
+
 // A kernel with its shared memory and how many of its CTAs an SM holds
 // (asked for once per device).
 struct AttendKernel {
@@ -127,14 +144,11 @@ llmq_status attend_kernel(llmq_ctx *ctx, const AttendArgs &a, int warps, AttendK
 }
 
 template <typename E, int D>
-void launch_store_d(const StoreArgs &a, bool vec, unsigned grid, cudaStream_t s) {
-  if (vec)
-    paged_store_kernel<E, D, true><<<grid, 256, 0, s>>>(a);
-  else
-    paged_store_kernel<E, D, false><<<grid, 256, 0, s>>>(a);
+cudaError_t launch_store_d(const StoreArgs &a, bool vec, unsigned grid, cudaStream_t s) {
+  return launch_after(vec ? paged_store_kernel<E, D, true> : paged_store_kernel<E, D, false>, dim3(grid), 256, s, 0, a);
 }
 template <typename E>
-void launch_store_e(const StoreArgs &a, bool vec, unsigned grid, cudaStream_t s) {
+cudaError_t launch_store_e(const StoreArgs &a, bool vec, unsigned grid, cudaStream_t s) {
   switch (a.c.head_dim) {
     case 32: return launch_store_d<E, 32>(a, vec, grid, s);
     case 64: return launch_store_d<E, 64>(a, vec, grid, s);
@@ -143,33 +157,13 @@ void launch_store_e(const StoreArgs &a, bool vec, unsigned grid, cudaStream_t s)
   }
 }
 cudaError_t launch_store(const StoreArgs &a, bool vec, unsigned grid, cudaStream_t s) {
-  if (a.c.kind == LLMQ_KV_QUANT8)
-    launch_store_e<PgInt8>(a, vec, grid, s);
-  else if (a.c.kind == LLMQ_KV_BF16)
-    launch_store_e<PgBf16>(a, vec, grid, s);
-  else
-    launch_store_e<PgF32>(a, vec, grid, s);
-  return cudaGetLastError();
-}
-
-// A launch that may start while the kernel before it on the stream ends; its
-// own first step waits for that kernel (griddepcontrol.wait).
-template <typename... P, typename... A>
-cudaError_t launch_after(void (*k)(P...), dim3 grid, unsigned threads, cudaStream_t s, A... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, static_cast<P>(args)...);
+  if (a.c.kind == LLMQ_KV_QUANT8) return launch_store_e<PgInt8>(a, vec, grid, s);
+  if (a.c.kind == LLMQ_KV_BF16) return launch_store_e<PgBf16>(a, vec, grid, s);
+  return launch_store_e<PgF32>(a, vec, grid, s);
 }
 
 cudaError_t launch_move(const EvictArgs &a, int tiles, unsigned grid, cudaStream_t s) {
-  auto go = [&](void (*k)(EvictArgs, int)) { return launch_after(k, dim3(grid), 256, s, a, tiles); };
+  auto go = [&](void (*k)(EvictArgs, int)) { return launch_after(k, dim3(grid), 256, s, 0, a, tiles); };
   switch (a.c.head_dim * elem_bytes(a.c.kind) / 16) {
     case 2: return go(evict_move_kernel<2>);
     case 4: return go(evict_move_kernel<4>);
@@ -318,7 +312,7 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   const unsigned g = grid1(units * a.splits);
   if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many sequences for one call");
   ServeWs *ws;
-  const size_t parts = a.splits > 1 ? (size_t)g * a.unit_heads * (D + 2) : 0, floats = parts + (weights_out ? rows * (a.score_stride + 2) + 4 : 0);
+  const size_t parts = a.splits > 1 ? (size_t)g * a.unit_heads * (D + 4) : 0, floats = parts + (weights_out ? rows * (a.score_stride + 2) + 4 : 0);
   if ((st = serve_ws(ctx, floats * 4, a.splits > 1 ? (size_t)units : 0, &ws)) != LLMQ_OK) return st;
   a.part = (float *)ws->buf;
   a.tickets = ws->tickets;
@@ -326,12 +320,11 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
     a.scores = a.part + (parts + 3) / 4 * 4;  // 16-byte aligned rows
     a.stat = a.scores + rows * a.score_stride;
   }
-  k->fn<<<g, k->threads, k->smem, ctx->stream>>>(a);
-  CKL();
+  CK(launch_after(k->fn, dim3(g), k->threads, ctx->stream, k->smem, a));
   if (weights_out) {
     const dim3 wg((max_len + 1023) / 1024, (unsigned)std::min((long long)n_seqs * p->v.n_kv_head, 65535LL));
     const bool vec = ((uintptr_t)weights | (uintptr_t)weights_out) % 16 == 0 && weights_stride % 4 == 0;
-    CK(launch_after(vec ? paged_weights_kernel<true> : paged_weights_kernel<false>, wg, 256, ctx->stream, a, max_len,
+    CK(launch_after(vec ? paged_weights_kernel<true> : paged_weights_kernel<false>, wg, 256, ctx->stream, 0, a, max_len,
                     weights, weights_out, weights_stride));
   }
   return LLMQ_OK;
@@ -360,11 +353,8 @@ llmq_status llmq_paged_evict(llmq_ctx *ctx, llmq_paged *p, int layer0, int n_lay
   const int tiles = (std::min(budget, max_len) + kEvPos - 1) / kEvPos;
   const unsigned g = grid1(rows), gm = g ? grid1(rows * tiles) : 0;
   if (!g || !gm) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
-  if ((uintptr_t)weights % 16 == 0 && weights_stride % 4 == 0)
-    evict_select_kernel<true><<<g, kEvThreads, 0, ctx->stream>>>(a);
-  else
-    evict_select_kernel<false><<<g, kEvThreads, 0, ctx->stream>>>(a);
-  CKL();
+  const bool vec = (uintptr_t)weights % 16 == 0 && weights_stride % 4 == 0;
+  CK(launch_after(vec ? evict_select_kernel<true> : evict_select_kernel<false>, dim3(g), kEvThreads, ctx->stream, 0, a));
   CK(launch_move(a, tiles, gm, ctx->stream));
   return LLMQ_OK;
 }
