@@ -14,12 +14,12 @@ struct DecodeState;
 }
 
 // The serving operators' device workspace on one stream: buf holds partial
-// results within a call, tickets are zero between calls.
+// results within a call, zeros (tickets, counts) is all zero between calls.
 struct ServeWs {
   void *buf = nullptr;
   size_t bytes = 0;
-  int *tickets = nullptr;
-  size_t n_tickets = 0;
+  void *zeros = nullptr;
+  size_t zero_bytes = 0;
 };
 
 struct llmq_ctx {

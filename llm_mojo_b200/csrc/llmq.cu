@@ -400,7 +400,7 @@ llmq_status llmq_destroy(llmq_ctx *ctx) {
     if (q) cudaFree(q);
   for (auto &w : ctx->serve_ws) {
     if (w.second.buf) cudaFree(w.second.buf);
-    if (w.second.tickets) cudaFree(w.second.tickets);
+    if (w.second.zeros) cudaFree(w.second.zeros);
   }
   if (ctx->own) cudaStreamDestroy(ctx->own);
   delete ctx;

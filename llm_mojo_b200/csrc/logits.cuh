@@ -1,5 +1,15 @@
 // logits.cuh -- the rules between the head and the sampler: penalties for
 // repeated tokens, biases and a mask of the allowed tokens.
+//
+// Each logit is read and written once, so memory bounds the call; the history
+// touches a few percent of a row's tokens. Two ways, by size:
+//  - small calls, one launch: each CTA counts its tile's tokens of the
+//    history in shared memory beside its logits (logit_rules_kernel);
+//  - large calls: the history and the biases scatter into per-token cells and
+//    a bitmap of the touched tokens (logit_count_kernel); one pass streams the
+//    others without waiting for anything (logit_stream_kernel); the touched
+//    ones follow, each claimed through its bit by one of its occurrences
+//    (logit_touch_kernel). Cells and bits are zero again afterwards.
 #pragma once
 
 #include "common.cuh"
@@ -19,9 +29,13 @@ struct RuleArgs {
   const float *bias_val;
   const uint32_t *mask;
   long long mask_stride;
-  unsigned long long *best;  // [n][tiles] (ordered value, ~id) of each tile's largest logit
-  int *tickets;              // [n], zero between launches
+  unsigned long long *best;  // small calls: [n][tiles] each tile's largest key; large ones: [n], zero between calls
+  int *tickets;              // [n], zero between calls
   int *argmax;               // or null
+  // large calls, rows r0 on; zero between calls
+  unsigned *bits;  // [n][words] touched tokens
+  uint2 *cells;    // [n][V]: x as the counts below, y the bias
+  int words, parts;  // parts: CTAs of a row's history and biases
 };
 
 // (ordered value, ~id): the largest key is the first of the largest logits;
@@ -41,6 +55,12 @@ struct RuleTile {
   float4 x[NG];
 };
 
+// The 32 bits of row's tokens v .. v + 31 (v from -3), those outside [0, V) 0.
+__device__ __forceinline__ unsigned rule_bits(const uint32_t *row, int v, int V) {
+  const uint32_t w0 = row[max(v, 0) >> 5], w1 = row[min(v + 31, V - 1) >> 5];
+  return v >= 0 ? __funnelshift_r(w0, w1, v & 31) : w0 << -v;
+}
+
 // Each warp has a run of 32 VPT logits, a lane VPT / 4 groups of four,
 // aligned to 16 bytes whatever the row's start (a row of odd length starts
 // anywhere: the first group may begin before it).
@@ -57,11 +77,7 @@ __device__ __forceinline__ void rule_open(const RuleArgs &a, int item, RuleTile<
   const int v = w.t0 + (threadIdx.x >> 5) * 32 * VPT + lane * 32;
   if (lane < VPT && v < w.hi && v + 32 > w.lo) {
     w.mine = 0xffffffffu;
-    if (a.mask) {
-      const uint32_t *m = a.mask + w.r * a.mask_stride;
-      const uint32_t w0 = m[max(v, 0) >> 5], w1 = m[min(v + 31, a.V - 1) >> 5];
-      w.mine = v >= 0 ? __funnelshift_r(w0, w1, v & 31) : w0 << -v;
-    }
+    if (a.mask) w.mine = rule_bits(a.mask + w.r * a.mask_stride, v, a.V);
     if (v < 0) w.mine &= 0xffffffffu << -v;
     if (v + 32 > w.hi) w.mine &= 0xffffffffu >> (v + 32 - w.hi);
   }
@@ -111,6 +127,7 @@ __global__ void __launch_bounds__(NTH) logit_rules_kernel(RuleArgs a) {
   unsigned *cnt = rsm;                             // bit 31: in the prompt; the rest: times in the answer
   float *bias = (float *)(rsm + (a.ids ? T : 0));  // of the tile
   const int tid = threadIdx.x, lane = tid & 31, r = blockIdx.x / a.tiles;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   // the first quads of each thread's history, on their way with the logits
   const int *ids = a.ids ? a.ids + r * a.ids_stride : nullptr;
   const int first = (int)((4 - (((uintptr_t)ids >> 2) & 3)) & 3);  // ids before a 16-byte boundary
@@ -250,6 +267,147 @@ __global__ void __launch_bounds__(NTH) logit_rules_kernel(RuleArgs a) {
     }
   }
   if (last && lane == 0) a.argmax[r] = k ? (int)~(unsigned)k : -1;
+}
+
+// ---- large calls -------------------------------------------------------------
+
+constexpr int kTouchThreads = 512, kTouchPer = 2048;  // history ids and biases of a CTA
+
+// A row's entry i: history ids, then biases. Returns the token, or -1.
+__device__ __forceinline__ int rule_entry(const RuleArgs &a, int r, int i, int H, int b0) {
+  const int id = i < H ? a.ids[r * a.ids_stride + i] : a.bias_ids[b0 + i - H];
+  return id >= 0 && id < a.V ? id : -1;
+}
+// How many entries row r has; of them H are history, and its biases start at b0.
+__device__ __forceinline__ int rule_entries(const RuleArgs &a, int r, int &H, int &b0) {
+  H = a.ids ? min(max(0, a.n_ids[r]), a.max_ids) : 0;
+  b0 = a.bias_off ? max(a.bias_off[r], 0) : 0;
+  return H + (a.bias_off ? max(min(a.bias_off[r + 1], a.n_bias) - b0, 0) : 0);
+}
+
+// grid n * parts
+__global__ void __launch_bounds__(kTouchThreads) logit_count_kernel(RuleArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int r = blockIdx.x / a.parts;
+  int H, b0;
+  const int total = rule_entries(a, r, H, b0), P = a.n_prompt ? a.n_prompt[r] : 0;
+  for (int i = blockIdx.x % a.parts * kTouchThreads + threadIdx.x; i < total; i += a.parts * kTouchThreads) {
+    const int id = rule_entry(a, r, i, H, b0);
+    if (id < 0) continue;
+    uint2 *cell = a.cells + (size_t)r * a.V + id;
+    if (i < H) {
+      if (i >= P)
+        atomicAdd(&cell->x, 1u);
+      else
+        atomicOr(&cell->x, 0x80000000u);
+    } else {
+      // the first of equal ids adds them up, in order
+      const int j = b0 + i - H, end = b0 + total - H;
+      if (j > b0 && a.bias_ids[j - 1] == id) continue;
+      float s = a.bias_val[j];
+      for (int e = j + 1; e < end && a.bias_ids[e] == id; e++) s += a.bias_val[e];
+      cell->y = __float_as_uint(s);
+    }
+    atomicOr(&a.bits[(size_t)r * a.words + (id >> 5)], 1u << (id & 31));
+  }
+}
+
+// Every token that nothing touched: allowed ones as they are, others
+// -infinity. One CTA per (row, tile of 4096), as in logit_rules_kernel but
+// for a thread's own groups only: no barrier, no shared memory. The largest
+// logit goes to the row's key by one atomic maximum a warp.
+__global__ void __launch_bounds__(256) logit_stream_kernel(RuleArgs a) {
+  constexpr int VPT = 16, NG = VPT / 4;
+  const int lane = threadIdx.x & 31;
+  RuleTile<NG> w;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  rule_open<256, VPT>(a, blockIdx.x, w);
+  unsigned touched = 0;
+  const int v0 = w.t0 + (threadIdx.x >> 5) * 32 * VPT;
+  if (a.bits && lane < VPT && v0 + lane * 32 < w.hi && v0 + lane * 32 + 32 > w.lo)
+    touched = rule_bits(a.bits + (size_t)w.r * a.words, v0 + lane * 32, a.V);
+  w.mine &= ~touched;
+  rule_load<VPT>(a, w);
+  float *outr = a.out + w.r * a.out_stride;
+  const bool vec_out = (((uintptr_t)(outr + w.t0) >> 2) & 3) == 0;
+  float bv = -INFINITY;
+  int bt = INT_MAX;
+#pragma unroll
+  for (int i = 0; i < NG; i++) {
+    const int v = v0 + i * 128 + lane * 4;
+    const unsigned skip = __shfl_sync(0xffffffffu, touched, i * 4 + (lane >> 3)) >> (lane & 7) * 4 & 15u;
+    const unsigned keep = rule_keep(w.mine, i);
+    if (v >= w.hi || v + 3 < w.lo) continue;
+    float y[4] = {w.x[i].x, w.x[i].y, w.x[i].z, w.x[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (!(keep >> j & 1u)) y[j] = -INFINITY;
+      if (y[j] > bv) {
+        bv = y[j];
+        bt = v + j;
+      }
+    }
+    if (vec_out && v >= w.lo && v + 3 < w.hi && !skip) {
+      *(float4 *)(outr + v) = make_float4(y[0], y[1], y[2], y[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (v + j >= w.lo && v + j < w.hi && !(skip >> j & 1u)) outr[v + j] = y[j];
+    }
+  }
+  if (!a.argmax) return;
+  const unsigned long long k = rule_key(bv, bt);
+  const unsigned top = __reduce_max_sync(0xffffffffu, (unsigned)(k >> 32));
+  if (!top) return;
+  const unsigned first = __reduce_max_sync(0xffffffffu, (unsigned)(k >> 32) == top ? (unsigned)k : 0u);
+  if (lane == 0) atomicMax(&a.best[w.r], ((unsigned long long)top << 32) | first);
+}
+
+// The touched tokens, and the row's argmax. grid n * parts; the row's last
+// part finishes it.
+__global__ void __launch_bounds__(kTouchThreads) logit_touch_kernel(RuleArgs a) {
+  __shared__ unsigned long long red[kTouchThreads / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int r = blockIdx.x / a.parts, lane = threadIdx.x & 31;
+  int H, b0;
+  const int total = rule_entries(a, r, H, b0);
+  const float rep = a.repetition ? a.repetition[r] : 1.0f, fr = a.frequency ? a.frequency[r] : 0.0f,
+              pr = a.presence ? a.presence[r] : 0.0f;
+  unsigned long long best = 0;
+  for (int i = blockIdx.x % a.parts * kTouchThreads + threadIdx.x; i < total; i += a.parts * kTouchThreads) {
+    const int id = rule_entry(a, r, i, H, b0);
+    if (id < 0) continue;
+    unsigned *word = &a.bits[(size_t)r * a.words + (id >> 5)];
+    if (!(*(volatile unsigned *)word >> (id & 31) & 1u)) continue;  // done by another occurrence
+    if (!(atomicAnd(word, ~(1u << (id & 31))) >> (id & 31) & 1u)) continue;
+    uint2 *cell = a.cells + (size_t)r * a.V + id;
+    const uint2 c = __ldcg(cell);
+    float y = a.x[r * a.x_stride + id];
+    const unsigned co = c.x & 0x7fffffffu;
+    if (c.x) y = y > 0.0f ? y / rep : y * rep;
+    if (co) y = (y - fr * (float)co) - pr;
+    y += __uint_as_float(c.y);
+    if (a.mask && !(a.mask[r * a.mask_stride + (id >> 5)] >> (id & 31) & 1u)) y = -INFINITY;
+    a.out[r * a.out_stride + id] = y;
+    *cell = make_uint2(0u, 0u);
+    best = max(best, rule_key(y, id));
+  }
+  if (!a.argmax) return;
+  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (lane == 0) red[threadIdx.x >> 5] = best;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int i = 1; i < kTouchThreads / 32; i++) best = max(best, red[i]);
+  if (a.parts > 1) {
+    atomicMax(&a.best[r], best);
+    __threadfence();
+    if (atomicAdd(&a.tickets[r], 1) != a.parts - 1) return;
+    __threadfence();
+    a.tickets[r] = 0;
+  }
+  best = max(best, __ldcg(&a.best[r]));
+  a.best[r] = 0;
+  a.argmax[r] = best ? (int)~(unsigned)best : -1;
 }
 
 }  // namespace llmq

@@ -2,6 +2,7 @@
 // and eviction, and the rules on logits (include/llmq.h).
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 #include <mutex>
 
 #include "context.cuh"
@@ -19,42 +20,34 @@ struct llmq_paged {
 
 namespace {
 
-// The stream's workspace with at least `bytes` of buffer and `tickets` zeroed
-// tickets. Growing waits for the stream, whose queued calls use the old one.
-llmq_status serve_ws(llmq_ctx *ctx, size_t bytes, size_t tickets, ServeWs **out) {
-  ServeWs &w = ctx->serve_ws[ctx->stream];
-  if (w.bytes >= bytes && w.n_tickets >= tickets) {
-    *out = &w;
-    return LLMQ_OK;
-  }
+// Grows one of the workspace's buffers.
+llmq_status serve_grow(llmq_ctx *ctx, void **buf, size_t *have, size_t bytes, bool zero) {
+  if (*have >= bytes) return LLMQ_OK;
   cudaStreamCaptureStatus cap;
   CK(cudaStreamIsCapturing(ctx->stream, &cap));
   if (cap != cudaStreamCaptureStatusNone)
     return fail(ctx, LLMQ_ERR_INVALID, "the serving workspace grows on first use: run the call once before capturing it");
-  CK(cudaStreamSynchronize(ctx->stream));
-  if (w.bytes < bytes) {
-    if (w.buf) cudaFree(w.buf);
-    w.buf = nullptr;
-    w.bytes = 0;
-    if (cudaMalloc(&w.buf, bytes) != cudaSuccess) {
-      cudaGetLastError();
-      return fail(ctx, LLMQ_ERR_NOMEM, "serving workspace of " + std::to_string(bytes) + " bytes");
-    }
-    w.bytes = bytes;
+  CK(cudaStreamSynchronize(ctx->stream));  // queued calls use the old one
+  if (*buf) cudaFree(*buf);
+  *buf = nullptr;
+  *have = 0;
+  if (cudaMalloc(buf, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ctx, LLMQ_ERR_NOMEM, "serving workspace of " + std::to_string(bytes) + " bytes");
   }
-  if (w.n_tickets < tickets) {
-    if (w.tickets) cudaFree(w.tickets);
-    w.tickets = nullptr;
-    w.n_tickets = 0;
-    if (cudaMalloc(&w.tickets, tickets * sizeof(int)) != cudaSuccess) {
-      cudaGetLastError();
-      return fail(ctx, LLMQ_ERR_NOMEM, "serving tickets");
-    }
-    CK(cudaMemsetAsync(w.tickets, 0, tickets * sizeof(int), ctx->stream));
-    w.n_tickets = tickets;
-  }
-  *out = &w;
+  if (zero) CK(cudaMemsetAsync(*buf, 0, bytes, ctx->stream));
+  *have = bytes;
   return LLMQ_OK;
+}
+
+// The stream's workspace with at least `bytes` of buffer and `zeros` bytes
+// that are zero.
+llmq_status serve_ws(llmq_ctx *ctx, size_t bytes, size_t zeros, ServeWs **out) {
+  ServeWs &w = ctx->serve_ws[ctx->stream];
+  llmq_status st = serve_grow(ctx, &w.buf, &w.bytes, bytes, false);
+  if (st == LLMQ_OK) st = serve_grow(ctx, &w.zeros, &w.zero_bytes, zeros, true);
+  *out = &w;
+  return st;
 }
 
 constexpr int kMaxDevices = 64;
@@ -174,6 +167,55 @@ cudaError_t launch_move(const EvictArgs &a, int tiles, unsigned grid, cudaStream
     case 24: return go(evict_move_kernel<24>);
     default: return go(evict_move_kernel<32>);
   }
+}
+
+// One launch: tiles of 4096 logits, or smaller ones while the call has fewer
+// CTAs than two per SM.
+llmq_status rules_small(llmq_ctx *ctx, RuleArgs &a) {
+  int vpt = 16;
+  constexpr int nth = 256;
+  while (vpt > 4 && (long long)a.n * ((a.V + 3 + nth * vpt - 1) / (nth * vpt)) < 2 * ctx->num_sms) vpt /= 2;
+  const int T = nth * vpt;
+  a.tiles = (a.V + 3 + T - 1) / T;  // a row may start 3 logits past a 16-byte boundary
+  const unsigned g = (unsigned)(a.n * a.tiles);
+  if (a.argmax && a.tiles > 1) {
+    ServeWs *ws;
+    const llmq_status st = serve_ws(ctx, (size_t)g * 8, (size_t)a.n * 4, &ws);
+    if (st != LLMQ_OK) return st;
+    a.best = (unsigned long long *)ws->buf;
+    a.tickets = (int *)ws->zeros;
+  }
+  const size_t sm = (size_t)T * 4 * ((a.ids ? 1 : 0) + (a.bias_off ? 1 : 0));
+  CK(launch_after(vpt == 16 ? logit_rules_kernel<nth, 16> : vpt == 8 ? logit_rules_kernel<nth, 8> : logit_rules_kernel<nth, 4>,
+                  dim3(g), nth, ctx->stream, sm, a));
+  return LLMQ_OK;
+}
+
+constexpr long long kCellBytes = 256LL << 20;  // of the large calls' cells at a time
+
+llmq_status rules_large(llmq_ctx *ctx, RuleArgs &a) {
+  const bool touch = a.ids || a.bias_off;
+  a.words = (a.V + 31) / 32;
+  a.tiles = (a.V + 3 + 4095) / 4096;
+  const long long most = (a.ids ? a.max_ids : 0) + (a.bias_off ? std::min(a.n_bias, a.V) : 0);
+  a.parts = (int)std::max(1LL, std::min(most / kTouchPer, 64LL));
+  if (touch || a.argmax) {
+    const size_t best = (size_t)a.n * 8, tick = ((size_t)a.n * 4 + 15) / 16 * 16;
+    const size_t cells = touch ? (size_t)a.n * a.V * 8 : 0, bits = touch ? (size_t)a.n * a.words * 4 : 0;
+    ServeWs *ws;
+    const llmq_status st = serve_ws(ctx, 0, best + tick + cells + bits, &ws);
+    if (st != LLMQ_OK) return st;
+    a.best = (unsigned long long *)ws->zeros;
+    a.tickets = (int *)((char *)ws->zeros + best);
+    if (touch) {
+      a.cells = (uint2 *)((char *)ws->zeros + best + tick);
+      a.bits = (unsigned *)((char *)a.cells + cells);
+    }
+  }
+  if (touch) CK(launch_after(logit_count_kernel, dim3(a.n * a.parts), kTouchThreads, ctx->stream, 0, a));
+  CK(launch_after(logit_stream_kernel, dim3(a.n * a.tiles), 256, ctx->stream, 0, a));
+  if (touch || a.argmax) CK(launch_after(logit_touch_kernel, dim3(a.n * a.parts), kTouchThreads, ctx->stream, 0, a));
+  return LLMQ_OK;
 }
 
 // Blocks of a one-dimensional grid, or 0 when there would be too many.
@@ -313,9 +355,9 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many sequences for one call");
   ServeWs *ws;
   const size_t parts = a.splits > 1 ? (size_t)g * a.unit_heads * (D + 4) : 0, floats = parts + (weights_out ? rows * (a.score_stride + 2) + 4 : 0);
-  if ((st = serve_ws(ctx, floats * 4, a.splits > 1 ? (size_t)units : 0, &ws)) != LLMQ_OK) return st;
+  if ((st = serve_ws(ctx, floats * 4, a.splits > 1 ? (size_t)units * 4 : 0, &ws)) != LLMQ_OK) return st;
   a.part = (float *)ws->buf;
-  a.tickets = ws->tickets;
+  a.tickets = (int *)ws->zeros;
   if (weights_out) {
     a.scores = a.part + (parts + 3) / 4 * 4;  // 16-byte aligned rows
     a.stat = a.scores + rows * a.score_stride;
@@ -372,34 +414,33 @@ llmq_status llmq_process_logits(llmq_ctx *ctx, const float *logits, long long lo
   if ((u.bias_offsets != nullptr) != (u.bias_ids != nullptr) || (u.bias_ids != nullptr) != (u.bias_values != nullptr))
     return fail(ctx, LLMQ_ERR_INVALID, "a bias needs offsets, ids and values");
   if ((u.bias_ids && u.n_bias < 0) || (u.mask && u.mask_stride < 0)) return fail(ctx, LLMQ_ERR_INVALID, "negative size");
+  if (!grid1((long long)n * ((V + 1026) / 1024))) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
   CK(cudaSetDevice(ctx->device));
-  // tiles of 4096 logits; smaller ones while the call has fewer CTAs than two
-  // per SM
-  int vpt = 16;
-  constexpr int nth = 256;
-  while (vpt > 4 && (long long)n * ((V + 3 + nth * vpt - 1) / (nth * vpt)) < 2 * ctx->num_sms) vpt /= 2;
-  const int T = nth * vpt;
-  const int tiles = (V + 3 + T - 1) / T;  // a row may start 3 logits past a 16-byte boundary
-  const unsigned g = grid1((long long)n * tiles);
-  if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
-  const size_t sm = (size_t)T * 4 * ((u.ids ? 1 : 0) + (u.bias_ids ? 1 : 0));
-  RuleArgs a{logits, out, logits_stride, out_stride, n, V, tiles, u.repetition, u.presence, u.frequency, u.ids,
-             u.n_ids, u.n_prompt, u.ids_stride, u.max_ids, u.n_bias, u.bias_offsets, u.bias_ids, u.bias_values, u.mask,
-             u.mask_stride, nullptr, nullptr, argmax};
-  if (argmax && tiles > 1) {
-    ServeWs *ws;
-    llmq_status st = serve_ws(ctx, (size_t)g * 8, n, &ws);
+  RuleArgs a{};
+  a.x = logits, a.x_stride = logits_stride, a.out = out, a.out_stride = out_stride, a.n = n, a.V = V;
+  a.repetition = u.repetition, a.presence = u.presence, a.frequency = u.frequency;
+  a.ids = u.ids, a.n_ids = u.n_ids, a.n_prompt = u.n_prompt, a.ids_stride = u.ids_stride, a.max_ids = u.max_ids;
+  a.bias_off = u.bias_offsets, a.bias_ids = u.bias_ids, a.bias_val = u.bias_values, a.n_bias = u.n_bias;
+  a.mask = u.mask, a.mask_stride = u.mask_stride, a.argmax = argmax;
+  const long long thr = getenv("THR") ? atoll(getenv("THR")) : 2000000;
+  if ((long long)n * V < thr) return rules_small(ctx, a);
+  // Groups of rows whose cells fit in kCellBytes
+  const int group = (int)std::min((long long)n, std::max(1LL, kCellBytes / 8 / V));
+  for (int r0 = 0; r0 < n; r0 += group) {
+    RuleArgs g = a;
+    g.n = std::min(group, n - r0);
+    g.x += r0 * a.x_stride, g.out += r0 * a.out_stride;
+    if (a.repetition) g.repetition += r0;
+    if (a.presence) g.presence += r0;
+    if (a.frequency) g.frequency += r0;
+    if (a.ids) g.ids += r0 * a.ids_stride, g.n_ids += r0;
+    if (a.n_prompt) g.n_prompt += r0;
+    if (a.bias_off) g.bias_off += r0;
+    if (a.mask) g.mask += r0 * a.mask_stride;
+    if (argmax) g.argmax += r0;
+    const llmq_status st = rules_large(ctx, g);
     if (st != LLMQ_OK) return st;
-    a.best = (unsigned long long *)ws->buf;
-    a.tickets = ws->tickets;
   }
-  if (vpt == 16)
-    logit_rules_kernel<nth, 16><<<g, nth, sm, ctx->stream>>>(a);
-  else if (vpt == 8)
-    logit_rules_kernel<nth, 8><<<g, nth, sm, ctx->stream>>>(a);
-  else
-    logit_rules_kernel<nth, 4><<<g, nth, sm, ctx->stream>>>(a);
-  CKL();
   return LLMQ_OK;
 }
 

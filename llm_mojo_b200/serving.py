@@ -12,11 +12,14 @@ after, as the kernels layer's are.
 from __future__ import annotations
 
 import ctypes as C
-import math
 from dataclasses import dataclass
 
-from ._lib import KV_BF16, KV_F32, KV_QUANT8, check, lib
+import torch
+
+from ._lib import KV_BF16, KV_F32, KV_QUANT8, OK, check, lib
 from .tensor import Context
+
+F32, I32 = torch.float32, torch.int32
 
 KINDS = {"int8": KV_QUANT8, "bf16": KV_BF16, "f32": KV_F32}
 
@@ -32,42 +35,38 @@ class _Array:
 
 def _check(ctx: Context, name: str, t, dtype, ndim: int, inner: int = 1):
     """t as the call takes it: on the context's device, `dtype`, `ndim`
-    dimensions of which the last `inner` are contiguous."""
-    if t.get_device() != ctx.device:
-        raise ValueError(f"{name} must be on cuda:{ctx.device}, not {t.device}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-    if t.dim() != ndim:
-        raise ValueError(f"{name} must have {ndim} dimensions, not {t.dim()}")
-    want = 1
-    for i in range(ndim - 1, ndim - 1 - inner, -1):
-        if t.shape[i] != 1 and t.stride(i) != want:
-            raise ValueError(f"{name}: the last {inner} dimensions must be contiguous")
-        want *= t.shape[i]
+    dimensions of which the last `inner` are contiguous. Returns its address."""
+    if t.dtype is not dtype or t.dim() != ndim or t.get_device() != ctx.device or not (
+            t.is_contiguous() or _rows_contiguous(t, inner)):
+        raise ValueError(f"{name} must be {dtype} on cuda:{ctx.device} with {ndim} dimensions, the last {inner} "
+                         f"contiguous; not {t.dtype} on {t.device}, {tuple(t.shape)} with strides {t.stride()}")
     return t.data_ptr()
 
 
+def _rows_contiguous(t, inner: int) -> bool:
+    want = 1
+    for n, stride in zip(reversed(t.shape[-inner:]), reversed(t.stride()[-inner:])):
+        if n != 1 and stride != want:
+            return False
+        want *= n
+    return True
+
+
 def _shape(name: str, t, want):
-    if tuple(t.shape) != tuple(want):
+    if t.shape != want:
         raise ValueError(f"{name} must be {tuple(want)}, not {tuple(t.shape)}")
 
 
-class _Ordered:
-    """Orders a call with torch's current stream."""
-
-    def __init__(self, ctx: Context):
-        self.ctx = ctx
-
-    def __enter__(self):
-        import torch
-
-        self.same = self.ctx.on_torch_stream()
-        if not self.same:
-            torch.cuda.current_stream(self.ctx.device).synchronize()
-
-    def __exit__(self, *exc):
-        if not self.same:
-            self.ctx.sync()
+def _call(ctx: Context, fn, *args):
+    """fn(ctx, *args) in order with torch's current stream."""
+    same = ctx.on_torch_stream()
+    if not same:
+        torch.cuda.current_stream(ctx.device).synchronize()
+    status = fn(ctx.h, *args)
+    if status != OK:
+        check(status, ctx.h)
+    if not same:
+        ctx.sync()
 
 
 class PagedKVCache:
@@ -81,13 +80,11 @@ class PagedKVCache:
 
     def __init__(self, ctx: Context, kind: str, n_layer: int, n_pages: int, page_size: int, n_kv_head: int,
                  head_dim: int):
-        import torch
-
         if kind not in KINDS:
             raise ValueError(f"unknown paged cache kind {kind}")
         self.ctx, self.kind = ctx, kind
         self.n_layer, self.n_pages, self.page_size = n_layer, n_pages, page_size
-        self.n_kv_head, self.head_dim = n_kv_head, head_dim
+        self.n_kv_head, self.head_dim, self.scale = n_kv_head, head_dim, 1.0 / max(head_dim, 1) ** 0.5
         h = C.c_void_p()
         check(lib().llmq_paged_create(ctx.h, KINDS[kind], n_layer, n_pages, page_size, n_kv_head, head_dim,
                                       C.byref(h)), ctx.h)
@@ -112,22 +109,20 @@ class PagedKVCache:
         """Stores rows k, v [n, n_kv_head, head_dim] (any row stride: the
         columns of a projection will do) at positions pos [n] of sequences seq
         [n] (None: row r is sequence r). A negative position is skipped."""
-        import torch
-
         ctx, n = self.ctx, k.shape[0]
-        kp, vp = _check(ctx, "k", k, torch.float32, 3, 2), _check(ctx, "v", v, torch.float32, 3, 2)
-        _shape("k", k, (n, self.n_kv_head, self.head_dim))
-        _shape("v", v, (n, self.n_kv_head, self.head_dim))
-        pp = _check(ctx, "pos", pos, torch.int32, 1)
+        kp, vp = _check(ctx, "k", k, F32, 3, 2), _check(ctx, "v", v, F32, 3, 2)
+        rows = (n, self.n_kv_head, self.head_dim)
+        _shape("k", k, rows)
+        _shape("v", v, rows)
+        pp = _check(ctx, "pos", pos, I32, 1)
         _shape("pos", pos, (n,))
         sp = None
         if seq is not None:
-            sp = _check(ctx, "seq", seq, torch.int32, 1)
+            sp = _check(ctx, "seq", seq, I32, 1)
             _shape("seq", seq, (n,))
-        tp = _check(ctx, "table", table, torch.int32, 2)
-        with _Ordered(ctx):
-            check(lib().llmq_paged_store(ctx.h, self.h, layer, kp, k.stride(0), vp, v.stride(0), sp, pp, n, tp,
-                                         table.stride(0), table.shape[1], table.shape[0]), ctx.h)
+        tp = _check(ctx, "table", table, I32, 2)
+        _call(ctx, lib().llmq_paged_store, self.h, layer, kp, k.stride(0), vp, v.stride(0), sp, pp, n, tp,
+              table.stride(0), table.shape[1], table.shape[0])
 
     def attend(self, layer: int, q, table, lens, max_len: int, scale: float | None = None, out=None, weights=None,
                weights_out=None):
@@ -137,42 +132,37 @@ class PagedKVCache:
         and/or weights_out ([n_seqs, n_kv_head, >= max_len], weights_out =
         weights for in place), weights_out = weights + the softmax weights
         summed over each kv head's query heads."""
-        import torch
-
         ctx = self.ctx
-        qp = _check(ctx, "q", q, torch.float32, 3, 2)
-        n, n_head = q.shape[0], q.shape[1]
-        _shape("q", q, (n, n_head, self.head_dim))
+        qp = _check(ctx, "q", q, F32, 3, 2)
+        n, n_head, dim = q.shape
+        if dim != self.head_dim:
+            raise ValueError(f"q must have {self.head_dim} dimensions a head, not {dim}")
         if out is None:
-            out = torch.empty((n, n_head, self.head_dim), dtype=torch.float32, device=q.device)
-        op = _check(ctx, "out", out, torch.float32, 3, 2)
-        _shape("out", out, q.shape)
-        tp, lp = _check(ctx, "table", table, torch.int32, 2), _check(ctx, "lens", lens, torch.int32, 1)
-        _shape("lens", lens, (n,))
-        if table.shape[0] != n:
-            raise ValueError("table and q must have a row per sequence")
+            out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
+            op = out.data_ptr()
+        else:
+            op = _check(ctx, "out", out, F32, 3, 2)
+            _shape("out", out, q.shape)
+        tp, lp = _check(ctx, "table", table, I32, 2), _check(ctx, "lens", lens, I32, 1)
+        if lens.shape[0] != n or table.shape[0] != n:
+            raise ValueError("table, lens and q must have a row per sequence")
         wp = wop = None
         stride = 0
         if weights is not None and weights_out is None:
             raise ValueError("weights without weights_out")
         if weights_out is not None:
-            wop = _check(ctx, "weights_out", weights_out, torch.float32, 3)
+            wop = _check(ctx, "weights_out", weights_out, F32, 3)
             stride = weights_out.stride(1)
             for name, w in (("weights", weights), ("weights_out", weights_out)):
                 if w is None:
                     continue
-                p = _check(ctx, name, w, torch.float32, 3)
-                if tuple(w.shape[:2]) != (n, self.n_kv_head) or w.shape[2] < max_len:
+                wp = _check(ctx, name, w, F32, 3) if name == "weights" else wp
+                if w.shape[0] != n or w.shape[1] != self.n_kv_head or w.shape[2] < max_len:
                     raise ValueError(f"{name} must be [{n}, {self.n_kv_head}, >= {max_len}]")
                 if w.stride(1) != stride or (n > 1 and w.stride(0) != stride * self.n_kv_head):
                     raise ValueError("weights and weights_out must have the same evenly spaced rows")
-                if name == "weights":
-                    wp = p
-        if scale is None:
-            scale = 1.0 / math.sqrt(self.head_dim)
-        with _Ordered(ctx):
-            check(lib().llmq_paged_attend(ctx.h, self.h, layer, qp, q.stride(0), op, out.stride(0), n, n_head, tp,
-                                          table.stride(0), table.shape[1], lp, max_len, scale, wp, wop, stride), ctx.h)
+        _call(ctx, lib().llmq_paged_attend, self.h, layer, qp, q.stride(0), op, out.stride(0), n, n_head, tp,
+              table.stride(0), table.shape[1], lp, max_len, self.scale if scale is None else scale, wp, wop, stride)
         return out
 
     def evict(self, table, lens, max_len: int, weights, budget: int, dst_table, sinks: int = 0, recent: int = 0,
@@ -183,16 +173,14 @@ class PagedKVCache:
         dst_table's pages, which must not be the source's. Returns (kept
         positions int32 [n_layers, n_seqs, n_kv_head, budget], -1 past the
         kept; their weights, 0 past them; the new lengths int32 [n_seqs])."""
-        import torch
-
         ctx, n = self.ctx, table.shape[0]
         n_layers = self.n_layer - layer0 if n_layers is None else n_layers
-        tp, lp = _check(ctx, "table", table, torch.int32, 2), _check(ctx, "lens", lens, torch.int32, 1)
-        dp = _check(ctx, "dst_table", dst_table, torch.int32, 2)
+        tp, lp = _check(ctx, "table", table, I32, 2), _check(ctx, "lens", lens, I32, 1)
+        dp = _check(ctx, "dst_table", dst_table, I32, 2)
         _shape("lens", lens, (n,))
         if dst_table.shape[0] != n:
             raise ValueError("table and dst_table must have a row per sequence")
-        wp = _check(ctx, "weights", weights, torch.float32, 4)
+        wp = _check(ctx, "weights", weights, F32, 4)
         if tuple(weights.shape[:3]) != (n_layers, n, self.n_kv_head) or weights.shape[3] < max_len:
             raise ValueError(f"weights must be [{n_layers}, {n}, {self.n_kv_head}, >= {max_len}]")
         ws = weights.stride(2)
@@ -202,13 +190,10 @@ class PagedKVCache:
         if budget <= 0:
             raise ValueError("budget must be positive")
         rows = (n_layers, n, self.n_kv_head, budget)
-        kept = torch.empty(rows, dtype=torch.int32, device=weights.device)
-        wout = torch.empty(rows, dtype=torch.float32, device=weights.device)
-        lens_out = torch.empty(n, dtype=torch.int32, device=weights.device)
-        with _Ordered(ctx):
-            check(lib().llmq_paged_evict(ctx.h, self.h, layer0, n_layers, n, tp, table.stride(0), table.shape[1], lp, max_len,
-                                         wp, ws, budget, sinks, recent, dp, dst_table.stride(0), dst_table.shape[1],
-                                         kept.data_ptr(), wout.data_ptr(), budget, lens_out.data_ptr()), ctx.h)
+        kept, wout, lens_out = lens.new_empty(rows), weights.new_empty(rows), torch.empty_like(lens)
+        _call(ctx, lib().llmq_paged_evict, self.h, layer0, n_layers, n, tp, table.stride(0), table.shape[1], lp, max_len,
+              wp, ws, budget, sinks, recent, dp, dst_table.stride(0), dst_table.shape[1], kept.data_ptr(),
+              wout.data_ptr(), budget, lens_out.data_ptr())
         return kept, wout, lens_out
 
     def free(self):
@@ -264,31 +249,40 @@ class LogitRules:
     mask: object = None
 
     def _struct(self, ctx: Context, n: int, V: int) -> _Rules:
-        import torch
-
         r = _Rules()
-        for name, dtype in (("repetition", torch.float32), ("presence", torch.float32), ("frequency", torch.float32),
-                            ("n_ids", torch.int32), ("n_prompt", torch.int32)):
-            t = getattr(self, name)
-            if t is not None:
-                setattr(r, name, _check(ctx, name, t, dtype, 1))
-                _shape(name, t, (n,))
+
+        def per_row(name, t, dtype):
+            p = _check(ctx, name, t, dtype, 1)
+            if t.shape[0] != n:
+                raise ValueError(f"{name} must have a value per row of logits")
+            return p
+
+        if self.repetition is not None:
+            r.repetition = per_row("repetition", self.repetition, F32)
+        if self.presence is not None:
+            r.presence = per_row("presence", self.presence, F32)
+        if self.frequency is not None:
+            r.frequency = per_row("frequency", self.frequency, F32)
+        if self.n_ids is not None:
+            r.n_ids = per_row("n_ids", self.n_ids, I32)
+        if self.n_prompt is not None:
+            r.n_prompt = per_row("n_prompt", self.n_prompt, I32)
         if self.ids is not None:
             if self.ids.shape[0] != n:
                 raise ValueError("ids must have a row per row of logits")
             # an empty tensor has no address: any valid one will do for no elements
-            r.ids = _check(ctx, "ids", self.ids, torch.int32, 2) or r.n_ids
+            r.ids = _check(ctx, "ids", self.ids, I32, 2) or r.n_ids
             r.ids_stride, r.max_ids = self.ids.stride(0), self.ids.shape[1]
         if self.bias is not None:
             off, ids, val = self.bias
-            r.bias_offsets = _check(ctx, "bias offsets", off, torch.int32, 1)
-            r.bias_ids = _check(ctx, "bias ids", ids, torch.int32, 1) or r.bias_offsets
-            r.bias_values = _check(ctx, "bias values", val, torch.float32, 1) or r.bias_offsets
+            r.bias_offsets = _check(ctx, "bias offsets", off, I32, 1)
+            r.bias_ids = _check(ctx, "bias ids", ids, I32, 1) or r.bias_offsets
+            r.bias_values = _check(ctx, "bias values", val, F32, 1) or r.bias_offsets
             _shape("bias offsets", off, (n + 1,))
             _shape("bias values", val, ids.shape)
-            r.n_bias = ids.numel()
+            r.n_bias = ids.shape[0]
         if self.mask is not None:
-            r.mask = _check(ctx, "mask", self.mask, torch.int32, 2)
+            r.mask = _check(ctx, "mask", self.mask, I32, 2)
             if self.mask.shape[0] != n or self.mask.shape[1] < (V + 31) // 32:
                 raise ValueError(f"mask must be [{n}, >= {(V + 31) // 32}]")
             r.mask_stride = self.mask.stride(0)
@@ -299,19 +293,18 @@ def process_logits(ctx: Context, logits, rules: LogitRules, out=None, argmax=Non
     """The rules on logits [n, V]: returns (out [n, V], argmax int32 [n]: the
     first index of each row's largest logit, -1 where nothing is left). out
     may be logits."""
-    import torch
-
-    lp = _check(ctx, "logits", logits, torch.float32, 2)
+    lp = _check(ctx, "logits", logits, F32, 2)
     n, V = logits.shape
     if out is None:
-        out = torch.empty((n, V), dtype=torch.float32, device=logits.device)
-    op = _check(ctx, "out", out, torch.float32, 2)
-    _shape("out", out, (n, V))
+        out = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty((n, V))
+        op = out.data_ptr()
+    else:
+        op = _check(ctx, "out", out, F32, 2)
+        _shape("out", out, (n, V))
     if argmax is None:
-        argmax = torch.empty(n, dtype=torch.int32, device=logits.device)
-    ap = _check(ctx, "argmax", argmax, torch.int32, 1)
+        argmax = logits.new_empty(n, dtype=I32)
+    ap = _check(ctx, "argmax", argmax, I32, 1)
     _shape("argmax", argmax, (n,))
-    r = rules._struct(ctx, n, V)
-    with _Ordered(ctx):
-        check(lib().llmq_process_logits(ctx.h, lp, logits.stride(0), op, out.stride(0), n, V, C.byref(r), ap), ctx.h)
+    _call(ctx, lib().llmq_process_logits, lp, logits.stride(0), op, out.stride(0), n, V,
+          C.byref(rules._struct(ctx, n, V)), ap)
     return out, argmax

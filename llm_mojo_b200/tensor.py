@@ -19,6 +19,14 @@ from ._lib import check, lib
 CUDA_STREAM_LEGACY = 1  # cudaStreamLegacy
 
 
+def torch_stream(device: int) -> int:
+    """The handle of torch's current stream."""
+    import torch
+
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without the stream object, 1 us less
+    return raw(device) if raw else torch.cuda.current_stream(device).cuda_stream
+
+
 def _ptr(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
 
@@ -43,16 +51,12 @@ class Context:
     def use_torch_stream(self):
         """Issues the context's work on torch's current stream (the legacy
         default stream, whose torch handle is 0, as cudaStreamLegacy)."""
-        import torch
-
-        self.set_stream(torch.cuda.current_stream(self.device).cuda_stream or CUDA_STREAM_LEGACY)
+        self.set_stream(torch_stream(self.device) or CUDA_STREAM_LEGACY)
 
     def on_torch_stream(self) -> bool:
         """Whether the context's work is ordered with torch's current stream
         because it is issued on it."""
-        import torch
-
-        return self.stream == (torch.cuda.current_stream(self.device).cuda_stream or CUDA_STREAM_LEGACY)
+        return self.stream == (torch_stream(self.device) or CUDA_STREAM_LEGACY)
 
     def close(self):
         if self.h:
