@@ -169,55 +169,6 @@ cudaError_t launch_move(const EvictArgs &a, int tiles, unsigned grid, cudaStream
   }
 }
 
-// One launch: tiles of 4096 logits, or smaller ones while the call has fewer
-// CTAs than two per SM.
-llmq_status rules_small(llmq_ctx *ctx, RuleArgs &a) {
-  int vpt = 16;
-  constexpr int nth = 256;
-  while (vpt > 4 && (long long)a.n * ((a.V + 3 + nth * vpt - 1) / (nth * vpt)) < 2 * ctx->num_sms) vpt /= 2;
-  const int T = nth * vpt;
-  a.tiles = (a.V + 3 + T - 1) / T;  // a row may start 3 logits past a 16-byte boundary
-  const unsigned g = (unsigned)(a.n * a.tiles);
-  if (a.argmax && a.tiles > 1) {
-    ServeWs *ws;
-    const llmq_status st = serve_ws(ctx, (size_t)g * 8, (size_t)a.n * 4, &ws);
-    if (st != LLMQ_OK) return st;
-    a.best = (unsigned long long *)ws->buf;
-    a.tickets = (int *)ws->zeros;
-  }
-  const size_t sm = (size_t)T * 4 * ((a.ids ? 1 : 0) + (a.bias_off ? 1 : 0));
-  CK(launch_after(vpt == 16 ? logit_rules_kernel<nth, 16> : vpt == 8 ? logit_rules_kernel<nth, 8> : logit_rules_kernel<nth, 4>,
-                  dim3(g), nth, ctx->stream, sm, a));
-  return LLMQ_OK;
-}
-
-constexpr long long kCellBytes = 256LL << 20;  // of the large calls' cells at a time
-
-llmq_status rules_large(llmq_ctx *ctx, RuleArgs &a) {
-  const bool touch = a.ids || a.bias_off;
-  a.words = (a.V + 31) / 32;
-  a.tiles = (a.V + 3 + 4095) / 4096;
-  const long long most = (a.ids ? a.max_ids : 0) + (a.bias_off ? std::min(a.n_bias, a.V) : 0);
-  a.parts = (int)std::max(1LL, std::min(most / kTouchPer, 64LL));
-  if (touch || a.argmax) {
-    const size_t best = (size_t)a.n * 8, tick = ((size_t)a.n * 4 + 15) / 16 * 16;
-    const size_t cells = touch ? (size_t)a.n * a.V * 8 : 0, bits = touch ? (size_t)a.n * a.words * 4 : 0;
-    ServeWs *ws;
-    const llmq_status st = serve_ws(ctx, 0, best + tick + cells + bits, &ws);
-    if (st != LLMQ_OK) return st;
-    a.best = (unsigned long long *)ws->zeros;
-    a.tickets = (int *)((char *)ws->zeros + best);
-    if (touch) {
-      a.cells = (uint2 *)((char *)ws->zeros + best + tick);
-      a.bits = (unsigned *)((char *)a.cells + cells);
-    }
-  }
-  if (touch) CK(launch_after(logit_count_kernel, dim3(a.n * a.parts), kTouchThreads, ctx->stream, 0, a));
-  CK(launch_after(logit_stream_kernel, dim3(a.n * a.tiles), 256, ctx->stream, 0, a));
-  if (touch || a.argmax) CK(launch_after(logit_touch_kernel, dim3(a.n * a.parts), kTouchThreads, ctx->stream, 0, a));
-  return LLMQ_OK;
-}
-
 // Blocks of a one-dimensional grid, or 0 when there would be too many.
 unsigned grid1(long long n) { return n > 0 && n <= INT_MAX ? (unsigned)n : 0u; }
 
@@ -422,25 +373,27 @@ llmq_status llmq_process_logits(llmq_ctx *ctx, const float *logits, long long lo
   a.ids = u.ids, a.n_ids = u.n_ids, a.n_prompt = u.n_prompt, a.ids_stride = u.ids_stride, a.max_ids = u.max_ids;
   a.bias_off = u.bias_offsets, a.bias_ids = u.bias_ids, a.bias_val = u.bias_values, a.n_bias = u.n_bias;
   a.mask = u.mask, a.mask_stride = u.mask_stride, a.argmax = argmax;
-  const long long thr = getenv("THR") ? atoll(getenv("THR")) : 2000000;
-  if ((long long)n * V < thr) return rules_small(ctx, a);
-  // Groups of rows whose cells fit in kCellBytes
-  const int group = (int)std::min((long long)n, std::max(1LL, kCellBytes / 8 / V));
-  for (int r0 = 0; r0 < n; r0 += group) {
-    RuleArgs g = a;
-    g.n = std::min(group, n - r0);
-    g.x += r0 * a.x_stride, g.out += r0 * a.out_stride;
-    if (a.repetition) g.repetition += r0;
-    if (a.presence) g.presence += r0;
-    if (a.frequency) g.frequency += r0;
-    if (a.ids) g.ids += r0 * a.ids_stride, g.n_ids += r0;
-    if (a.n_prompt) g.n_prompt += r0;
-    if (a.bias_off) g.bias_off += r0;
-    if (a.mask) g.mask += r0 * a.mask_stride;
-    if (argmax) g.argmax += r0;
-    const llmq_status st = rules_large(ctx, g);
+  // tiles of 4096 logits, or smaller ones while the call has fewer CTAs than
+  // two per SM
+  int vpt = getenv("VPT") ? atoi(getenv("VPT")) : 16;
+  constexpr int nth = 256;
+  while (vpt > 4 && (long long)n * ((V + 3 + nth * vpt - 1) / (nth * vpt)) < 2 * ctx->num_sms) vpt /= 2;
+  const int T = nth * vpt;
+  a.tiles = (V + 3 + T - 1) / T;  // a row may start 3 logits past a 16-byte boundary
+  const int keys = a.tiles * (nth / 32);
+  const int thr = getenv("THR") ? atoi(getenv("THR")) : 2;
+  const bool follow = argmax && (long long)n * a.tiles >= thr * ctx->num_sms;  // a second launch rather than tickets
+  if (argmax) {
+    ServeWs *ws;
+    const llmq_status st = serve_ws(ctx, (size_t)n * keys * 8, follow ? 0 : (size_t)n * 4, &ws);
     if (st != LLMQ_OK) return st;
+    a.best = (unsigned long long *)ws->buf;
+    a.tickets = follow ? nullptr : (int *)ws->zeros;
   }
+  const size_t sm = (size_t)T * 4 * ((a.ids ? 1 : 0) + (a.bias_off ? 1 : 0));
+  CK(launch_after(vpt == 16 ? logit_rules_kernel<nth, 16> : vpt == 8 ? logit_rules_kernel<nth, 8> : logit_rules_kernel<nth, 4>,
+                  dim3(n * a.tiles), nth, ctx->stream, sm, a));
+  if (follow) CK(launch_after(logit_argmax_kernel, dim3((n + 3) / 4), 128, ctx->stream, 0, a.best, keys, argmax, n));
   return LLMQ_OK;
 }
 
