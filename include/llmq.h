@@ -342,6 +342,9 @@ typedef struct llmq_paged llmq_paged;
 llmq_status llmq_paged_create(llmq_ctx *ctx, int kind, int n_layer, int n_pages, int page_size, int n_kv_head,
                               int head_dim, llmq_paged **out);
 llmq_status llmq_paged_free(llmq_paged *p);
+/* The cache's kind and sizes. Any pointer may be NULL. */
+llmq_status llmq_paged_shape(const llmq_paged *p, int *kind, int *n_layer, int *n_pages, int *page_size, int *n_kv_head,
+                             int *head_dim);
 /* The pool's device buffers (ks, vs: NULL without scales). Any pointer may be
  * NULL. */
 llmq_status llmq_paged_buffers(const llmq_paged *p, void **k, void **v, float **ks, float **vs);
@@ -358,7 +361,8 @@ llmq_status llmq_paged_store(llmq_ctx *ctx, llmq_paged *p, int layer, const floa
 /* Attention of one new token per sequence: for sequence b and query head h
  * (kv head h / (n_head / n_kv_head)), out = sum_j softmax_j(scale * q . k_j)
  * v_j over the positions j < lens_dev[b] whose page exists; 0 where there is
- * none. Lengths are cut to max_len, which sizes the launch, and to the table.
+ * none. Lengths are cut to max_len (at most 2^30), which sizes the launch, and
+ * to the table. Keys and values are finite.
  * q_dev, out_dev: [n_head][head_dim] rows, q_stride / out_stride floats
  * apart. With weights_out_dev, the softmax weights are accumulated per kv
  * head: weights_out[b][kv head][j] = weights[b][kv head][j] + the sum of its
@@ -415,6 +419,22 @@ typedef struct llmq_logit_rules {
  * V <= 2^24. The struct is on the host and read during the call. */
 llmq_status llmq_process_logits(llmq_ctx *ctx, const float *logits_dev, long long logits_stride, float *out_dev,
                                 long long out_stride, int n, int V, const llmq_logit_rules *rules, int *argmax_dev);
+
+/* One decode step of B sequences with a paged cache in place of the batch's
+ * own: token tokens_dev[b] with position embedding positions_dev[b], its key
+ * and value stored in every layer at cache position slots_dev[b], attention
+ * over the first lens_dev[b] <= max_len positions (the new one among them),
+ * logits into logits_dev [B][V]. After evictions a sequence's cache is
+ * shorter than its text, so the two positions differ. weights_dev, if not
+ * NULL: the accumulated softmax weights [n_layer][B][n_head] in rows
+ * weights_stride floats apart, added to in place (a new position's must be 0
+ * before its step). The cache needs the model's layers, heads and head size.
+ * Ids and positions outside the model's are cut to it. Asynchronous on the
+ * context's stream; wait errors of the matmuls show at the next llmq_sync. */
+llmq_status llmq_batch_paged_step(llmq_ctx *ctx, llmq_batch *b, llmq_paged *p, int B, const int *tokens_dev,
+                                  const int *positions_dev, const int *slots_dev, const int *table_dev,
+                                  long long table_stride, int table_cols, const int *lens_dev, int max_len,
+                                  float *weights_dev, long long weights_stride, float *logits_dev);
 
 #ifdef __cplusplus
 }

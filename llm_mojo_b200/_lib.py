@@ -83,10 +83,12 @@ SIGNATURES = {
     "llmq_model_profile_read": (I, [P, P, P, I, I]),
     "llmq_paged_create": (I, [P, I, I, I, I, I, I, PP]),
     "llmq_paged_free": (I, [P]),
+    "llmq_paged_shape": (I, [P, P, P, P, P, P, P]),
     "llmq_paged_buffers": (I, [P, PP, PP, PP, PP]),
     "llmq_paged_store": (I, [P, P, I, P, LL, P, LL, P, P, I, P, LL, I, I]),
     "llmq_paged_attend": (I, [P, P, I, P, LL, P, LL, I, I, P, LL, I, P, I, C.c_float, P, P, LL]),
     "llmq_paged_evict": (I, [P, P, I, I, I, P, LL, I, P, I, P, LL, I, I, I, P, LL, I, P, P, LL, P]),
+    "llmq_batch_paged_step": (I, [P, P, P, I, P, P, P, P, LL, I, P, I, P, LL, P]),
     "llmq_process_logits": (I, [P, P, LL, P, LL, I, I, P, P]),
 }
 

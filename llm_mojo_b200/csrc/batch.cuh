@@ -596,4 +596,16 @@ __global__ void embed_batch_kernel(WeightView head, const float *wpe, float *x, 
   }
 }
 
+// The same with a position per sequence; ids and positions cut to the model.
+__global__ void embed_at_kernel(WeightView head, const float *wpe, float *x, const int *tokens, const int *pos, int max_pos) {
+  const int b = blockIdx.x, C = head.cols, gpr = head.cols / head.group;
+  const int token = min(max(tokens[b], 0), head.rows - 1), p = min(max(pos[b], 0), max_pos - 1);
+  for (int i = threadIdx.x; i < C; i += blockDim.x) {
+    const size_t gi = (size_t)token * gpr + i / head.group;
+    const float s = half_bits_to_float(head.scale[gi]);
+    const float v = (float)(code_at(head, token, i) - (int)head.zp[gi]) * s;
+    x[(size_t)b * C + i] = v + wpe[(size_t)p * C + i];
+  }
+}
+
 }  // namespace llmq

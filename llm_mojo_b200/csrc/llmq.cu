@@ -1,5 +1,6 @@
 // C ABI of the B200 quantized-matmul hot path (include/llmq.h).
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <map>
@@ -2715,6 +2716,47 @@ llmq_status llmq_batch_generate_async(llmq_ctx *ctx, llmq_batch *bt, const int *
   CK(cudaSetDevice(ctx->device));
   CK(cudaMemcpyAsync(bt->tokens, prompts_dev, (size_t)B * n_prompt * 4, cudaMemcpyDeviceToDevice, ctx->stream));
   return batch_run(bt, B, n_prompt, steps, ids_dev);
+}
+
+llmq_status llmq_batch_paged_step(llmq_ctx *ctx, llmq_batch *bt, llmq_paged *p, int B, const int *tokens,
+                                  const int *positions, const int *slots, const int *table, long long table_stride,
+                                  int table_cols, const int *lens, int max_len, float *weights, long long weights_stride,
+                                  float *logits) {
+  if (!ctx || !bt || !p || !tokens || !positions || !slots || !table || !lens || !logits)
+    return fail(ctx, LLMQ_ERR_INVALID, "null argument");
+  if (B <= 0 || B > bt->max_seqs) return fail(ctx, LLMQ_ERR_INVALID, "bad batch size");
+  llmq_model *m = bt->m;
+  const int C = m->C, HS = C / m->n_head;
+  int layers = 0, heads = 0, dim = 0;
+  llmq_paged_shape(p, nullptr, &layers, nullptr, nullptr, &heads, &dim);
+  if (layers < m->n_layer || heads != m->n_head || dim != HS)
+    return fail(ctx, LLMQ_ERR_INVALID, "the paged cache has not the model's layers, heads and head size");
+  if (weights && weights_stride < max_len) return fail(ctx, LLMQ_ERR_INVALID, "weights_stride below max_len");
+  CK(cudaSetDevice(ctx->device));
+  cudaStream_t s = ctx->stream;
+  ctx->tc_used = true;  // the GEMMs' waits report through the context's error word
+  embed_at_kernel<<<B, 256, 0, s>>>(m->head->view(), m->wpe(), bt->x, tokens, positions, 1024);
+  CKL();
+  llmq_status st;
+  for (int l = 0; l < m->n_layer; l++) {
+    const llmq_weight *const *w = &m->mats[4 * l];
+    if ((st = batch_linear(bt, w[0], bt->x, m->vec(l, 0), m->vec(l, 1), m->vec(l, 2), bt->qkv, B, EPI_BIAS, s)))
+      return st;
+    if ((st = llmq_paged_store(ctx, p, l, bt->qkv + C, 3 * C, bt->qkv + 2 * C, 3 * C, nullptr, slots, B, table,
+                               table_stride, table_cols, B)))
+      return st;
+    float *wl = weights ? weights + (size_t)l * B * m->n_head * weights_stride : nullptr;
+    if ((st = llmq_paged_attend(ctx, p, l, bt->qkv, 3 * C, bt->att, C, B, m->n_head, table, table_stride, table_cols,
+                                lens, max_len, 1.0f / sqrtf((float)HS), wl, wl, weights_stride)))
+      return st;
+    if ((st = batch_linear(bt, w[1], bt->att, nullptr, nullptr, m->vec(l, 3), bt->x, B, EPI_BIAS | EPI_RESID, s)))
+      return st;
+    if ((st = batch_linear(bt, w[2], bt->x, m->vec(l, 4), m->vec(l, 5), m->vec(l, 6), bt->fc, B, EPI_BIAS | EPI_GELU, s)))
+      return st;
+    if ((st = batch_linear(bt, w[3], bt->fc, nullptr, nullptr, m->vec(l, 7), bt->x, B, EPI_BIAS | EPI_RESID, s)))
+      return st;
+  }
+  return batch_linear(bt, m->head, bt->x, m->lnf_w(), m->lnf_b(), nullptr, logits, B, 0, s);
 }
 
 llmq_status llmq_batch_generate(llmq_ctx *ctx, llmq_batch *bt, const int *prompts, int B, int n_prompt, int steps,

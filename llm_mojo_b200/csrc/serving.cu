@@ -2,7 +2,6 @@
 // and eviction, and the rules on logits (include/llmq.h).
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
 #include <mutex>
 
 #include "context.cuh"
@@ -223,6 +222,16 @@ llmq_status llmq_paged_free(llmq_paged *p) {
   return LLMQ_OK;
 }
 
+llmq_status llmq_paged_shape(const llmq_paged *p, int *kind, int *n_layer, int *n_pages, int *page_size, int *n_kv_head,
+                             int *head_dim) {
+  if (!p) return LLMQ_ERR_INVALID;
+  int *out[6] = {kind, n_layer, n_pages, page_size, n_kv_head, head_dim};
+  const int val[6] = {p->v.kind, p->v.n_layer, p->v.n_pages, p->v.page_size, p->v.n_kv_head, p->v.head_dim};
+  for (int i = 0; i < 6; i++)
+    if (out[i]) *out[i] = val[i];
+  return LLMQ_OK;
+}
+
 llmq_status llmq_paged_buffers(const llmq_paged *p, void **k, void **v, float **ks, float **vs) {
   if (!p) return LLMQ_ERR_INVALID;
   if (k) *k = p->v.k;
@@ -254,15 +263,15 @@ llmq_status llmq_paged_store(llmq_ctx *ctx, llmq_paged *p, int layer, const floa
 
 llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, const float *q, long long q_stride,
                               float *out, long long out_stride, int n_seqs, int n_head, const int *table,
-                              long long table_stride, int table_cols, const int *lens, int max_len, float scale, const float *weights,
-                              float *weights_out, long long weights_stride) {
+                              long long table_stride, int table_cols, const int *lens, int max_len, float scale,
+                              const float *weights, float *weights_out, long long weights_stride) {
   llmq_status st = paged_check(ctx, p, layer, 1, table, table_stride, table_cols, n_seqs);
   if (st != LLMQ_OK) return st;
   if (!q || !out || !lens) return fail(ctx, LLMQ_ERR_INVALID, "null argument");
   if (n_head <= 0 || n_head % p->v.n_kv_head) return fail(ctx, LLMQ_ERR_INVALID, "n_head must be a multiple of n_kv_head");
   const long long C = (long long)n_head * p->v.head_dim;
   if (q_stride < 0 || (n_seqs > 1 && out_stride < C)) return fail(ctx, LLMQ_ERR_INVALID, "rows overlap");
-  if (max_len <= 0) return fail(ctx, LLMQ_ERR_INVALID, "bad max_len");
+  if (max_len <= 0 || max_len > 1 << 30) return fail(ctx, LLMQ_ERR_INVALID, "bad max_len");
   if (weights && !weights_out) return fail(ctx, LLMQ_ERR_INVALID, "weights without weights_out");
   if (weights_out && weights_stride < max_len) return fail(ctx, LLMQ_ERR_INVALID, "weights_stride below max_len");
   CK(cudaSetDevice(ctx->device));
@@ -290,22 +299,23 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   // 2 / 4 warps: 3072 units x <=256 positions 22 / 25 / 33, 1536 x <=256 21 /
   // 17 / 19, 576 x <=256 12 / 12 / 9)
   int warps = units >= ctx->num_sms * 16 && a.max_len <= 256 ? 1 : units >= ctx->num_sms * 8 ? 2 : 4;
-  if (getenv("WARPS")) warps = atoi(getenv("WARPS"));
   AttendKernel *k;
   if ((st = attend_kernel(ctx, a, warps, &k)) != LLMQ_OK) return st;
-  // Chunks: one wave of resident CTAs if every sequence were the longest,
-  // in whole blocks, at most kPmJoin of a unit
+  // Chunks, in whole blocks, two at least (1 x 200 positions: 4.8 us, 7.4 in
+  // single blocks, which have to be joined), at most kPmJoin of a unit: as
+  // many as the GPU holds CTAs at once for one sequence (131071 positions:
+  // 48 us, 53 with twice as many), twice that for several, of which only the
+  // longest fill their chunks (8 ragged sequences: 109 us, 150 with one wave)
   const long long wave = (long long)ctx->num_sms * k->per_sm[ctx->device % kMaxDevices];
-  const double waves = getenv("WAVES") ? atof(getenv("WAVES")) : n_seqs == 1 ? 1.0 : 2.0;
-  const long long fit = std::min((long long)kPmJoin, std::max(1LL, (long long)(waves * wave / units)));
-  const int minb = getenv("MINB") ? atoi(getenv("MINB")) : 2;
-  long long blocks = (a.max_len + k->block - 1) / k->block;
-  a.chunk = (int)std::max((long long)minb, (blocks + fit - 1) / fit) * k->block;
+  const long long fit = std::min((long long)kPmJoin, std::max(1LL, (n_seqs == 1 ? 1 : 2) * wave / units));
+  const long long blocks = (a.max_len + k->block - 1) / k->block;
+  a.chunk = (int)std::max(2LL, (blocks + fit - 1) / fit) * k->block;
   a.splits = (a.max_len + a.chunk - 1) / a.chunk;
   const unsigned g = grid1(units * a.splits);
   if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many sequences for one call");
   ServeWs *ws;
-  const size_t parts = a.splits > 1 ? (size_t)g * a.unit_heads * (D + 4) : 0, floats = parts + (weights_out ? rows * (a.score_stride + 2) + 4 : 0);
+  const size_t parts = a.splits > 1 ? (size_t)g * a.unit_heads * (D + 4) : 0;
+  const size_t floats = parts + (weights_out ? rows * (a.score_stride + 2) + 4 : 0);
   if ((st = serve_ws(ctx, floats * 4, a.splits > 1 ? (size_t)units * 4 : 0, &ws)) != LLMQ_OK) return st;
   a.part = (float *)ws->buf;
   a.tickets = (int *)ws->zeros;
@@ -332,7 +342,7 @@ llmq_status llmq_paged_evict(llmq_ctx *ctx, llmq_paged *p, int layer0, int n_lay
   if (st != LLMQ_OK) return st;
   if (!lens || !weights || !dst_table || !kept || !weights_out || !lens_out)
     return fail(ctx, LLMQ_ERR_INVALID, "null argument");
-  if (max_len <= 0 || budget <= 0 || sinks < 0 || recent < 0 || sinks > budget || recent > budget - sinks)
+  if (max_len <= 0 || max_len > 1 << 30 || budget <= 0 || sinks < 0 || recent < 0 || sinks > budget || recent > budget - sinks)
     return fail(ctx, LLMQ_ERR_INVALID, "sinks and recent must fit in a positive budget");
   if (weights_stride < max_len || weights_out_stride < budget || weights_out_stride > INT_MAX)
     return fail(ctx, LLMQ_ERR_INVALID, "bad weights stride");
@@ -373,16 +383,19 @@ llmq_status llmq_process_logits(llmq_ctx *ctx, const float *logits, long long lo
   a.ids = u.ids, a.n_ids = u.n_ids, a.n_prompt = u.n_prompt, a.ids_stride = u.ids_stride, a.max_ids = u.max_ids;
   a.bias_off = u.bias_offsets, a.bias_ids = u.bias_ids, a.bias_val = u.bias_values, a.n_bias = u.n_bias;
   a.mask = u.mask, a.mask_stride = u.mask_stride, a.argmax = argmax;
-  // tiles of 4096 logits, or smaller ones while the call has fewer CTAs than
-  // two per SM
-  int vpt = getenv("VPT") ? atoi(getenv("VPT")) : 16;
+  // Tiles of 4096 logits, or smaller ones while the call has fewer CTAs than
+  // two per SM (256 x 50257: 33 us with 4096, 39 with 2048, whose CTAs read
+  // the history twice as often)
+  int vpt = 16;
   constexpr int nth = 256;
   while (vpt > 4 && (long long)n * ((V + 3 + nth * vpt - 1) / (nth * vpt)) < 2 * ctx->num_sms) vpt /= 2;
   const int T = nth * vpt;
   a.tiles = (V + 3 + T - 1) / T;  // a row may start 3 logits past a 16-byte boundary
   const int keys = a.tiles * (nth / 32);
-  const int thr = getenv("THR") ? atoi(getenv("THR")) : 2;
-  const bool follow = argmax && (long long)n * a.tiles >= thr * ctx->num_sms;  // a second launch rather than tickets
+  // A second launch joins the argmax from two CTAs per SM on, where waiting
+  // for each CTA's stores before its ticket costs more (256 x 50257: 33 us
+  // against 38; 1 x 50257, with tickets, 5.0 us)
+  const bool follow = argmax && (long long)n * a.tiles >= 2 * ctx->num_sms;
   if (argmax) {
     ServeWs *ws;
     const llmq_status st = serve_ws(ctx, (size_t)n * keys * 8, follow ? 0 : (size_t)n * 4, &ws);

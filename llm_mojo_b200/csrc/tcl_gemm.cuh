@@ -316,8 +316,8 @@ struct TcArgsL {
   const int *xsl;     //   int8 rows: [sequences][16] lane sums of x
   WeightView w;
   const float *bias;  // int4 rows: [rows] or null
-  float *out;         // int4 rows: [sequences][rows]
-  float *part_val;    // int8 rows: [sequences][nparts] argmax candidates, 4 per row tile
+  float *out;         // [sequences][rows]; int8 rows: null for the argmax candidates alone
+  float *part_val;    // int8 rows without out: [sequences][nparts] argmax candidates, 4 per row tile
   int *part_idx;
   int *err;
   int B, OUT, K, nkb, nseg, epi, ntiles, nparts;
@@ -470,6 +470,10 @@ __device__ __forceinline__ void tcl_epilogue(const TcArgsL &p, TcSmemL<TT> &sm, 
         if (n < p.w.rows && m < p.B) {
           bv = sm.tree[2][c][tid] * sm.sx[cg * CW + c];
           bi = n;
+        }
+        if (p.out) {  // the logits themselves
+          if (bi == n) p.out[(size_t)m * p.OUT + n] = bv;
+          continue;
         }
         for (int o = 16; o > 0; o >>= 1) {
           const float ov = __shfl_xor_sync(0xffffffffu, bv, o);

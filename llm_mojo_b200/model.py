@@ -174,6 +174,25 @@ class Batch:
         check(lib().llmq_batch_generate_async(self.model.ctx.h, self.h, C.c_void_p(prompts_dev.data_ptr()), B, P,
                                               steps, C.c_void_p(ids_dev.data_ptr())), self.model.ctx.h)
 
+    def paged_step(self, cache, tokens, positions, slots, table, lens, max_len: int, logits, weights=None):
+        """One decode step of B sequences with a serving.PagedKVCache in place
+        of the batch's own caches: tokens, position embeddings, cache slots
+        and lengths (the new position among them) int32 CUDA tensors [B],
+        logits [B, V]; weights [n_layer, B, n_head, >= max_len] accumulate the
+        softmax weights in place. Enqueued on the context's stream, which the
+        tensors' work must be on too (Context.use_torch_stream)."""
+        B = tokens.shape[0]
+        for t in (tokens, positions, slots, lens, logits):
+            assert t.is_cuda and t.is_contiguous() and t.shape[0] == B
+        assert logits.shape[1] == self.model.V and table.shape[0] == B and table.stride(1) == 1
+        w, stride = None, 0
+        if weights is not None:
+            assert weights.is_contiguous() and weights.shape[1] == B and weights.shape[3] >= max_len
+            w, stride = weights.data_ptr(), weights.shape[3]
+        check(lib().llmq_batch_paged_step(self.model.ctx.h, self.h, cache.h, B, tokens.data_ptr(), positions.data_ptr(),
+                                          slots.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1],
+                                          lens.data_ptr(), max_len, w, stride, logits.data_ptr()), self.model.ctx.h)
+
     def free(self):
         if getattr(self, "h", None):
             lib().llmq_batch_free(self.h)

@@ -9,6 +9,7 @@ and is released with free(), as WeightMatrix values are.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -50,8 +51,22 @@ class Context:
 
     def use_torch_stream(self):
         """Issues the context's work on torch's current stream (the legacy
-        default stream, whose torch handle is 0, as cudaStreamLegacy)."""
+        default stream, whose torch handle is 0, as cudaStreamLegacy; the
+        decode steps that run as captured graphs need a stream that can be
+        captured, which that one cannot)."""
         self.set_stream(torch_stream(self.device) or CUDA_STREAM_LEGACY)
+
+    @contextlib.contextmanager
+    def torch_stream(self):
+        """use_torch_stream for a with block; the stream before it is back
+        afterwards, with the block's work done."""
+        before = self.stream
+        self.use_torch_stream()
+        try:
+            yield
+        finally:
+            self.sync()
+            self.set_stream(before)
 
     def on_torch_stream(self) -> bool:
         """Whether the context's work is ordered with torch's current stream

@@ -37,3 +37,32 @@ def test_rules_struct_matches_the_header():
         if decl:
             names += [x.strip(" *") for x in re.sub(r"^(const )?(float|int|long long|uint32_t) ", "", decl).split(",")]
     assert names == [f[0] for f in _Rules._fields_]
+
+
+def test_pack_mask():
+    import torch
+
+    from llm_mojo_b200.paged_generate import pack_mask
+
+    g = torch.Generator().manual_seed(1)
+    for V in (1, 31, 32, 33, 100):
+        ok = torch.rand(3, V, generator=g) < 0.5
+        ok[0, V - 1] = True
+        words = pack_mask(ok)
+        assert words.shape == (3, (V + 31) // 32) and words.dtype == torch.int32
+        for r in range(3):
+            assert [bool(int(words[r, t // 32]) >> (t % 32) & 1) for t in range(V)] == ok[r].tolist()
+
+
+def test_page_pool():
+    import pytest
+
+    from llm_mojo_b200.paged_generate import PagePool
+
+    p = PagePool(4)
+    a, b = p.take(3), p.take(1)
+    assert sorted(a + b) == [0, 1, 2, 3]
+    with pytest.raises(RuntimeError):
+        p.take(1)
+    p.give(a)
+    assert sorted(p.take(3)) == sorted(a)
