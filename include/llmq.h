@@ -341,6 +341,13 @@ llmq_status llmq_batch_generate_async(llmq_ctx *ctx, llmq_batch *b, const int *p
 typedef struct llmq_paged llmq_paged;
 llmq_status llmq_paged_create(llmq_ctx *ctx, int kind, int n_layer, int n_pages, int page_size, int n_kv_head,
                               int head_dim, llmq_paged **out);
+/* The same over device buffers of the caller's (16-byte aligned, with the
+ * sizes above; ks_dev and vs_dev for int8 only), which it keeps until after
+ * llmq_paged_free and need not clear: a process whose allocator owns the
+ * memory hands out pools without cudaMalloc's wait. */
+llmq_status llmq_paged_create_in(llmq_ctx *ctx, int kind, int n_layer, int n_pages, int page_size, int n_kv_head,
+                                 int head_dim, void *k_dev, void *v_dev, float *ks_dev, float *vs_dev,
+                                 llmq_paged **out);
 llmq_status llmq_paged_free(llmq_paged *p);
 /* The cache's kind and sizes. Any pointer may be NULL. */
 llmq_status llmq_paged_shape(const llmq_paged *p, int *kind, int *n_layer, int *n_pages, int *page_size, int *n_kv_head,

@@ -82,6 +82,7 @@ SIGNATURES = {
     "llmq_model_profile": (I, [P, P, I]),
     "llmq_model_profile_read": (I, [P, P, P, I, I]),
     "llmq_paged_create": (I, [P, I, I, I, I, I, I, PP]),
+    "llmq_paged_create_in": (I, [P, I, I, I, I, I, I, P, P, P, P, PP]),
     "llmq_paged_free": (I, [P]),
     "llmq_paged_shape": (I, [P, P, P, P, P, P, P]),
     "llmq_paged_buffers": (I, [P, PP, PP, PP, PP]),

@@ -13,7 +13,8 @@
 using namespace llmq;
 
 struct llmq_paged {
-  llmq_ctx *ctx;
+  int device = 0;
+  bool owned = false;  // whether the buffers are the handle's
   PagedView v{};
 };
 
@@ -57,7 +58,7 @@ int elem_bytes(int kind) { return kind == LLMQ_KV_F32 ? 4 : kind == LLMQ_KV_BF16
 llmq_status paged_check(llmq_ctx *ctx, const llmq_paged *p, int layer0, int n_layers, const int *table,
                         long long table_stride, int table_cols, int n_seqs) {
   if (!ctx || !p || !table) return fail(ctx, LLMQ_ERR_INVALID, "null argument");
-  if (p->ctx->device != ctx->device) return fail(ctx, LLMQ_ERR_INVALID, "the cache is on another device");
+  if (p->device != ctx->device) return fail(ctx, LLMQ_ERR_INVALID, "the cache is on another device");
   if (layer0 < 0 || n_layers <= 0 || layer0 > p->v.n_layer - n_layers) return fail(ctx, LLMQ_ERR_INVALID, "bad layer");
   if (n_seqs <= 0 || table_cols <= 0 || table_stride < 0) return fail(ctx, LLMQ_ERR_INVALID, "bad page table shape");
   return LLMQ_OK;
@@ -171,53 +172,80 @@ cudaError_t launch_move(const EvictArgs &a, int tiles, unsigned grid, cudaStream
 // Blocks of a one-dimensional grid, or 0 when there would be too many.
 unsigned grid1(long long n) { return n > 0 && n <= INT_MAX ? (unsigned)n : 0u; }
 
-}  // namespace
-
-extern "C" {
-
-llmq_status llmq_paged_create(llmq_ctx *ctx, int kind, int n_layer, int n_pages, int page_size, int n_kv_head,
-                              int head_dim, llmq_paged **out) {
-  if (!ctx || !out) return fail(ctx, LLMQ_ERR_INVALID, "null argument");
-  *out = nullptr;
+llmq_status paged_shape_check(llmq_ctx *ctx, int kind, int n_layer, int n_pages, int page_size, int n_kv_head,
+                              int head_dim) {
   if (kind != LLMQ_KV_QUANT8 && kind != LLMQ_KV_F32 && kind != LLMQ_KV_BF16)
     return fail(ctx, LLMQ_ERR_UNSUPPORTED, "a paged cache holds int8, float32 or bfloat16");
   if (n_layer <= 0 || n_pages <= 0 || page_size <= 0 || n_kv_head <= 0 || head_dim <= 0 || head_dim % 32 ||
       head_dim > 128)
     return fail(ctx, LLMQ_ERR_INVALID, "bad paged cache shape (head_dim: 32, 64, 96 or 128)");
-  CK(cudaSetDevice(ctx->device));
-  const double rows_d = (double)n_layer * n_pages * n_kv_head * page_size;
-  if (rows_d * head_dim * 4 > 4e12) return fail(ctx, LLMQ_ERR_NOMEM, "paged cache larger than any device");
-  if ((double)n_pages * n_kv_head * page_size > INT_MAX)
-    return fail(ctx, LLMQ_ERR_INVALID, "more than 2^31 - 1 rows in a layer");
-  const size_t rows = (size_t)n_layer * n_pages * n_kv_head * page_size;
-  const size_t bytes = rows * head_dim * elem_bytes(kind);
+  const double rows = (double)n_pages * n_kv_head * page_size;
+  if (rows * n_layer * head_dim * 4 > 4e12) return fail(ctx, LLMQ_ERR_NOMEM, "paged cache larger than any device");
+  if (rows > INT_MAX) return fail(ctx, LLMQ_ERR_INVALID, "more than 2^31 - 1 rows in a layer");
+  return LLMQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+llmq_status llmq_paged_create_in(llmq_ctx *ctx, int kind, int n_layer, int n_pages, int page_size, int n_kv_head,
+                                 int head_dim, void *k, void *v, float *ks, float *vs, llmq_paged **out) {
+  if (!ctx || !out) return fail(ctx, LLMQ_ERR_INVALID, "null argument");
+  *out = nullptr;
+  const llmq_status st = paged_shape_check(ctx, kind, n_layer, n_pages, page_size, n_kv_head, head_dim);
+  if (st != LLMQ_OK) return st;
+  const bool scaled = kind == LLMQ_KV_QUANT8;
+  if (!k || !v || (scaled && (!ks || !vs))) return fail(ctx, LLMQ_ERR_INVALID, "null buffer");
+  if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)ks | (uintptr_t)vs) % 16)
+    return fail(ctx, LLMQ_ERR_INVALID, "buffers must be 16-byte aligned");
   llmq_paged *p = new llmq_paged();
-  p->ctx = ctx;
-  p->v = PagedView{nullptr, nullptr, nullptr, nullptr, kind, n_layer, n_pages, page_size, n_kv_head, head_dim};
-  cudaError_t e = cudaMalloc(&p->v.k, bytes);
-  if (e == cudaSuccess) e = cudaMalloc(&p->v.v, bytes);
-  if (e == cudaSuccess && kind == LLMQ_KV_QUANT8) e = cudaMalloc(&p->v.ks, rows * 4);
-  if (e == cudaSuccess && kind == LLMQ_KV_QUANT8) e = cudaMalloc(&p->v.vs, rows * 4);
-  if (e == cudaSuccess) e = cudaMemsetAsync(p->v.k, 0, bytes, ctx->stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(p->v.v, 0, bytes, ctx->stream);
-  if (e == cudaSuccess && kind == LLMQ_KV_QUANT8) e = cudaMemsetAsync(p->v.ks, 0, rows * 4, ctx->stream);
-  if (e == cudaSuccess && kind == LLMQ_KV_QUANT8) e = cudaMemsetAsync(p->v.vs, 0, rows * 4, ctx->stream);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
-  if (e != cudaSuccess) {
-    llmq_paged_free(p);
-    cudaGetLastError();
-    return fail(ctx, e == cudaErrorMemoryAllocation ? LLMQ_ERR_NOMEM : LLMQ_ERR_CUDA,
-                std::string("paged cache: ") + cudaGetErrorString(e));
-  }
+  p->device = ctx->device;
+  p->v = PagedView{k, v, scaled ? ks : nullptr, scaled ? vs : nullptr, kind, n_layer, n_pages, page_size, n_kv_head, head_dim};
   *out = p;
+  return LLMQ_OK;
+}
+
+llmq_status llmq_paged_create(llmq_ctx *ctx, int kind, int n_layer, int n_pages, int page_size, int n_kv_head,
+                              int head_dim, llmq_paged **out) {
+  if (!ctx || !out) return fail(ctx, LLMQ_ERR_INVALID, "null argument");
+  *out = nullptr;
+  llmq_status st = paged_shape_check(ctx, kind, n_layer, n_pages, page_size, n_kv_head, head_dim);
+  if (st != LLMQ_OK) return st;
+  CK(cudaSetDevice(ctx->device));
+  const size_t rows = (size_t)n_layer * n_pages * n_kv_head * page_size;
+  const size_t bytes[4] = {rows * head_dim * elem_bytes(kind), rows * head_dim * elem_bytes(kind), rows * 4, rows * 4};
+  void *buf[4] = {};
+  cudaError_t e = cudaSuccess;
+  for (int i = 0; i < (kind == LLMQ_KV_QUANT8 ? 4 : 2) && e == cudaSuccess; i++) {
+    e = cudaMalloc(&buf[i], bytes[i]);
+    if (e == cudaSuccess) e = cudaMemsetAsync(buf[i], 0, bytes[i], ctx->stream);
+  }
+  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+  if (e == cudaSuccess) {
+    st = llmq_paged_create_in(ctx, kind, n_layer, n_pages, page_size, n_kv_head, head_dim, buf[0], buf[1],
+                              (float *)buf[2], (float *)buf[3], out);
+  } else {
+    cudaGetLastError();
+    st = fail(ctx, e == cudaErrorMemoryAllocation ? LLMQ_ERR_NOMEM : LLMQ_ERR_CUDA,
+              std::string("paged cache: ") + cudaGetErrorString(e));
+  }
+  if (st != LLMQ_OK) {
+    for (void *q : buf)
+      if (q) cudaFree(q);
+    return st;
+  }
+  (*out)->owned = true;
   return LLMQ_OK;
 }
 
 llmq_status llmq_paged_free(llmq_paged *p) {
   if (!p) return LLMQ_ERR_INVALID;
-  cudaSetDevice(p->ctx->device);
-  for (void *q : {p->v.k, p->v.v, (void *)p->v.ks, (void *)p->v.vs})
-    if (q) cudaFree(q);
+  if (p->owned) {
+    cudaSetDevice(p->device);
+    for (void *q : {p->v.k, p->v.v, (void *)p->v.ks, (void *)p->v.vs})
+      if (q) cudaFree(q);
+  }
   delete p;
   return LLMQ_OK;
 }

@@ -24,15 +24,6 @@ F32, I32 = torch.float32, torch.int32
 KINDS = {"int8": KV_QUANT8, "bf16": KV_BF16, "f32": KV_F32}
 
 
-class _Array:
-    """A device buffer of the library as torch.as_tensor takes it; holds its
-    owner, so that views outlive no storage."""
-
-    def __init__(self, owner, ptr: int, shape, typestr: str):
-        self.owner = owner
-        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (ptr, False), "version": 3}
-
-
 def _check(ctx: Context, name: str, t, dtype, ndim: int, inner: int = 1):
     """t as the call takes it: on the context's device, `dtype`, `ndim`
     dimensions of which the last `inner` are contiguous. Returns its address."""
@@ -72,8 +63,9 @@ def _call(ctx: Context, fn, *args):
 class PagedKVCache:
     """The pages of one cache, for all its sequences: kind 'int8' (codes with
     a float32 scale per position and head, QuantKV[8]'s rule), 'bf16' or
-    'f32'. k and v are torch views of the pool, [n_layer, n_pages, n_kv_head,
-    page_size, head_dim]; ks and vs of its scales (None without).
+    'f32'. k and v are the pool, [n_layer, n_pages, n_kv_head, page_size,
+    head_dim]; ks and vs its scales (None without): tensors of torch's
+    allocator, not cleared.
 
     A page table (int32 [n_seqs, n]) gives the page of each run of page_size
     positions; an entry outside the pool (-1) is no page."""
@@ -85,25 +77,25 @@ class PagedKVCache:
         self.ctx, self.kind = ctx, kind
         self.n_layer, self.n_pages, self.page_size = n_layer, n_pages, page_size
         self.n_kv_head, self.head_dim, self.scale = n_kv_head, head_dim, 1.0 / max(head_dim, 1) ** 0.5
-        h = C.c_void_p()
-        check(lib().llmq_paged_create(ctx.h, KINDS[kind], n_layer, n_pages, page_size, n_kv_head, head_dim,
-                                      C.byref(h)), ctx.h)
-        self._storage = _Storage(ctx, h)
-        self.h = h
-        ptr = [C.c_void_p() for _ in range(4)]
-        check(lib().llmq_paged_buffers(h, *[C.byref(p) for p in ptr]))
+        if min(n_layer, n_pages, page_size, n_kv_head, head_dim) <= 0 or head_dim > 128 or (
+                n_layer * n_pages * n_kv_head * page_size * head_dim > 1 << 39):
+            # no such buffers: the library says why
+            check(lib().llmq_paged_create(ctx.h, KINDS[kind], n_layer, n_pages, page_size, n_kv_head, head_dim,
+                                          C.byref(C.c_void_p())), ctx.h)
         shape = (n_layer, n_pages, n_kv_head, page_size, head_dim)
-        typestr = {"int8": "|i1", "bf16": "<i2", "f32": "<f4"}[kind]
-
-        def view(p, shape, typestr):
-            return torch.as_tensor(_Array(self._storage, p.value, shape, typestr), device=f"cuda:{ctx.device}")
-
-        self.k, self.v = view(ptr[0], shape, typestr), view(ptr[1], shape, typestr)
-        if kind == "bf16":
-            self.k, self.v = self.k.view(torch.bfloat16), self.v.view(torch.bfloat16)
+        at = dict(device=f"cuda:{ctx.device}")
+        dtype = {"int8": torch.int8, "bf16": torch.bfloat16, "f32": F32}[kind]
+        self.k, self.v = torch.empty(shape, dtype=dtype, **at), torch.empty(shape, dtype=dtype, **at)
         self.ks = self.vs = None
         if kind == "int8":
-            self.ks, self.vs = view(ptr[2], shape[:-1], "<f4"), view(ptr[3], shape[:-1], "<f4")
+            self.ks, self.vs = torch.empty(shape[:-1], dtype=F32, **at), torch.empty(shape[:-1], dtype=F32, **at)
+        # the buffers again: k and the others are the caller's to keep or drop
+        self._buffers = [t for t in (self.k, self.v, self.ks, self.vs) if t is not None]
+        ptr = [t.data_ptr() if t is not None else None for t in (self.k, self.v, self.ks, self.vs)]
+        h = C.c_void_p()
+        check(lib().llmq_paged_create_in(ctx.h, KINDS[kind], n_layer, n_pages, page_size, n_kv_head, head_dim, *ptr,
+                                         C.byref(h)), ctx.h)
+        self.h = h
 
     def store(self, layer: int, k, v, pos, table, seq=None):
         """Stores rows k, v [n, n_kv_head, head_dim] (any row stride: the
@@ -197,22 +189,15 @@ class PagedKVCache:
         return kept, wout, lens_out
 
     def free(self):
-        """Releases the pool; its views must not be used any more."""
-        self.k = self.v = self.ks = self.vs = None
-        self._storage.free()
-        self.h = None
-
-
-class _Storage:
-    """Owns a llmq_paged handle."""
-
-    def __init__(self, ctx: Context, h):
-        self.ctx, self.h = ctx, h
-
-    def free(self):
-        if self.h:
+        """Gives the buffers back to torch once the context's stream is done
+        with them."""
+        if getattr(self, "h", None):
+            if self.ctx.h:
+                self.ctx.sync()
             lib().llmq_paged_free(self.h)
             self.h = None
+        self.k = self.v = self.ks = self.vs = None
+        self._buffers = []
 
     def __del__(self):
         try:

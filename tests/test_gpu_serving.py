@@ -741,3 +741,39 @@ def test_views_keep_the_pool(torch, ctx):
 
     gc.collect()
     assert torch.equal(k, want)
+
+
+@pytest.mark.parametrize("kind", PAGED)
+def test_c_owned_pool(torch, ctx, kind):
+    """llmq_paged_create's own buffers start as zeros and hold what is
+    stored; borrowed ones must be there and aligned."""
+    import ctypes as C
+
+    from llm_mojo_b200 import _lib
+    from llm_mojo_b200.serving import KINDS
+
+    L = _lib.lib()
+    h = C.c_void_p()
+    assert L.llmq_paged_create(ctx.h, KINDS[kind], 2, 3, 4, 2, 32, C.byref(h)) == _lib.OK
+    size = [C.c_int() for _ in range(6)]
+    assert L.llmq_paged_shape(h, *[C.byref(s) for s in size]) == _lib.OK
+    assert [s.value for s in size] == [KINDS[kind], 2, 3, 4, 2, 32]
+    table = torch.tensor([[1, 2]], dtype=torch.int32, device="cuda")
+    q = torch.ones(1, 2, 32, device="cuda")
+    out = torch.full((1, 2, 32), 9.0, device="cuda")
+    lens = torch.tensor([8], dtype=torch.int32, device="cuda")
+    args = (q.data_ptr(), 64, out.data_ptr(), 64, 1, 2, table.data_ptr(), 2, 2, lens.data_ptr(), 8, 1.0, None, None, 0)
+    assert L.llmq_paged_attend(ctx.h, h, 1, *args) == _lib.OK
+    assert torch.count_nonzero(out) == 0
+    x = torch.full((8, 2, 32), 2.0, device="cuda")
+    pos, seq = torch.arange(8, dtype=torch.int32, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+    assert L.llmq_paged_store(ctx.h, h, 1, x.data_ptr(), 64, x.data_ptr(), 64, seq.data_ptr(), pos.data_ptr(), 8,
+                              table.data_ptr(), 2, 2, 1) == _lib.OK
+    assert L.llmq_paged_attend(ctx.h, h, 1, *args) == _lib.OK
+    torch.cuda.synchronize()
+    assert float((out - 2.0).abs().max()) < 2.0 ** -20
+    assert L.llmq_paged_free(h) == _lib.OK
+    b = torch.zeros(4096, device="cuda")
+    for ptr in ((None, b.data_ptr()), (b.data_ptr(), b.data_ptr() + 4)):
+        assert L.llmq_paged_create_in(ctx.h, KINDS[kind], 1, 1, 4, 1, 32, *ptr, b.data_ptr(), b.data_ptr(),
+                                      C.byref(h)) == _lib.ERR_INVALID and not h
