@@ -33,12 +33,10 @@ __device__ __forceinline__ int evict_len(const EvictArgs &a, int b) {
 // An unsigned key in the order of the floats; NaN is below every number and
 // -0 equals 0.
 __device__ __forceinline__ unsigned evict_key(float x) {
-  if (x != x) return 0u;
-  const unsigned u = __float_as_uint(x + 0.0f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  const int u = __float_as_int(x + 0.0f);
+  const unsigned k = (unsigned)u ^ ((unsigned)(u >> 31) | 0x80000000u);
+  return x != x ? 0u : k;
 }
-
-constexpr int kEvThreads = 1024;
 
 // A thread's four weights from position j on, j a multiple of 4 (positions
 // past the row's end: unspecified).
@@ -52,16 +50,24 @@ __device__ __forceinline__ float4 evict_load(const float *w, int j, int len) {
 // One CTA per row. The need-th largest key of the positions between the
 // sinks and the recent ones by radix select: digits of 11, 11 and 10 bits
 // from the top, each a histogram of the keys that agree with the digits
-// found so far, in shared memory (integer atomics: exact). Then the kept
-// positions in order: one prefix sum of (above the threshold or always kept,
-// equal to it) per 4096 positions, of the equal ones the first `ties`. The
-// row is read four times, but for the first time from L2.
-// grid (n_layers * n_seqs * n_kv_head), 1024 threads.
-template <bool VEC>
-__global__ void __launch_bounds__(kEvThreads) evict_select_kernel(EvictArgs a) {
-  __shared__ int hist[2048];
-  __shared__ int wsum[32];
-  __shared__ int s_bin, s_need;
+// found so far, in shared memory (integer atomics: exact). The second pass
+// also lists the keys that agree, a few percent of a spread row, so that the
+// third reads the list where it fits. Then the kept positions in order: one
+// prefix sum of (above the threshold or always kept, equal to it) per 4 NTH
+// positions, of the equal ones the first `ties`. The row is read three or
+// four times, but for the first time from L2; instructions bound it, and, in
+// short rows, barriers: NTH 256 up to 2048 positions (144 rows of 1024: 6
+// us, 10 with 1024 threads), 1024 beyond.
+// grid (n_layers * n_seqs * n_kv_head), NTH threads.
+constexpr int kEvList = 4096;
+
+template <bool VEC, int NTH>
+__global__ void __launch_bounds__(NTH) evict_select_kernel(EvictArgs a) {
+  constexpr int kBins = 2048, kPer = kBins / NTH, kW = NTH / 32;
+  __shared__ int hist[kBins];
+  __shared__ unsigned list[kEvList];
+  __shared__ int wsum[kW];
+  __shared__ int s_bin, s_need, s_listed;
   const int row = blockIdx.x, b = row / a.c.n_kv_head % a.src.n_seqs, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int len = evict_len(a, b), n = min(len, a.budget);
@@ -69,72 +75,93 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(EvictArgs a) {
   float *wout = a.wout + row * a.wout_stride;
   int *kept = a.kept + (size_t)row * a.budget;
   if (row < a.src.n_seqs * a.c.n_kv_head && row % a.c.n_kv_head == 0 && tid == 0) a.lens_out[b] = n;
-  for (long long j = n + tid; j < a.wout_stride; j += kEvThreads) wout[j] = 0.0f;
-  for (int j = n + tid; j < a.budget; j += kEvThreads) kept[j] = -1;
+  for (long long j = n + tid; j < a.wout_stride; j += NTH) wout[j] = 0.0f;
+  for (int j = n + tid; j < a.budget; j += NTH) kept[j] = -1;
   if (len <= a.budget) {
-    for (int j = tid; j < len; j += kEvThreads) {
+    for (int j = tid; j < len; j += NTH) {
       kept[j] = j;
       wout[j] = w[j];
     }
     return;
   }
+  // the sum of v over the threads up to and with this one; all: over all of them
+  auto scan = [&](int v, int &all) {
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += t;
+    }
+    if (lane == 31) wsum[wid] = v;
+    __syncthreads();
+    int t = lane < kW ? wsum[lane] : 0;
+    for (int o = 1; o < kW; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) t += u;
+    }
+    all = __shfl_sync(0xffffffffu, t, kW - 1);
+    const int before = __shfl_sync(0xffffffffu, t, max(wid - 1, 0));
+    return v + (wid ? before : 0);
+  };
   const int lo = a.sinks, hi = len - a.recent;
   int need = a.budget - a.sinks - a.recent;
   unsigned thr = 0;  // the digits found, from the top
   if (need > 0) {
 #pragma unroll 1
     for (int pass = 0; pass < 3; pass++) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const unsigned mask = pass == 2 ? 1023u : 2047u;
       const unsigned known = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-      for (int i = tid; i < 2048; i += kEvThreads) hist[i] = 0;
+      for (int i = tid; i < kBins; i += NTH) hist[i] = 0;
+      if (tid == 0 && pass < 2) s_listed = 0;
       __syncthreads();
-#pragma unroll 4
-      for (int j = tid * 4; j < hi; j += kEvThreads * 4) {
-        const float4 x = evict_load<VEC>(w, j, hi);
-        const float y[4] = {x.x, x.y, x.z, x.w};
+      auto count = [&](unsigned key) {
+        if ((key ^ thr) & known) return;
+        atomicAdd(&hist[key >> shift & mask], 1);
+        if (pass == 1) {
+          const int at = atomicAdd(&s_listed, 1);
+          if (at < kEvList) list[at] = key;
+        }
+      };
+      if (pass == 2 && s_listed <= kEvList) {
+        for (int i = tid; i < s_listed; i += NTH) count(list[i]);
+      } else {
+#pragma unroll 2
+        for (int j = tid * 4; j < hi; j += NTH * 4) {
+          const float4 x = evict_load<VEC>(w, j, hi);
+          const unsigned key[4] = {evict_key(x.x), evict_key(x.y), evict_key(x.z), evict_key(x.w)};
+          if (j >= lo && j + 3 < hi) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const unsigned key = evict_key(y[i]);
-          if (j + i >= lo && j + i < hi && ((key ^ thr) & known) == 0) atomicAdd(&hist[key >> shift & (bins - 1)], 1);
+            for (int i = 0; i < 4; i++) count(key[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if (j + i >= lo && j + i < hi) count(key[i]);
+          }
         }
       }
       __syncthreads();
-      // the bin of the need-th largest: bins from the top, two a thread
-      const int b1 = 2047 - 2 * tid, h1 = hist[b1], h0 = hist[b1 - 1];
-      int s = h1 + h0;
-      for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += t;
-      }
-      if (lane == 31) wsum[wid] = s;
-      __syncthreads();
-      if (wid == 0) {
-        int t = wsum[lane];
-        for (int o = 1; o < 32; o <<= 1) {
-          const int u = __shfl_up_sync(0xffffffffu, t, o);
-          if (lane >= o) t += u;
-        }
-        wsum[lane] = t;
-      }
-      __syncthreads();
-      s += wid ? wsum[wid - 1] : 0;  // keys in this thread's bins and above
-      const int above = s - h1 - h0;
-      if (above < need && need <= s) {
-        const bool first = need <= above + h1;
-        s_bin = first ? b1 : b1 - 1;
-        s_need = need - above - (first ? 0 : h1);
+      // the bin of the need-th largest: bins from the top, kPer a thread
+      const int top = kBins - 1 - kPer * tid;
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; i++) mine += hist[top - i];
+      int all;
+      const int upto = scan(mine, all), above = upto - mine;
+      if (above < need && need <= upto) {
+        int s = above, i = 0;
+        while (s + hist[top - i] < need) s += hist[top - i++];
+        s_bin = top - i;
+        s_need = need - s;
       }
       __syncthreads();
       thr |= (unsigned)s_bin << shift;
       need = s_need;
-      __syncthreads();
     }
   } else {
     thr = 0xffffffffu;  // no key reaches it (NaN of any kind maps to 0)
   }
   // need is now how many of the keys equal to thr stay
   int base = 0, tbase = 0;
-  for (int j0 = 0; j0 < len; j0 += kEvThreads * 4) {
+  for (int j0 = 0; j0 < len; j0 += NTH * 4) {
     const int j = j0 + tid * 4;
     const float4 x = evict_load<VEC>(w, j, len);
     const float y[4] = {x.x, x.y, x.z, x.w};
@@ -146,21 +173,10 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(EvictArgs a) {
       flag[i] = j + i >= len ? 0 : (!mid || key > thr) ? 1 : key == thr ? 0x10000 : 0;
       mine += flag[i];
     }
-    int s = mine;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += t;
-    }
-    if (lane == 31) wsum[wid] = s;
     __syncthreads();
-    int t = wsum[lane];
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, t, o);
-      if (lane >= o) t += u;
-    }
-    const int all = __shfl_sync(0xffffffffu, t, 31), before = wid ? __shfl_sync(0xffffffffu, t, max(wid - 1, 0)) : 0;
-    s += before - mine;
-    int sure = base + (s & 0xffff), ties = tbase + (s >> 16);
+    int all;
+    const int before = scan(mine, all) - mine;
+    int sure = base + (before & 0xffff), ties = tbase + (before >> 16);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       if (flag[i] == 1 || (flag[i] && ties < need)) {
@@ -173,7 +189,6 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(EvictArgs a) {
     }
     base += all & 0xffff;
     tbase += all >> 16;
-    __syncthreads();
   }
 }
 

@@ -71,61 +71,65 @@ __device__ __forceinline__ void pack_store(typename E::T *dst, const float4 &x, 
   }
 }
 
-// A group of LG lanes (D / 4, and 8 of 32 idle at D = 96) has a head's key
-// or value, four elements a lane, kStoreItems of them in flight: memory is
-// all that this kernel does. int8: s = max|x| / 127 (1 when 0), codes round(x
-// * (1 / s)), half away from zero, as QuantKV.quantize (kvcache.mojo:319-331).
-// VEC: 16-byte loads (aligned rows). grid of 256 threads over the items, (row,
-// kv head, key or value) in that order.
-constexpr int kStoreItems = 4;
+// A warp has one row and up to kStoreHeads heads per group of LG lanes (D / 4,
+// and 8 of 32 idle at D = 96), key and value, four elements a lane: the row's
+// page is looked up once, and 2 kStoreHeads loads are in flight a lane.
+// int8: s = max|x| / 127 (1 when 0), codes round(x * (1 / s)), half away from
+// zero, as QuantKV.quantize (kvcache.mojo:319-331). VEC: 16-byte loads
+// (aligned rows). Memory bounds it: 16387 rows of 8 x 128 to bfloat16 take 35
+// us at 5.8 TB/s (with the lookup in every head's lanes, 41). grid of 256
+// threads over (row, block of heads).
+constexpr int kStoreHeads = 4;
 
 template <typename E, int D, bool VEC>
 __global__ void __launch_bounds__(256) paged_store_kernel(StoreArgs a) {
-  constexpr int LG = D == 96 ? 32 : D / 4, kPer = 256 / LG;
+  constexpr int LG = D == 96 ? 32 : D / 4, kG = 32 / LG, kH = kG * kStoreHeads;  // kH: heads of a warp
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x % LG, nh = a.c.n_kv_head;
-  const long long i0 = ((long long)blockIdx.x * kPer + threadIdx.x / LG) * kStoreItems;
-  const long long items = (long long)a.n_rows * nh * 2;
-  float4 x[kStoreItems];
-  long long row[kStoreItems];
+  const int lane = threadIdx.x % LG, grp = threadIdx.x % 32 / LG, nh = a.c.n_kv_head, blocks = (nh + kH - 1) / kH;
+  const unsigned w = blockIdx.x * 8 + threadIdx.x / 32, r = w / (unsigned)blocks;
+  if (r >= (unsigned)a.n_rows) return;
+  const int h0 = (int)(w - r * blocks) * kH + grp;
+  const bool on = lane * 4 < D;
+  const float *src[2] = {a.k + r * a.k_stride + h0 * D + lane * 4, a.v + r * a.v_stride + h0 * D + lane * 4};
+  float4 x[kStoreHeads][2];
 #pragma unroll
-  for (int j = 0; j < kStoreItems; j++) {
-    const long long i = i0 + j;
-    row[j] = -1;
-    x[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (i >= items) continue;
-    const int which = i & 1;
-    const unsigned q = (unsigned)(i >> 1), r = q / (unsigned)nh, h = q - r * nh;
-    const float *src = (which ? a.v + r * a.v_stride : a.k + r * a.k_stride) + h * D + lane * 4;
-    if (lane * 4 < D) {
+  for (int j = 0; j < kStoreHeads; j++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      x[j][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (!on || h0 + j * kG >= nh) continue;
+      const float *p = src[i] + j * kG * D;
       if constexpr (VEC)
-        x[j] = __ldcs((const float4 *)src);
+        x[j][i] = __ldcs((const float4 *)p);
       else
-        x[j] = make_float4(src[0], src[1], src[2], src[3]);
+        x[j][i] = make_float4(p[0], p[1], p[2], p[3]);
     }
-    const int pos = a.pos[r], sq = a.seq ? a.seq[r] : (int)r;
-    if (pos < 0 || sq < 0 || sq >= a.t.n_seqs) continue;
-    const int pi = pos / a.c.page_size;
-    if (pi >= a.t.cols) continue;
-    const int page = a.t.page(sq, pi);
-    if (page < 0 || page >= a.c.n_pages) continue;
-    row[j] = (long long)a.c.row(a.layer, page, h, pos - pi * a.c.page_size);
-  }
+  const int pos = a.pos[r], sq = a.seq ? a.seq[r] : (int)r;
+  if (pos < 0 || sq < 0 || sq >= a.t.n_seqs) return;
+  const int pi = pos / a.c.page_size;
+  if (pi >= a.t.cols) return;
+  const int page = a.t.page(sq, pi);
+  if (page < 0 || page >= a.c.n_pages) return;
+  const size_t row0 = a.c.row(a.layer, page, h0, pos - pi * a.c.page_size);
 #pragma unroll
-  for (int j = 0; j < kStoreItems; j++) {
-    const int which = j & 1;
-    float inv = 0.0f;
-    if constexpr (E::kScaled) {
-      float m = fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w)));
+  for (int j = 0; j < kStoreHeads; j++) {
+    const size_t row = row0 + (size_t)(j * kG) * a.c.page_size;
 #pragma unroll
-      for (int o = LG / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      float s = m / 127.0f;
-      if (s == 0.0f) s = 1.0f;
-      inv = 1.0f / s;
-      if (lane == 0 && row[j] >= 0) (which ? a.c.vs : a.c.ks)[row[j]] = s;
+    for (int i = 0; i < 2; i++) {
+      float inv = 0.0f, s = 1.0f;
+      if constexpr (E::kScaled) {
+        const float4 &y = x[j][i];
+        float m = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
+#pragma unroll
+        for (int o = LG / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        s = m / 127.0f;
+        if (s == 0.0f) s = 1.0f;
+        inv = 1.0f / s;
+      }
+      if (h0 + j * kG >= nh) continue;
+      if (E::kScaled && lane == 0) (i ? a.c.vs : a.c.ks)[row] = s;
+      if (on) pack_store<E>((typename E::T *)(i ? a.c.v : a.c.k) + row * D + lane * 4, x[j][i], inv);
     }
-    if (row[j] >= 0 && lane * 4 < D)
-      pack_store<E>((typename E::T *)(which ? a.c.v : a.c.k) + row[j] * D + lane * 4, x[j], inv);
   }
 }
 

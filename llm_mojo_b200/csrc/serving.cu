@@ -280,9 +280,9 @@ llmq_status llmq_paged_store(llmq_ctx *ctx, llmq_paged *p, int layer, const floa
   CK(cudaSetDevice(ctx->device));
   const StoreArgs a{p->v, PageTable{table, table_stride, table_cols, n_seqs}, layer, n_rows, k, v, k_stride, v_stride,
                     seq, pos};
-  const int per = kStoreItems * (p->v.head_dim == 96 ? 8 : 1024 / p->v.head_dim);  // items of a CTA
-  const long long items = (long long)n_rows * p->v.n_kv_head * 2;
-  const unsigned g = items <= 2LL * INT_MAX ? grid1((items + per - 1) / per) : 0;
+  const int per = kStoreHeads * (p->v.head_dim == 96 ? 1 : 128 / p->v.head_dim);  // heads of a warp
+  const long long warps = (long long)n_rows * ((p->v.n_kv_head + per - 1) / per);
+  const unsigned g = warps <= INT_MAX ? grid1((warps + 7) / 8) : 0;
   if (!g) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
   const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && (n_rows == 1 || (k_stride % 4 == 0 && v_stride % 4 == 0));
   CK(launch_store(a, vec, g, ctx->stream));
@@ -385,7 +385,11 @@ llmq_status llmq_paged_evict(llmq_ctx *ctx, llmq_paged *p, int layer0, int n_lay
   const unsigned g = grid1(rows), gm = g ? grid1(rows * tiles) : 0;
   if (!g || !gm) return fail(ctx, LLMQ_ERR_INVALID, "too many rows for one call");
   const bool vec = (uintptr_t)weights % 16 == 0 && weights_stride % 4 == 0;
-  CK(launch_after(vec ? evict_select_kernel<true> : evict_select_kernel<false>, dim3(g), kEvThreads, ctx->stream, 0, a));
+  if (max_len <= 2048)
+    CK(launch_after(vec ? evict_select_kernel<true, 256> : evict_select_kernel<false, 256>, dim3(g), 256, ctx->stream, 0, a));
+  else
+    CK(launch_after(vec ? evict_select_kernel<true, 1024> : evict_select_kernel<false, 1024>, dim3(g), 1024, ctx->stream, 0,
+                    a));
   CK(launch_move(a, tiles, gm, ctx->stream));
   return LLMQ_OK;
 }
