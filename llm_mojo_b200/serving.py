@@ -17,7 +17,7 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import KV_BF16, KV_F32, KV_QUANT8, OK, check, lib
-from .tensor import Context
+from .tensor import CUDA_STREAM_LEGACY, Context, torch_stream
 
 F32, I32 = torch.float32, torch.int32
 
@@ -50,13 +50,13 @@ def _shape(name: str, t, want):
 
 def _call(ctx: Context, fn, *args):
     """fn(ctx, *args) in order with torch's current stream."""
-    same = ctx.on_torch_stream()
-    if not same:
+    if ctx.stream == (torch_stream(ctx.device) or CUDA_STREAM_LEGACY):
+        status = fn(ctx.h, *args)
+        if status != OK:
+            check(status, ctx.h)
+    else:
         torch.cuda.current_stream(ctx.device).synchronize()
-    status = fn(ctx.h, *args)
-    if status != OK:
-        check(status, ctx.h)
-    if not same:
+        check(fn(ctx.h, *args), ctx.h)
         ctx.sync()
 
 
@@ -96,6 +96,8 @@ class PagedKVCache:
         check(lib().llmq_paged_create_in(ctx.h, KINDS[kind], n_layer, n_pages, page_size, n_kv_head, head_dim, *ptr,
                                          C.byref(h)), ctx.h)
         self.h = h
+        self._store, self._attend = lib().llmq_paged_store, lib().llmq_paged_attend
+        self._evict = lib().llmq_paged_evict
 
     def store(self, layer: int, k, v, pos, table, seq=None):
         """Stores rows k, v [n, n_kv_head, head_dim] (any row stride: the
@@ -113,7 +115,7 @@ class PagedKVCache:
             sp = _check(ctx, "seq", seq, I32, 1)
             _shape("seq", seq, (n,))
         tp = _check(ctx, "table", table, I32, 2)
-        _call(ctx, lib().llmq_paged_store, self.h, layer, kp, k.stride(0), vp, v.stride(0), sp, pp, n, tp,
+        _call(ctx, self._store, self.h, layer, kp, k.stride(0), vp, v.stride(0), sp, pp, n, tp,
               table.stride(0), table.shape[1], table.shape[0])
 
     def attend(self, layer: int, q, table, lens, max_len: int, scale: float | None = None, out=None, weights=None,
@@ -121,9 +123,9 @@ class PagedKVCache:
         """Attention of q [n_seqs, n_head, head_dim], one new token per
         sequence, over its first lens[b] <= max_len positions; returns out of
         q's shape. scale: 1 / sqrt(head_dim) unless given. With weights
-        and/or weights_out ([n_seqs, n_kv_head, >= max_len], weights_out =
-        weights for in place), weights_out = weights + the softmax weights
-        summed over each kv head's query heads."""
+        and/or weights_out ([n_seqs, n_kv_head, >= max_len], of one layout;
+        weights_out = weights for in place), weights_out = weights + the
+        softmax weights summed over each kv head's query heads."""
         ctx = self.ctx
         qp = _check(ctx, "q", q, F32, 3, 2)
         n, n_head, dim = q.shape
@@ -140,20 +142,24 @@ class PagedKVCache:
             raise ValueError("table, lens and q must have a row per sequence")
         wp = wop = None
         stride = 0
-        if weights is not None and weights_out is None:
-            raise ValueError("weights without weights_out")
-        if weights_out is not None:
+        if weights_out is None:
+            if weights is not None:
+                raise ValueError("weights without weights_out")
+        else:
             wop = _check(ctx, "weights_out", weights_out, F32, 3)
-            stride = weights_out.stride(1)
-            for name, w in (("weights", weights), ("weights_out", weights_out)):
-                if w is None:
-                    continue
-                wp = _check(ctx, name, w, F32, 3) if name == "weights" else wp
-                if w.shape[0] != n or w.shape[1] != self.n_kv_head or w.shape[2] < max_len:
-                    raise ValueError(f"{name} must be [{n}, {self.n_kv_head}, >= {max_len}]")
-                if w.stride(1) != stride or (n > 1 and w.stride(0) != stride * self.n_kv_head):
-                    raise ValueError("weights and weights_out must have the same evenly spaced rows")
-        _call(ctx, lib().llmq_paged_attend, self.h, layer, qp, q.stride(0), op, out.stride(0), n, n_head, tp,
+            rows = weights_out.stride()
+            stride = rows[1]
+            if n > 1 and rows[0] != stride * self.n_kv_head:
+                raise ValueError("weights_out must have evenly spaced rows")
+            shape = weights_out.shape
+            if shape[0] != n or shape[1] != self.n_kv_head or shape[2] < max_len:
+                raise ValueError(f"weights_out must be [{n}, {self.n_kv_head}, >= {max_len}]")
+            if weights is not None:
+                wp = _check(ctx, "weights", weights, F32, 3)
+                if weights.shape != shape or weights.stride()[1:] != rows[1:] or (
+                        n > 1 and weights.stride(0) != rows[0]):
+                    raise ValueError("weights must have the shape and strides of weights_out")
+        _call(ctx, self._attend, self.h, layer, qp, q.stride(0), op, out.stride(0), n, n_head, tp,
               table.stride(0), table.shape[1], lp, max_len, self.scale if scale is None else scale, wp, wop, stride)
         return out
 
@@ -183,7 +189,7 @@ class PagedKVCache:
             raise ValueError("budget must be positive")
         rows = (n_layers, n, self.n_kv_head, budget)
         kept, wout, lens_out = lens.new_empty(rows), weights.new_empty(rows), torch.empty_like(lens)
-        _call(ctx, lib().llmq_paged_evict, self.h, layer0, n_layers, n, tp, table.stride(0), table.shape[1], lp, max_len,
+        _call(ctx, self._evict, self.h, layer0, n_layers, n, tp, table.stride(0), table.shape[1], lp, max_len,
               wp, ws, budget, sinks, recent, dp, dst_table.stride(0), dst_table.shape[1], kept.data_ptr(),
               wout.data_ptr(), budget, lens_out.data_ptr())
         return kept, wout, lens_out
@@ -287,9 +293,11 @@ def process_logits(ctx: Context, logits, rules: LogitRules, out=None, argmax=Non
         op = _check(ctx, "out", out, F32, 2)
         _shape("out", out, (n, V))
     if argmax is None:
-        argmax = logits.new_empty(n, dtype=I32)
-    ap = _check(ctx, "argmax", argmax, I32, 1)
-    _shape("argmax", argmax, (n,))
+        argmax = torch.empty(n, dtype=I32, device=logits.device)
+        ap = argmax.data_ptr()
+    else:
+        ap = _check(ctx, "argmax", argmax, I32, 1)
+        _shape("argmax", argmax, (n,))
     _call(ctx, lib().llmq_process_logits, lp, logits.stride(0), op, out.stride(0), n, V,
           C.byref(rules._struct(ctx, n, V)), ap)
     return out, argmax

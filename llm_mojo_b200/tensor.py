@@ -20,12 +20,19 @@ from ._lib import check, lib
 CUDA_STREAM_LEGACY = 1  # cudaStreamLegacy
 
 
+_raw_stream = None
+
+
 def torch_stream(device: int) -> int:
     """The handle of torch's current stream."""
-    import torch
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
 
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without the stream object, 1 us less
-    return raw(device) if raw else torch.cuda.current_stream(device).cuda_stream
+        # without the stream object, 1 us less
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
 
 
 def _ptr(a: np.ndarray):
