@@ -1,8 +1,16 @@
 // logits.cuh -- the rules between the head and the sampler: penalties for
 // repeated tokens, biases and a mask of the allowed tokens.
 //
-// Each logit is read and written once, so memory bounds large calls and
-// latency small ones; in between it is the instructions per logit that count.
+// Each logit is read and written once, so memory bounds a call in the end:
+// 256 x 50257 without rules takes 20 us, 5.2 TB/s (a device-to-device copy of
+// the same rows through torch 34 us). With every rule 33 us, 3.2 TB/s: 830
+// instructions a warp per 512 logits, 440 of them without rules, fill 73% of
+// the issue slots, and CTAs wait at their barriers for the history. Tried and
+// slower: persistent CTAs with the next tile's loads ahead (66 us), counts
+// scattered into per-token cells in global memory before one streaming pass
+// (67), the touched tokens listed and worked out by a thread each (35.5) or
+// dealt to each warp's lanes (35.6), tiles of 8192 (38). One row: 5 us, the
+// latency of a CTA and of the tickets.
 #pragma once
 
 #include "common.cuh"

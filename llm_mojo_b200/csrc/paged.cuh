@@ -175,7 +175,8 @@ __device__ __forceinline__ float4 row_load4(const float *p, int j, int n) {
 // head's query heads of their softmax weight of position j (0 past the
 // length) for j < n: four positions a thread, the heads' scores (which the
 // attention left in L2) in head order. Launched to overlap the attention's
-// end. grid (ceil(n / 1024), n_seqs * n_kv_head), 256 threads.
+// end. Latency and L2 bound it: about 8 us after 8 sequences x <=32768 with 4
+// heads to a kv head. grid (ceil(n / 1024), n_seqs * n_kv_head), 256 threads.
 template <bool VEC>
 __global__ void __launch_bounds__(256) paged_weights_kernel(AttendArgs a, int n, const float *win, float *wout,
                                                             long long stride) {

@@ -24,7 +24,23 @@
 // bytes of row lane / 4), V transposed (a pair of rows). For int8 the
 // transposed element is a pair of codes, which one byte permute each turns
 // into two operands. Copies in flight cost no registers, and warps wait for
-// nothing but their own copies.
+// nothing but their own copies. (Rows permuted by exclusive-or instead of
+// padded: grouped bfloat16 126 us against 105; 8-byte copies into per-lane
+// slots, without ldmatrix: L1 at 77% and 157 us.)
+//
+// mma.sync, not tcgen05: a new token brings 8 columns to a row of the cache,
+// and the tensor pipe is 18-29% busy while memory is the limit; tcgen05 would
+// want the rows as 16-bit tiles in shared memory, so int8 codes converted,
+// written back and read again.
+//
+// What bounds it (B200, device times; the copy rate is 6.53 TB/s): bytes in
+// long calls, 8 sequences x <=32768 positions, 32 heads on 8 of 128, bfloat16:
+// 99 us, 5.3 TB/s; one sequence x 131071, 12 heads of 64, int8: 48 us, 4.4
+// TB/s, of which about 9 us are the start and the join of the chunks (524288
+// positions: 164 us, 5.2 TB/s), and 190 instructions per 16 positions fill
+// half of the issue slots; latency and those instructions in batches of short
+// sequences, 256 x <=256, 12 heads of 64, int8: 18 us, 3.1 TB/s; the latency
+// of one CTA in the smallest, 1 x 200: 4.0 us.
 #pragma once
 
 #include "paged.cuh"
