@@ -324,18 +324,18 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   const long long units = (long long)n_seqs * p->v.n_kv_head * a.head_chunks;
   // Fewer warps a CTA for many units of short sequences, whose prologues and
   // joins then cost less than idle warps do (int8, 64 dimensions, us with 1 /
-  // 2 / 4 warps: 3072 units x <=256 positions 22 / 25 / 33, 1536 x <=256 21 /
-  // 17 / 19, 576 x <=256 12 / 12 / 9)
+  // 2 / 4 warps: 3072 units x <=100 positions 13 / 17 / 23, 1536 x <=256 18 /
+  // 14 / 16, 576 x <=256 12 / 11 / 8)
   int warps = units >= ctx->num_sms * 16 && a.max_len <= 256 ? 1 : units >= ctx->num_sms * 8 ? 2 : 4;
   AttendKernel *k;
   if ((st = attend_kernel(ctx, a, warps, &k)) != LLMQ_OK) return st;
-  // Chunks, in whole blocks, two at least (1 x 200 positions: 4.8 us, 7.4 in
-  // single blocks, which have to be joined), at most kPmJoin of a unit: as
-  // many as the GPU holds CTAs at once for one sequence (131071 positions:
-  // 48 us, 53 with twice as many), twice that for several, of which only the
-  // longest fill their chunks (8 ragged sequences: 109 us, 150 with one wave)
+  // Chunks, in whole blocks, two at least (1 x 200 positions: 3.9 us, 6.2 in
+  // single blocks, which have to be joined), at most kPmJoin of a unit: twice
+  // as many as the GPU holds CTAs at once, since only the longest sequences
+  // fill theirs (8 ragged sequences x <=32768: 105 us, 126 with once as many;
+  // one sequence x 131071: 48 us with either)
   const long long wave = (long long)ctx->num_sms * k->per_sm[ctx->device % kMaxDevices];
-  const long long fit = std::min((long long)kPmJoin, std::max(1LL, (n_seqs == 1 ? 1 : 2) * wave / units));
+  const long long fit = std::min((long long)kPmJoin, std::max(1LL, 2 * wave / units));
   const long long blocks = (a.max_len + k->block - 1) / k->block;
   a.chunk = (int)std::max(2LL, (blocks + fit - 1) / fit) * k->block;
   a.splits = (a.max_len + a.chunk - 1) / a.chunk;

@@ -777,3 +777,67 @@ def test_c_owned_pool(torch, ctx, kind):
     for ptr in ((None, b.data_ptr()), (b.data_ptr(), b.data_ptr() + 4)):
         assert L.llmq_paged_create_in(ctx.h, KINDS[kind], 1, 1, 4, 1, 32, *ptr, b.data_ptr(), b.data_ptr(),
                                       C.byref(h)) == _lib.ERR_INVALID and not h
+
+
+def test_capture(torch):
+    """Calls captured in a graph replay with new inputs; a workspace that
+    would have to grow during a capture is refused, and the capture goes on."""
+    from llm_mojo_b200._lib import ERR_INVALID, LlmqError
+    from llm_mojo_b200.serving import LogitRules, process_logits
+    from llm_mojo_b200.tensor import Context
+
+    own = Context(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        own.use_torch_stream()
+        lens = [700, 90]
+        table, n_pages = make_table(torch, lens, 16, 3)
+        c = make_cache(torch, own, "bf16", 1, n_pages, 16, 2, 64, 4)
+        q = torch.randn(2, 4, 64, device="cuda")
+        ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        w, wo = torch.zeros(2, 2, 700, device="cuda"), torch.zeros(2, 2, 700, device="cuda")
+        x = torch.randn(2, 50257, device="cuda")
+        pen = torch.full((2,), 1.2, device="cuda")
+        ids = torch.randint(0, 50257, (2, 50), dtype=torch.int32, device="cuda")
+        rules = LogitRules(repetition=pen, ids=ids, n_ids=torch.full((2,), 50, dtype=torch.int32, device="cuda"))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            with pytest.raises(LlmqError) as e:
+                c.attend(0, q, table, ln, 700, weights=w, weights_out=wo)
+            assert e.value.status == ERR_INVALID
+            q.add_(0.0)
+        c.attend(0, q, table, ln, 700, weights=w, weights_out=wo)
+        process_logits(own, x, rules)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = c.attend(0, q, table, ln, 700, weights=w, weights_out=wo)
+            y, top = process_logits(own, x, rules)
+        for _ in range(3):
+            q.normal_()
+            x.normal_()
+            graph.replay()
+            got = [t.clone() for t in (out, wo, y, top)]
+            w2 = torch.zeros_like(wo)
+            want = [c.attend(0, q, table, ln, 700, weights=w, weights_out=w2), w2, *process_logits(own, x, rules)]
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        side.synchronize()
+        del graph
+    c.free()
+    own.close()
+
+
+@pytest.mark.parametrize("kind", PAGED)
+def test_attend_nan_stays_in_its_head(torch, ctx, kind):
+    """A query with a NaN gives NaN for its own head; the others, of the same
+    key head, too, are as without it."""
+    table, n_pages = make_table(torch, [150], 16, 3)
+    c = make_cache(torch, ctx, kind, 1, n_pages, 16, 2, 64, 4)
+    q = torch.randn(1, 8, 64, device="cuda")
+    ln = torch.tensor([150], dtype=torch.int32, device="cuda")
+    want = c.attend(0, q, table, ln, 150)
+    q[0, 5, 11] = float("nan")
+    got = c.attend(0, q, table, ln, 150)
+    assert torch.isnan(got[0, 5]).all()
+    keep = [0, 1, 2, 3, 4, 6, 7]
+    assert torch.equal(got[0, keep], want[0, keep])
