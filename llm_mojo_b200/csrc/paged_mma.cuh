@@ -156,8 +156,10 @@ struct PmShape {
   static constexpr int kRow = D * kEs, kNc = kRow / 16;  // bytes and 16-byte pieces of a row
   static constexpr int kPad = kRow + 16;                 // a row in the ring: an odd number of pieces
   static constexpr int kSteps = D / 16;  // steps of the scores; and tiles of dimensions of the output
-  // tiles of 16 positions taken together: two while their operands fit in registers
-  static constexpr int kU = kRow <= 128 ? 2 : 1;
+  // tiles of 16 positions taken together: two while their operands fit in
+  // registers (one in the one-warp CTAs, more of which an SM then holds: 256 x
+  // <=256 17.8 us against 18.3)
+  static constexpr int kU = kRow <= 128 && W > 1 ? 2 : 1;
   // a stage of a warp's ring, for each tile: 16 rows of K, 16 of V, and (int8) their scales
   static constexpr int kVat = 16 * kPad, kSat = 32 * kPad, kTile = kSat + (KIND == PM_I8 ? 128 : 0);
   static constexpr int kStage = kU * kTile;
