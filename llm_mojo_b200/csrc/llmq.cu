@@ -2283,8 +2283,12 @@ int fmt_code(const llmq_weight *w) { return fmt_of(w->view()); }
 constexpr int TCL_TT = 16;          // sequences per lane-mode GEMM tile
 constexpr int TCL_MIN_SEQS = 16;    // AUTO: the lane-mode GEMM from this many sequences
 
-// Whether batch_linear runs w for B sequences as the lane-mode tcgen05 GEMM.
+// Whether batch_linear runs w for B sequences as the lane-mode tcgen05 GEMM:
+// BLOCKED int4 rows as a layer (its epilogue writes the outputs, with bias,
+// GELU and residual), per-channel int8 rows as the head (argmax candidates or
+// the plain logits).
 bool batch_uses_tcl(const llmq_batch *bt, const llmq_weight *w, int B) {
+  if ((w == bt->m->head) != (w->bits == 8)) return false;
   if (!w->tcl_a || bt->kernel == LLMQ_BATCH_CUDA_CORE) return false;
   return bt->kernel == LLMQ_BATCH_TCGEN05 || B >= TCL_MIN_SEQS;
 }
