@@ -189,16 +189,18 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(AttendArgs a, int n,
     float4 w = win ? row_load4<VEC>(win + (size_t)u * stride, j, n) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (j < len) {
       const size_t r0 = (size_t)b * a.n_head + kh * G;
+      float4 p = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // the heads' sum, rounded into w once
 #pragma unroll 4
       for (int g = 0; g < G; g++) {
         const float4 s = *(const float4 *)(a.scores + (r0 + g) * a.score_stride + j);
         const float2 st = *(const float2 *)(a.stat + 2 * (r0 + g));
         const float M = st.x == -INFINITY ? 0.0f : st.x, inv = st.y > 0.0f ? 1.0f / st.y : st.y;
-        w.x = fmaf(exp2_approx(s.x - M), inv, w.x);
-        if (j + 1 < len) w.y = fmaf(exp2_approx(s.y - M), inv, w.y);
-        if (j + 2 < len) w.z = fmaf(exp2_approx(s.z - M), inv, w.z);
-        if (j + 3 < len) w.w = fmaf(exp2_approx(s.w - M), inv, w.w);
+        p.x = fmaf(exp2_approx(s.x - M), inv, p.x);
+        if (j + 1 < len) p.y = fmaf(exp2_approx(s.y - M), inv, p.y);
+        if (j + 2 < len) p.z = fmaf(exp2_approx(s.z - M), inv, p.z);
+        if (j + 3 < len) p.w = fmaf(exp2_approx(s.w - M), inv, p.w);
       }
+      w.x += p.x, w.y += p.y, w.z += p.z, w.w += p.w;
     }
     float *o = wout + (size_t)u * stride + j;
     if (VEC && j + 3 < n) {

@@ -40,7 +40,7 @@
 // positions: 164 us, 5.2 TB/s), and 190 instructions per 16 positions fill
 // half of the issue slots; latency and those instructions in batches of short
 // sequences, 256 x <=256, 12 heads of 64, int8: 18 us, 3.1 TB/s; the latency
-// of one CTA in the smallest, 1 x 200: 4.0 us.
+// of one CTA in the smallest, 1 x 200: 4.1 us.
 #pragma once
 
 #include "paged.cuh"
@@ -52,11 +52,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The first product of a sum, from c in the even columns and 0 in the odd.
-__device__ __forceinline__ void mma_f16_from(float (&d)[4], float c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+// The first products of a sum.
+__device__ __forceinline__ void mma_f16_from0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c), "f"(0.0f));
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void mma_bf16_from0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -105,19 +105,15 @@ __device__ __forceinline__ float pm_read1(unsigned src) {
 }
 
 // Two f16 from two biased codes (code ^ 0x80) in bytes i and j of x: 1024 +
-// byte, less 1152; all exact. For V: its sums nearly cancel, and a bias left
-// in them would cost their low bits.
+// byte, less 1152; all exact. (Keys as subnormals with the bias taken from
+// the accumulator's start: 3% faster, 25% less accurate; values that way
+// would lose the low bits of sums that nearly cancel.)
 __device__ __forceinline__ uint32_t codes_f16(uint32_t x, uint32_t sel) {
   const uint32_t h = __byte_perm(x, 0x64646464u, sel), off = 0x64806480u;
   uint32_t r;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(off));
   return r;
 }
-
-// The same as subnormals, 2^-24 (code + 128). For K: the bias is 128 2^-24
-// times the sum of the query, which the score's accumulator starts from, of
-// the size of the products themselves.
-__device__ __forceinline__ uint32_t codes_sub(uint32_t x, uint32_t sel) { return __byte_perm(x, 0u, sel); }
 
 // x, y as two f16 terms each: hi = (f16 x, f16 y), lo = the rest.
 __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo) {
@@ -157,8 +153,8 @@ struct PmShape {
   static constexpr int kPad = kRow + 16;                 // a row in the ring: an odd number of pieces
   static constexpr int kSteps = D / 16;  // steps of the scores; and tiles of dimensions of the output
   // tiles of 16 positions taken together: two while their operands fit in
-  // registers (one in the one-warp CTAs, more of which an SM then holds: 256 x
-  // <=256 17.8 us against 18.3)
+  // registers (one in the one-warp CTAs, more of which an SM then holds: 3% on
+  // 256 x <=256)
   static constexpr int kU = kRow <= 128 && W > 1 ? 2 : 1;
   // a stage of a warp's ring, for each tile: 16 rows of K, 16 of V, and (int8) their scales
   static constexpr int kVat = 16 * kPad, kSat = 32 * kPad, kTile = kSat + (KIND == PM_I8 ? 128 : 0);
@@ -354,11 +350,10 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
   // the query's operand, kept for the whole chunk: the first or the second
   // term (int8, bfloat16), qb the third of bfloat16 in the even columns
   uint32_t qa[HT][NT][2], qb[HT][I8 ? 1 : NT][2];
-  float fs[HT], cb[HT];  // of the lane's own head t: the scores' factor, and (int8) where they start
+  float fs[HT];  // the scores' factor of the lane's own head t
 #pragma unroll
   for (int ht = 0; ht < HT; ht++) {
     fs[ht] = a.scale2;
-    cb[ht] = 0.0f;
     if constexpr (I8) {
       // the largest |q| of the head to [2^13, 2^14): the second terms reach 2^-38 of it
       float mx = 0.0f;
@@ -369,8 +364,7 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const int e = min(max((int)(__float_as_uint(mx) >> 23), 1), 254) - 127;
-      const float up = pow2i(min(13 - e, 126)), down = a.scale2 * pow2i(max(e - 13, -126)) * 0x1p24f;
-      float sum = 0.0f;  // of the column's term
+      const float up = pow2i(min(13 - e, 126)), down = a.scale2 * pow2i(max(e - 13, -126));
 #pragma unroll
       for (int k = 0; k < NT; k++)
 #pragma unroll
@@ -378,13 +372,7 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
           uint32_t hi, lo;
           split_f16(xq[ht][k][i] * up, xq[ht][k][i + 1] * up, hi, lo);
           qa[ht][k][i / 2] = g & 1 ? lo : hi;
-          const float2 f = __half22float2(*(const __half2 *)&qa[ht][k][i / 2]);
-          sum += f.x + f.y;
         }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 4);  // both terms
-      cb[ht] = -0x1p-17f * __shfl_sync(0xffffffffu, sum, 8 * t);
       fs[ht] = __shfl_sync(0xffffffffu, down, 8 * t);
     } else {
 #pragma unroll
@@ -431,11 +419,11 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
           for (int k = 0; k < NT; k++) {
             if constexpr (I8) {
               const uint32_t x = kr[k] ^ 0x80808080u, y = kr[NC + k] ^ 0x80808080u;
-              const uint32_t f[4] = {codes_sub(x, 0x4140), codes_sub(y, 0x4140), codes_sub(x, 0x4342), codes_sub(y, 0x4342)};
+              const uint32_t f[4] = {codes_f16(x, 0x4140), codes_f16(y, 0x4140), codes_f16(x, 0x4342), codes_f16(y, 0x4342)};
 #pragma unroll
               for (int ht = 0; ht < HT; ht++) {
                 if (k == 0)
-                  mma_f16_from(c[ht], cb[ht], f, qa[ht][k][0], qa[ht][k][1]);
+                  mma_f16_from0(c[ht], f, qa[ht][k][0], qa[ht][k][1]);
                 else
                   mma_f16(c[ht], f, qa[ht][k][0], qa[ht][k][1]);
               }
@@ -617,8 +605,13 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
                 }
 #pragma unroll
                 for (int ht = 0; ht < HT; ht++) {
-                  mma_bf16(acc[ht][j], w, pa[ht][0], pa[ht][1]);
-                  mma_bf16(acc[ht][j], w, pb[ht][0], pb[ht][1]);
+                  // into the running sum with a rounded addition: the products' own truncates, which adds up along
+                  // a chunk (three times the error)
+                  float o[4];
+                  mma_bf16_from0(o, w, pb[ht][0], pb[ht][1]);
+                  mma_bf16(o, w, pa[ht][0], pa[ht][1]);
+#pragma unroll
+                  for (int i = 0; i < 4; i++) acc[ht][j][i] += o[i];
                 }
               } else {
                 uint32_t f[3][4];
@@ -635,9 +628,12 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
                 }
 #pragma unroll
                 for (int ht = 0; ht < HT; ht++) {
-                  mma_bf16(acc[ht][j], f[0], pb[ht][0], pb[ht][1]);
+                  float o[4];
+                  mma_bf16_from0(o, f[0], pb[ht][0], pb[ht][1]);
 #pragma unroll
-                  for (int k = 2; k >= 0; k--) mma_bf16(acc[ht][j], f[k], pa[ht][0], pa[ht][1]);
+                  for (int k = 2; k >= 0; k--) mma_bf16(o, f[k], pa[ht][0], pa[ht][1]);
+#pragma unroll
+                  for (int i = 0; i < 4; i++) acc[ht][j][i] += o[i];
                 }
               }
             }
