@@ -56,8 +56,9 @@ __device__ __forceinline__ float4 evict_load(const float *w, int j, int len) {
 // prefix sum of (above the threshold or always kept, equal to it) per 4 NTH
 // positions, of the equal ones the first `ties`. The row is read three or
 // four times, but for the first time from L2; instructions bound it, and, in
-// short rows, barriers: NTH 256 up to 2048 positions (144 rows of 1024: 6
-// us, 10 with 1024 threads), 1024 beyond.
+// short rows, barriers and latency: NTH 256 up to 2048 positions (144 rows of
+// 1024, profiled alone: 9.5 us, 10.1 with 1024 threads and three times the
+// instructions), 1024 beyond (256 rows of <=16384: 28 us).
 // grid (n_layers * n_seqs * n_kv_head), NTH threads.
 constexpr int kEvList = 4096;
 
@@ -198,7 +199,7 @@ constexpr int kEvPos = 64;  // kept positions that a CTA moves
 // row (layer, sequence, kv head) per CTA: 16-byte pieces, 8 in flight a
 // thread. NV: pieces of a cache row. Memory bounds it: 4 layers x 8 sequences
 // x 8 heads, <=4096 rows of 256 bytes kept in each: 139 us at 6.1 TB/s; 144
-// rows of 512 x 256 bytes, one and a half waves of CTAs: 13 us, 5.8 TB/s.
+// rows of 512 x 256 bytes, one and a half waves of CTAs: 15 us, 5.1 TB/s.
 template <int NV>
 __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, int tiles) {
   __shared__ long long from[kEvPos], to[kEvPos];  // rows; from < 0: nothing to move

@@ -76,8 +76,8 @@ __device__ __forceinline__ void pack_store(typename E::T *dst, const float4 &x, 
 // page is looked up once, and 2 kStoreHeads loads are in flight a lane.
 // int8: s = max|x| / 127 (1 when 0), codes round(x * (1 / s)), half away from
 // zero, as QuantKV.quantize (kvcache.mojo:319-331). VEC: 16-byte loads
-// (aligned rows). Memory bounds it: 16387 rows of 8 x 128 to bfloat16 take 35
-// us at 5.8 TB/s (with the lookup in every head's lanes, 41). grid of 256
+// (aligned rows). Memory bounds it: 16387 rows of 8 x 128 to bfloat16 take 33
+// us at 6.2 TB/s (with the lookup in every head's lanes, 41). grid of 256
 // threads over (row, block of heads).
 constexpr int kStoreHeads = 4;
 
@@ -175,8 +175,8 @@ __device__ __forceinline__ float4 row_load4(const float *p, int j, int n) {
 // head's query heads of their softmax weight of position j (0 past the
 // length) for j < n: four positions a thread, the heads' scores (which the
 // attention left in L2) in head order. Launched to overlap the attention's
-// end. Latency and L2 bound it: about 8 us after 8 sequences x <=32768 with 4
-// heads to a kv head. grid (ceil(n / 1024), n_seqs * n_kv_head), 256 threads.
+// end. Latency and L2 bound it: about 6 us after 8 sequences x <=32768 with 4
+// heads to a kv head (12 alone, with cold caches). grid (ceil(n / 1024), n_seqs * n_kv_head), 256 threads.
 template <bool VEC>
 __global__ void __launch_bounds__(256) paged_weights_kernel(AttendArgs a, int n, const float *win, float *wout,
                                                             long long stride) {

@@ -35,7 +35,7 @@
 //
 // What bounds it (B200, device times; the copy rate is 6.53 TB/s): bytes in
 // long calls, 8 sequences x <=32768 positions, 32 heads on 8 of 128, bfloat16:
-// 99 us, 5.3 TB/s; one sequence x 131071, 12 heads of 64, int8: 48 us, 4.4
+// 99 us, 5.3 TB/s (104 with the weights); one sequence x 131071, 12 heads of 64, int8: 48 us, 4.4
 // TB/s, of which about 9 us are the start and the join of the chunks (524288
 // positions: 164 us, 5.2 TB/s), and 190 instructions per 16 positions fill
 // half of the issue slots; latency and those instructions in batches of short
