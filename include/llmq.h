@@ -329,7 +329,9 @@ llmq_status llmq_batch_generate_async(llmq_ctx *ctx, llmq_batch *b, const int *p
  * sequence (kvcache.mojo) and whose sampler takes the head's logits as they
  * are. All calls are asynchronous on the context's stream; their workspaces
  * belong to the context, one per stream, and grow on first use (outside any
- * stream capture).
+ * stream capture). A captured call replays with the workspace that it was
+ * captured with, which lives as long as the context: replay it on the stream
+ * it was captured on, or with none of that stream's calls in flight.
  *
  * A paged cache: one pool of pages for all sequences, k and v
  * [n_layer][n_pages][n_kv_head][page_size][head_dim] in int8

@@ -6,6 +6,7 @@
 
 #include <map>
 #include <string>
+#include <vector>
 
 #include "../../include/llmq.h"
 
@@ -15,11 +16,15 @@ struct DecodeState;
 
 // The serving operators' device workspace on one stream: buf holds partial
 // results within a call, zeros (tickets, counts) is all zero between calls.
+// A buffer that became too small is kept with the context, for the graphs
+// captured with it; each is at least twice the one before where memory
+// allows, so that together they are no larger than the last.
 struct ServeWs {
   void *buf = nullptr;
   size_t bytes = 0;
   void *zeros = nullptr;
   size_t zero_bytes = 0;
+  std::vector<void *> retired;
 };
 
 struct llmq_ctx {

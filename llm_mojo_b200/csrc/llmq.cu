@@ -402,6 +402,7 @@ llmq_status llmq_destroy(llmq_ctx *ctx) {
   for (auto &w : ctx->serve_ws) {
     if (w.second.buf) cudaFree(w.second.buf);
     if (w.second.zeros) cudaFree(w.second.zeros);
+    for (void *q : w.second.retired) cudaFree(q);
   }
   if (ctx->own) cudaStreamDestroy(ctx->own);
   delete ctx;

@@ -20,23 +20,31 @@ struct llmq_paged {
 
 namespace {
 
-// Grows one of the workspace's buffers.
-llmq_status serve_grow(llmq_ctx *ctx, void **buf, size_t *have, size_t bytes, bool zero) {
+// Grows one of the workspace's buffers. The old one stays for calls in flight
+// and graphs captured with it.
+llmq_status serve_grow(llmq_ctx *ctx, ServeWs &w, void **buf, size_t *have, size_t bytes, bool zero) {
   if (*have >= bytes) return LLMQ_OK;
   cudaStreamCaptureStatus cap;
   CK(cudaStreamIsCapturing(ctx->stream, &cap));
   if (cap != cudaStreamCaptureStatusNone)
     return fail(ctx, LLMQ_ERR_INVALID, "the serving workspace grows on first use: run the call once before capturing it");
-  CK(cudaStreamSynchronize(ctx->stream));  // queued calls use the old one
-  if (*buf) cudaFree(*buf);
-  *buf = nullptr;
-  *have = 0;
-  if (cudaMalloc(buf, bytes) != cudaSuccess) {
+  void *grown = nullptr;
+  size_t size = std::max(bytes, 2 * *have);
+  cudaError_t e = cudaMalloc(&grown, size);
+  if (e != cudaSuccess && size > bytes) {
     cudaGetLastError();
-    return fail(ctx, LLMQ_ERR_NOMEM, "serving workspace of " + std::to_string(bytes) + " bytes");
+    size = bytes;
+    e = cudaMalloc(&grown, size);
   }
-  if (zero) CK(cudaMemsetAsync(*buf, 0, bytes, ctx->stream));
-  *have = bytes;
+  if (e == cudaSuccess && zero && (e = cudaMemsetAsync(grown, 0, size, ctx->stream)) != cudaSuccess) cudaFree(grown);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ctx, e == cudaErrorMemoryAllocation ? LLMQ_ERR_NOMEM : LLMQ_ERR_CUDA,
+                "serving workspace of " + std::to_string(bytes) + " bytes: " + cudaGetErrorString(e));
+  }
+  if (*buf) w.retired.push_back(*buf);
+  *buf = grown;
+  *have = size;
   return LLMQ_OK;
 }
 
@@ -44,8 +52,8 @@ llmq_status serve_grow(llmq_ctx *ctx, void **buf, size_t *have, size_t bytes, bo
 // that are zero.
 llmq_status serve_ws(llmq_ctx *ctx, size_t bytes, size_t zeros, ServeWs **out) {
   ServeWs &w = ctx->serve_ws[ctx->stream];
-  llmq_status st = serve_grow(ctx, &w.buf, &w.bytes, bytes, false);
-  if (st == LLMQ_OK) st = serve_grow(ctx, &w.zeros, &w.zero_bytes, zeros, true);
+  llmq_status st = serve_grow(ctx, w, &w.buf, &w.bytes, bytes, false);
+  if (st == LLMQ_OK) st = serve_grow(ctx, w, &w.zeros, &w.zero_bytes, zeros, true);
   *out = &w;
   return st;
 }

@@ -827,6 +827,49 @@ def test_capture(torch):
     own.close()
 
 
+def test_capture_outlives_the_workspace_it_used(torch):
+    """A captured call replays after larger ones have made the workspace grow."""
+    from llm_mojo_b200.serving import LogitRules, process_logits
+    from llm_mojo_b200.tensor import Context
+
+    own = Context(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        own.use_torch_stream()
+        lens = [700, 90]
+        table, n_pages = make_table(torch, lens, 16, 3)
+        c = make_cache(torch, own, "bf16", 1, n_pages, 16, 2, 64, 4)
+        q = torch.randn(2, 4, 64, device="cuda")
+        ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        wo = torch.zeros(2, 2, 700, device="cuda")
+        x = torch.randn(2, 5000, device="cuda")
+        rules = LogitRules()
+        c.attend(0, q, table, ln, 700, weights_out=wo)
+        process_logits(own, x, rules)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = c.attend(0, q, table, ln, 700, weights_out=wo)
+            y, top = process_logits(own, x, rules)
+        graph.replay()
+        want = [t.clone() for t in (out, wo, y, top)]
+        rows = 512
+        tables, lns = table[:1].repeat(rows, 1), ln[:1].repeat(rows)
+        many = torch.randn(rows, 4, 64, device="cuda")
+        for n in (64, 128, rows):
+            c.attend(0, many[:n], tables[:n], lns[:n], 700, weights_out=torch.empty(n, 2, 700, device="cuda"))
+        process_logits(own, torch.randn(rows, 5000, device="cuda"), rules)
+        for t in (out, wo, y, top):
+            t.zero_()
+        for _ in range(3):
+            graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip((out, wo, y, top), want))
+        side.synchronize()
+        del graph
+    c.free()
+    own.close()
+
+
 @pytest.mark.parametrize("kind", PAGED)
 def test_attend_nan_stays_in_its_head(torch, ctx, kind):
     """A query with a NaN gives NaN for its own head; the others, of the same
