@@ -83,7 +83,8 @@ __global__ void __launch_bounds__(NTH) logit_rules_kernel(RuleArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float *xr = a.x + r * a.x_stride;
   const int lead = (int)(((uintptr_t)xr >> 2) & 3);  // logits between the 16-byte boundary and the row's start
-  const int t0 = tile * T - lead, lo = max(t0, 0), hi = min(t0 + T, a.V);  // the tile's tokens: [lo, hi)
+  // the tile's tokens: [lo, hi), none in a last tile that only a row of a larger lead has tokens in
+  const int t0 = tile * T - lead, lo = max(t0, 0), hi = max(lo, min(t0 + T, a.V));
   const bool inner = t0 >= 0 && t0 + T <= a.V;
   const int at0 = warp * 32 * VPT + lane * 4;  // the thread's group i: slots at0 + 128 i on
   // the first quads of each thread's history, on their way with the logits
