@@ -335,10 +335,12 @@ __global__ void __launch_bounds__(W * 32, pm_per_sm(KIND, D, HT) * 4 / W) paged_
       }
       rows[i] = row;
     }
-    if constexpr (W > 1)
+    if constexpr (W > 1) {
       hole = __syncthreads_or(hole);
-    else
+    } else {
       hole = __any_sync(0xffffffffu, hole);
+      __syncwarp();  // the vote alone does not order the other lanes' rows before the copies below
+    }
 #pragma unroll
     for (int i = 0; i < S - 1; i++) {
       if ((warp + i * W) * U < ntiles) issue((warp + i * W) * U, i);

@@ -44,3 +44,99 @@ def test_rules_last_tile(torch, ctx, V, n, shift):
     out, top = process_logits(ctx, torch.from_numpy(x).cuda()[:, shift: shift + V], to_rules(torch, r))
     want, best = rules_reference(np.ascontiguousarray(x[:, shift: shift + V]), **r)
     assert np.array_equal(out.cpu().numpy(), want) and np.array_equal(top.cpu().numpy(), best)
+
+
+# ---- attention ---------------------------------------------------------------
+
+
+def pool(torch, ctx, kind, n_pages, ps, hk, D, seed):
+    """A cache of one layer with random rows, and its values in 64 bits
+    [n_pages, n_kv_head, page_size, head_dim]."""
+    from llm_mojo_b200.serving import PagedKVCache
+
+    c = PagedKVCache(ctx, kind, 1, n_pages, ps, hk, D)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    val = []
+    for t, s in ((c.k, c.ks), (c.v, c.vs)):
+        if s is None:
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+            val.append(t[0].double())
+        else:
+            t.copy_(torch.randint(-127, 128, t.shape, generator=g, device="cuda", dtype=torch.int8))
+            s.copy_(torch.rand(s.shape, generator=g, device="cuda") * 0.03 + 0.002)
+            val.append(t[0].double() * s[0].double()[..., None])
+    return c, *val
+
+
+def check_attend(torch, c, k, v, q, table, lens, weighted):
+    """attend of every sequence against 64 bits, a table row after another.
+    Tolerance, of the values' largest: a score's rounding errors, one per
+    product and sum, add up like a random walk, four deviations of which
+    shift the weights by as much, relatively; the sums over positions
+    likewise; 16 roundings for exponentials, scales and the join."""
+    n, H, D = q.shape
+    hk, ps, top = c.n_kv_head, c.page_size, int(lens.max())
+    w = torch.rand(n, hk, top, device="cuda") if weighted else None
+    wo = torch.full_like(w, -7.0) if weighted else None
+    out = c.attend(0, q, table, lens, top, weights=w, weights_out=wo)
+    pos = torch.arange(top, device="cuda")
+    for b, length in enumerate(lens.tolist()):
+        page = table[b][pos[:length] // ps].long()
+        ok = (page >= 0) & (page < c.n_pages)
+        at = pos[:length][ok]
+        if not at.numel():
+            assert torch.count_nonzero(out[b]) == 0
+            assert not weighted or torch.equal(wo[b], w[b])
+            continue
+        kb, vb = k[page[ok], :, at % ps], v[page[ok], :, at % ps]  # [positions, kv head, D]
+        qb = q[b].double().view(hk, H // hk, D)
+        p = torch.softmax(torch.einsum("hgd,lhd->hgl", qb, kb) / D ** 0.5, -1)
+        smax = float(torch.einsum("hgd,lhd->hgl", qb.abs(), kb.abs()).max()) / D ** 0.5
+        rel = 2.0 ** -23 * (4 * D ** 0.5 * smax + 4 * at.numel() ** 0.5 + 16)
+        want = torch.einsum("hgl,lhd->hgd", p, vb).reshape(H, D)
+        assert float((out[b].double() - want).abs().max()) <= rel * float(vb.abs().max()), b
+        if weighted:
+            add = w[b].double()
+            add[:, at] += p.sum(1)
+            assert float((wo[b].double() - add).abs().max()) <= rel * (H // hk) + 2.0 ** -23 * (H // hk + 1), b
+
+
+@pytest.mark.parametrize("kind", ["int8", "bf16", "f32"])
+@pytest.mark.parametrize("n,hk,G,D,ps,top", [
+    # one warp a CTA: more than 16 units (sequence, kv head, up to 8 query heads) an SM, up to 256 positions
+    (256, 12, 1, 64, 16, 100),
+    (256, 12, 8, 64, 5, 100),
+    (208, 12, 1, 64, 5, 256),
+    (304, 8, 1, 128, 16, 77),
+    (304, 8, 3, 128, 7, 70),
+    (304, 8, 11, 32, 16, 60),
+    (304, 8, 6, 96, 48, 90),
+    # two: more than 8
+    (256, 12, 1, 64, 16, 300),
+    (256, 12, 2, 64, 5, 300),
+    (128, 12, 8, 64, 16, 300),
+    (160, 8, 1, 32, 1, 500),
+    (160, 8, 8, 96, 3, 280),
+    (160, 8, 5, 128, 64, 290),
+])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_attend_full_batches(torch, ctx, kind, n, hk, G, D, ps, top, weighted):
+    """Batches that fill the GPU with CTAs of one and of two warps, lengths
+    from nothing on, a missing page here and there."""
+    rng = np.random.default_rng(n + D + G)
+    lens = rng.integers(0, top + 1, n)
+    lens[:4] = top, 1, 0, min(top, 17)
+    need = -(-lens // ps)
+    n_pages = int(need.sum()) + 1
+    table = np.full((n, need.max()), -1, dtype=np.int32)
+    ids, at = rng.permutation(n_pages), 0
+    for b, x in enumerate(need):
+        table[b, :x] = ids[at: at + x]
+        at += x
+    table[5::9, 0] = -1
+    table[7::9, -1] = n_pages
+    c, k, v = pool(torch, ctx, kind, n_pages, ps, hk, D, 5)
+    q = torch.randn(n, hk * G, D, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda") * 1.5
+    check_attend(torch, c, k, v, q, torch.from_numpy(table).cuda(), torch.from_numpy(lens.astype(np.int32)).cuda(),
+                 weighted)
+    c.free()
