@@ -140,3 +140,54 @@ def test_attend_full_batches(torch, ctx, kind, n, hk, G, D, ps, top, weighted):
     check_attend(torch, c, k, v, q, torch.from_numpy(table).cuda(), torch.from_numpy(lens.astype(np.int32)).cuda(),
                  weighted)
     c.free()
+
+
+@pytest.mark.parametrize("kind", ["int8", "bf16", "f32"])
+def test_attend_long_sums_are_not_biased(torch, ctx, kind):
+    """Positive values with equal weights, 20000 positions in one chunk, of
+    which a warp has 313 tiles of 16. A tile's product may truncate 16
+    addends, 2^-24 of the largest, up to twice the mean, each: 2^-23 of the
+    sum, twice for the terms; what else is rounded is rounded to nearest: on
+    the average over all outputs 3 of 2^-23. An output alone: these, 16 for
+    the join, and 313 roundings like a random walk."""
+    n, hk, D, top, ps = 80, 12, 64, 20000, 16
+    n_pages = top // ps
+    c, _, _ = pool(torch, ctx, kind, n_pages, ps, hk, D, 3)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    c.k.zero_()
+    if kind == "int8":
+        c.v.copy_(torch.randint(1, 128, c.v.shape, generator=g, device="cuda", dtype=torch.int8))
+        c.vs.copy_(0.5 + 0.5 * torch.rand(c.vs.shape, generator=g, device="cuda"))
+    else:
+        c.v.copy_(0.1 + torch.rand(c.v.shape, generator=g, device="cuda"))
+    order = torch.randperm(n_pages, generator=g, device="cuda")
+    lens = [top - 7 * b for b in range(n)]
+    out = c.attend(0, torch.ones(n, hk, D, device="cuda"), order.to(torch.int32)[None].expand(n, -1),
+                   torch.tensor(lens, dtype=torch.int32, device="cuda"), top)
+    v = c.v[0].double() if c.vs is None else c.v[0].double() * c.vs[0].double()[..., None]
+    v = v[order].transpose(1, 2).reshape(top, hk, D)
+    want = torch.stack([v[:x].mean(0) for x in lens])
+    ulps = (out.double() - want) / want * 2.0 ** 23
+    assert abs(float(ulps.mean())) <= 3
+    assert float(ulps.abs().max()) <= 19 + (top / 64) ** 0.5
+    c.free()
+
+
+@pytest.mark.parametrize("kind", ["int8", "bf16", "f32"])
+@pytest.mark.parametrize("n,hk,G,D,ps,top", [(256, 12, 1, 64, 16, 9000), (80, 12, 1, 64, 24, 8500),
+                                             (60, 12, 2, 32, 5, 4200), (80, 8, 5, 96, 32, 4500)])
+def test_attend_chunks_of_several_runs(torch, ctx, kind, n, hk, G, D, ps, top):
+    """So many sequences that a chunk is a whole sequence, longer than the
+    4096 positions whose rows are looked up at a time; missing pages in the
+    second run."""
+    rng = np.random.default_rng(top)
+    need = -(-top // ps)
+    table = rng.permutation(need).astype(np.int32)
+    table[4100 // ps], table[-1] = -1, need
+    lens = rng.integers(4097, top + 1, n).astype(np.int32)
+    lens[:5] = top, 4096, 4097, 0, 8192 if top > 8192 else 4098
+    c, k, v = pool(torch, ctx, kind, need, ps, hk, D, 6)
+    q = torch.randn(n, hk * G, D, generator=torch.Generator(device="cuda").manual_seed(8), device="cuda") * 1.5
+    check_attend(torch, c, k, v, q, torch.from_numpy(table)[None].cuda().expand(n, -1), torch.from_numpy(lens).cuda(),
+                 True)
+    c.free()
