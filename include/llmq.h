@@ -392,7 +392,8 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
  * [n_seqs][dst_cols], whose pages must differ from the source's (pages
  * that sequences share are only read). kept_dev [n_layers][n_seqs]
  * [n_kv_head][budget]: the positions, -1 past n. weights_out_dev (same row
- * order, weights_out_stride floats apart): their weights, 0 past n.
+ * order, weights_out_stride floats apart): their weights, 0 from n to the
+ * budget; what lies between two rows' budgets is not written.
  * lens_out_dev[b] = n. The outputs overlap no input. Lengths are cut as in
  * llmq_paged_attend. */
 llmq_status llmq_paged_evict(llmq_ctx *ctx, llmq_paged *p, int layer0, int n_layers, int n_seqs, const int *table_dev,

@@ -76,8 +76,10 @@ __global__ void __launch_bounds__(NTH) evict_select_kernel(EvictArgs a) {
   float *wout = a.wout + row * a.wout_stride;
   int *kept = a.kept + (size_t)row * a.budget;
   if (row < a.src.n_seqs * a.c.n_kv_head && row % a.c.n_kv_head == 0 && tid == 0) a.lens_out[b] = n;
-  for (long long j = n + tid; j < a.wout_stride; j += NTH) wout[j] = 0.0f;
-  for (int j = n + tid; j < a.budget; j += NTH) kept[j] = -1;
+  for (int j = n + tid; j < a.budget; j += NTH) {
+    kept[j] = -1;
+    wout[j] = 0.0f;
+  }
   if (len <= a.budget) {
     for (int j = tid; j < len; j += NTH) {
       kept[j] = j;

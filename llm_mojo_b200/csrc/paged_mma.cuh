@@ -18,7 +18,7 @@
 // 8 in a row. What these choices cost stays below float32's own roundings:
 // root mean square errors against 64 bits, 64 x 200, 12 heads of 64, are
 // 4.7e-8 / 2.8e-8 / 3.5e-8 of the largest output (int8 / bfloat16 / float32;
-// 3.2e-8 with the product left out), in plain float32 10.0 / 5.9 / 6.4e-8.
+// 3.2e-8 with that product kept), in plain float32 10.0 / 5.9 / 6.4e-8.
 // A lane's accumulators are the terms of one head, so they add up in place,
 // and few query heads still fill the columns with what accuracy needs. P goes
 // from the accumulators' layout to the operand's by one transposing move per

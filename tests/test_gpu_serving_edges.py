@@ -191,3 +191,31 @@ def test_attend_chunks_of_several_runs(torch, ctx, kind, n, hk, G, D, ps, top):
     check_attend(torch, c, k, v, q, torch.from_numpy(table)[None].cuda().expand(n, -1), torch.from_numpy(lens).cuda(),
                  True)
     c.free()
+
+
+# ---- eviction ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("length", [48, 11])
+def test_evict_writes_only_its_rows(torch, ctx, length):
+    """Rows of weights inside a wider buffer: what lies between them, and
+    after the last, stays."""
+    from llm_mojo_b200 import _lib
+    from llm_mojo_b200.serving import PagedKVCache
+
+    c = PagedKVCache(ctx, "bf16", 1, 8, 16, 2, 64)
+    table = torch.tensor([[0, 1, 2]], dtype=torch.int32, device="cuda")
+    dst = torch.tensor([[4, 5]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([length], dtype=torch.int32, device="cuda")
+    w = torch.rand(2, 48, device="cuda")
+    wide = torch.full((4, 33), 7.0, device="cuda")  # two rows of 20
+    kept, n = torch.zeros(2, 20, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert _lib.lib().llmq_paged_evict(ctx.h, c.h, 0, 1, 1, table.data_ptr(), 3, 3, lens.data_ptr(), 48, w.data_ptr(),
+                                       48, 20, 0, 0, dst.data_ptr(), 2, 2, kept.data_ptr(), wide.data_ptr(), 33,
+                                       n.data_ptr()) == _lib.OK
+    for h in range(2):
+        keep = kept[h][kept[h] >= 0].long()
+        assert keep.numel() == min(length, 20) == int(n[0])
+        assert torch.equal(wide[h, : keep.numel()], w[h, keep]) and torch.count_nonzero(wide[h, keep.numel(): 20]) == 0
+    assert torch.all(wide[:, 20:] == 7.0) and torch.all(wide[2:] == 7.0)
+    c.free()
