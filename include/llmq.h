@@ -394,7 +394,12 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
  * [n_kv_head][budget]: the positions, -1 past n. weights_out_dev (same row
  * order, weights_out_stride floats apart): their weights, 0 from n to the
  * budget; what lies between two rows' budgets is not written.
- * lens_out_dev[b] = n. The outputs overlap no input. Lengths are cut as in
+ * lens_out_dev[b] = n. A position without a page in table_dev is selected as
+ * any other (the lowest weight, or NaN, leaves it out); if one is kept, in any
+ * row of sequence b, there is nothing to move, and lens_out_dev[b] = -1: the
+ * sequence is refused, and attended to with that length it is empty. A kept
+ * position whose page dst_table_dev does not have is not moved, and masked
+ * there. The outputs overlap no input. Lengths are cut as in
  * llmq_paged_attend. */
 llmq_status llmq_paged_evict(llmq_ctx *ctx, llmq_paged *p, int layer0, int n_layers, int n_seqs, const int *table_dev,
                              long long table_stride, int table_cols, const int *lens_dev, int max_len,

@@ -199,7 +199,8 @@ constexpr int kEvPos = 64;  // kept positions that a CTA moves
 
 // Moves the kept rows, key and value (and scales), of kEvPos positions of one
 // row (layer, sequence, kv head) per CTA: 16-byte pieces, 8 in flight a
-// thread. NV: pieces of a cache row. Memory bounds it: 4 layers x 8 sequences
+// thread. A sequence of which a kept position has no page gets length -1
+// (every CTA that sees one writes the same). NV: pieces of a cache row. Memory bounds it: 4 layers x 8 sequences
 // x 8 heads, <=4096 rows of 256 bytes kept in each: 139 us at 6.1 TB/s; 144
 // rows of 512 x 256 bytes, one and a half waves of CTAs: 15 us, 5.1 TB/s.
 template <int NV>
@@ -212,9 +213,12 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, int tiles)
   if (tid < kEvPos) {
     const int j = j0 + tid, s = j < a.budget ? a.kept[(size_t)row * a.budget + j] : -1;
     from[tid] = -1;
-    if (s >= 0 && j / ps < a.dst.cols) {
-      const int sp = a.src.page(b, s / ps), dp = a.dst.page(b, j / ps);
-      if (sp >= 0 && sp < a.c.n_pages && dp >= 0 && dp < a.c.n_pages) {
+    if (s >= 0) {
+      const int sp = a.src.page(b, s / ps), dp = j / ps < a.dst.cols ? a.dst.page(b, j / ps) : -1;
+      const bool there = sp >= 0 && sp < a.c.n_pages;
+      // nothing to move: slot j would hold what lay there before, and be attended to
+      if (!there) a.lens_out[b] = -1;
+      if (there && dp >= 0 && dp < a.c.n_pages) {
         from[tid] = (long long)a.c.row(layer, sp, h, s % ps);
         to[tid] = (long long)a.c.row(layer, dp, h, j % ps);
         if (a.c.ks) {

@@ -170,7 +170,9 @@ class PagedKVCache:
         [n_layers, n_seqs, n_kv_head, >= max_len]; their rows move in order to
         dst_table's pages, which must not be the source's. Returns (kept
         positions int32 [n_layers, n_seqs, n_kv_head, budget], -1 past the
-        kept; their weights, 0 past them; the new lengths int32 [n_seqs])."""
+        kept; their weights, 0 past them; the new lengths int32 [n_seqs], -1
+        for a sequence that would keep a position without a page: it is
+        refused, and attended to with that length it is empty)."""
         ctx, n = self.ctx, table.shape[0]
         n_layers = self.n_layer - layer0 if n_layers is None else n_layers
         tp, lp = _check(ctx, "table", table, I32, 2), _check(ctx, "lens", lens, I32, 1)

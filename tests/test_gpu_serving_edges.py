@@ -219,3 +219,36 @@ def test_evict_writes_only_its_rows(torch, ctx, length):
         assert torch.equal(wide[h, : keep.numel()], w[h, keep]) and torch.count_nonzero(wide[h, keep.numel(): 20]) == 0
     assert torch.all(wide[:, 20:] == 7.0) and torch.all(wide[2:] == 7.0)
     c.free()
+
+
+@pytest.mark.parametrize("kind", ["int8", "bf16", "f32"])
+@pytest.mark.parametrize("budget", [20, 60])  # below and above the lengths
+def test_evict_refuses_positions_without_a_page(torch, ctx, kind, budget):
+    """A sequence that would keep a position whose page is missing gets
+    length -1, and attention gives zeros for it, not what the destination
+    held; missing positions that are not kept do not matter."""
+    c, k, v = pool(torch, ctx, kind, 20, 16, 2, 64, 4)
+    for t in (c.k, c.v) if kind != "int8" else (c.ks, c.vs):
+        t[0, 8:] = float("nan")  # the destinations
+    table = torch.tensor([[0, -1, 2], [3, 4, 5], [0, 20, 2]], dtype=torch.int32, device="cuda")
+    dst = torch.arange(8, 20, dtype=torch.int32, device="cuda").view(3, 4)
+    lens = torch.tensor([48, 48, 48], dtype=torch.int32, device="cuda")
+    w = torch.rand(1, 3, 2, 48, device="cuda") + 1.0
+    w[:, 2, :, 16:32] = float("nan")
+    kept, _, got = c.evict(table, lens, 48, w, budget, dst, sinks=2, recent=3)
+    n = min(48, budget)
+    assert got.tolist() == [-1, n, n if budget == 20 else -1]
+    q = torch.randn(3, 4, 64, device="cuda")
+    out = c.attend(0, q, dst, got, n)
+    for b in range(3):
+        if got[b] < 0:
+            assert torch.count_nonzero(out[b]) == 0
+            continue
+        for h in range(4):
+            at = kept[0, b, h // 2, :n].long()
+            kb, vb = (x[table[b][at // 16].long(), h // 2, at % 16] for x in (k, v))
+            p = torch.softmax(kb @ q[b, h].double() / 8, 0)
+            smax = float((kb.abs() @ q[b, h].double().abs()).max()) / 8
+            tol = 2.0 ** -23 * (32 * smax + 4 * n ** 0.5 + 16) * float(vb.abs().max())
+            assert float((out[b, h].double() - p @ vb).abs().max()) <= tol
+    c.free()
