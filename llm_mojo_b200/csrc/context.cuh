@@ -74,4 +74,9 @@ inline llmq_status fail(llmq_ctx *ctx, llmq_status st, const std::string &msg) {
     if (e_ != cudaSuccess) return fail(ctx, LLMQ_ERR_CUDA, std::string("launch: ") + cudaGetErrorString(e_)); \
   } while (0)
 
+// Whether llmq_paged_store and llmq_paged_attend would refuse a step over
+// n_layers layers of p with these arguments (serving.cu).
+llmq_status paged_step_check(llmq_ctx *ctx, const llmq_paged *p, int n_layers, const int *table, long long table_stride,
+                             int table_cols, int n_seqs, int max_len);
+
 }  // namespace llmq

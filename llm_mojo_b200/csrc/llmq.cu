@@ -2737,12 +2737,14 @@ llmq_status llmq_batch_paged_step(llmq_ctx *ctx, llmq_batch *bt, llmq_paged *p, 
   if (layers < m->n_layer || heads != m->n_head || dim != HS)
     return fail(ctx, LLMQ_ERR_INVALID, "the paged cache has not the model's layers, heads and head size");
   if (weights && weights_stride < max_len) return fail(ctx, LLMQ_ERR_INVALID, "weights_stride below max_len");
+  // before anything is enqueued: a refused step leaves the cache as it is
+  llmq_status st = paged_step_check(ctx, p, m->n_layer, table, table_stride, table_cols, B, max_len);
+  if (st != LLMQ_OK) return st;
   CK(cudaSetDevice(ctx->device));
   cudaStream_t s = ctx->stream;
   ctx->tc_used = true;  // the GEMMs' waits report through the context's error word
   embed_at_kernel<<<B, 256, 0, s>>>(m->head->view(), m->wpe(), bt->x, tokens, positions, 1024);
   CKL();
-  llmq_status st;
   for (int l = 0; l < m->n_layer; l++) {
     const llmq_weight *const *w = &m->mats[4 * l];
     if ((st = batch_linear(bt, w[0], bt->x, m->vec(l, 0), m->vec(l, 1), m->vec(l, 2), bt->qkv, B, EPI_BIAS, s)))

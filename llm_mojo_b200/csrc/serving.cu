@@ -72,6 +72,10 @@ llmq_status paged_check(llmq_ctx *ctx, const llmq_paged *p, int layer0, int n_la
   return LLMQ_OK;
 }
 
+llmq_status max_len_check(llmq_ctx *ctx, int max_len) {
+  return max_len > 0 && max_len <= 1 << 30 ? LLMQ_OK : fail(ctx, LLMQ_ERR_INVALID, "bad max_len");
+}
+
 // A launch that may begin while the kernel before it on the stream ends; its
 // own first step waits for that kernel (griddepcontrol.wait).
 template <typename... P, typename... A>
@@ -195,6 +199,12 @@ llmq_status paged_shape_check(llmq_ctx *ctx, int kind, int n_layer, int n_pages,
 
 }  // namespace
 
+llmq_status llmq::paged_step_check(llmq_ctx *ctx, const llmq_paged *p, int n_layers, const int *table,
+                                   long long table_stride, int table_cols, int n_seqs, int max_len) {
+  const llmq_status st = paged_check(ctx, p, 0, n_layers, table, table_stride, table_cols, n_seqs);
+  return st != LLMQ_OK ? st : max_len_check(ctx, max_len);
+}
+
 extern "C" {
 
 llmq_status llmq_paged_create_in(llmq_ctx *ctx, int kind, int n_layer, int n_pages, int page_size, int n_kv_head,
@@ -307,7 +317,7 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   if (n_head <= 0 || n_head % p->v.n_kv_head) return fail(ctx, LLMQ_ERR_INVALID, "n_head must be a multiple of n_kv_head");
   const long long C = (long long)n_head * p->v.head_dim;
   if (q_stride < 0 || (n_seqs > 1 && out_stride < C)) return fail(ctx, LLMQ_ERR_INVALID, "rows overlap");
-  if (max_len <= 0 || max_len > 1 << 30) return fail(ctx, LLMQ_ERR_INVALID, "bad max_len");
+  if ((st = max_len_check(ctx, max_len)) != LLMQ_OK) return st;
   if (weights && !weights_out) return fail(ctx, LLMQ_ERR_INVALID, "weights without weights_out");
   if (weights_out && weights_stride < max_len) return fail(ctx, LLMQ_ERR_INVALID, "weights_stride below max_len");
   CK(cudaSetDevice(ctx->device));
