@@ -179,19 +179,27 @@ class Batch:
         of the batch's own caches: tokens, position embeddings, cache slots
         and lengths (the new position among them) int32 CUDA tensors [B],
         logits [B, V]; weights [n_layer, B, n_head, >= max_len] accumulate the
-        softmax weights in place. Enqueued on the context's stream, which the
-        tensors' work must be on too (Context.use_torch_stream)."""
-        B = tokens.shape[0]
-        for t in (tokens, positions, slots, lens, logits):
-            assert t.is_cuda and t.is_contiguous() and t.shape[0] == B
-        assert logits.shape[1] == self.model.V and table.shape[0] == B and table.stride(1) == 1
-        w, stride = None, 0
+        softmax weights in place. Checked and ordered with torch's current
+        stream as the operators of serving are."""
+        from .serving import F32, I32, _call, _check, _shape
+
+        ctx, B = self.model.ctx, tokens.shape[0]
+        ptr = []
+        for name, t in (("tokens", tokens), ("positions", positions), ("slots", slots), ("lens", lens)):
+            ptr.append(_check(ctx, name, t, I32, 1))
+            _shape(name, t, (B,))
+        tp, lp = _check(ctx, "table", table, I32, 2), _check(ctx, "logits", logits, F32, 2, 2)
+        if table.shape[0] != B:
+            raise ValueError("table must have a row per sequence")
+        _shape("logits", logits, (B, self.model.V))
+        wp, stride = None, 0
         if weights is not None:
-            assert weights.is_contiguous() and weights.shape[1] == B and weights.shape[3] >= max_len
-            w, stride = weights.data_ptr(), weights.shape[3]
-        check(lib().llmq_batch_paged_step(self.model.ctx.h, self.h, cache.h, B, tokens.data_ptr(), positions.data_ptr(),
-                                          slots.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1],
-                                          lens.data_ptr(), max_len, w, stride, logits.data_ptr()), self.model.ctx.h)
+            wp, stride = _check(ctx, "weights", weights, F32, 4, 4), weights.shape[3]
+            rows = (self.model.n_layer, B, cache.n_kv_head)
+            if weights.shape[:3] != rows or stride < max_len:
+                raise ValueError(f"weights must be {[*rows]} rows of at least {max_len}, not {tuple(weights.shape)}")
+        _call(ctx, lib().llmq_batch_paged_step, self.h, cache.h, B, *ptr[:3], tp, table.stride(0), table.shape[1],
+              ptr[3], max_len, wp, stride, lp)
 
     def free(self):
         if getattr(self, "h", None):

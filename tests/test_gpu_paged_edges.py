@@ -53,3 +53,55 @@ def test_refused_step_changes_nothing(torch, model, bad):
     assert torch.all(c.k == 5.0) and torch.all(c.v == 5.0) and torch.count_nonzero(logits) == 0
     c.free()
     bt.free()
+
+
+def test_step_checks_its_tensors(torch, model):
+    """Types, shapes, strides and devices that the step would misread, and
+    weights that it would write past the end of, are refused."""
+    from llm_mojo_b200.model import Batch
+    from llm_mojo_b200.serving import PagedKVCache
+
+    bt = Batch(model, 2, 1)
+    c = PagedKVCache(model.ctx, "int8", 2, 2, 16, 12, 64)
+    zero, table, logits = i32(torch, [0, 0]), i32(torch, [[0], [1]]), torch.zeros(2, 50257, device="cuda")
+    wide = torch.zeros(2, 50260, device="cuda")
+    w = torch.zeros(2, 2, 12, 4, device="cuda")
+    ok = dict(tokens=zero, positions=zero, slots=zero, table=table, lens=zero + 1, max_len=4, logits=logits, weights=w)
+    for bad in (dict(tokens=zero.long()), dict(positions=zero.float()), dict(slots=zero[:1]), dict(lens=zero.long()),
+                dict(lens=zero.cpu()), dict(table=table.long()), dict(table=table[:1]), dict(table=table[0]),
+                dict(logits=logits.double()), dict(logits=logits[:, 1:]), dict(logits=wide[:, :50257]),
+                dict(weights=w[:1]), dict(weights=w[:, :1]), dict(weights=w[:, :, :11]), dict(weights=w[..., :3]),
+                dict(weights=w.double()), dict(weights=w.transpose(2, 3).contiguous().transpose(2, 3))):
+        with pytest.raises(ValueError):
+            bt.paged_step(c, **dict(ok, **bad))
+    bt.paged_step(c, **ok)
+    c.free()
+    bt.free()
+
+
+def test_step_is_ordered_with_the_current_stream(torch, model):
+    """On a context with a stream of its own the step takes what torch's
+    current stream has written, and the caller reads what it wrote."""
+    from llm_mojo_b200.model import Batch
+    from llm_mojo_b200.serving import PagedKVCache
+
+    bt = Batch(model, 1, 1)
+    c = PagedKVCache(model.ctx, "f32", 2, 1, 16, 12, 64)
+    assert not model.ctx.on_torch_stream()
+    zero, table = i32(torch, [0]), i32(torch, [[0]])
+    want = torch.zeros(1, 50257, device="cuda")
+    bt.paged_step(c, i32(torch, [777]), zero, zero, table, zero + 1, 1, want)
+    big = torch.randn(8192, 8192, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        tok, logits = zero.clone(), torch.zeros(1, 50257, device="cuda")
+        for _ in range(30):
+            big @ big
+        tok.fill_(777)
+        bt.paged_step(c, tok, zero, zero, table, zero + 1, 1, logits)
+        got = logits.clone()
+    side.synchronize()
+    assert torch.equal(got, want)
+    c.free()
+    bt.free()
