@@ -38,15 +38,20 @@ class PagedGenerator:
     """Generates for up to max_seqs sequences at once with a GPT-2 `model`.
 
     kind: the cache ('int8', 'bf16' or 'f32'). limit: a sequence's cache is
-    cut when it holds this many positions (None: never), to `budget`
-    positions, of which the first `sinks` and the last `recent` always stay.
+    cut when it holds this many positions (None: never; max_len at most), to
+    `budget` positions, of which the first `sinks` and the last `recent`
+    always stay.
     Memory for cache positions is then max_seqs * limit, and budget more
     while a sequence is cut, whatever the texts' lengths."""
 
     def __init__(self, model: Model, max_seqs: int, kind: str = "int8", page_size: int = 16, max_len: int = 1024,
                  limit: int | None = None, budget: int | None = None, sinks: int = 4, recent: int = 32):
-        if limit is not None and not 0 < (budget or 0) < limit:
-            raise ValueError("a limit needs a positive budget below it")
+        if limit is not None and not 0 < (budget or 0) < min(limit, max_len):
+            raise ValueError("a limit needs a positive budget below it and below max_len")
+        if limit is not None and (min(sinks, recent) < 0 or sinks + recent > budget):
+            raise ValueError("sinks and recent must fit in the budget")
+        if min(max_seqs, page_size, max_len) <= 0:
+            raise ValueError("max_seqs, page_size and max_len must be positive")
         self.model, self.max_seqs, self.page_size = model, max_seqs, page_size
         self.limit, self.budget, self.sinks, self.recent = limit, budget, sinks, recent
         self.cap = min(max_len, limit or max_len)  # positions that a sequence's cache may hold
@@ -67,6 +72,10 @@ class PagedGenerator:
         there is none), else a draw of sample."""
         if not 0 < len(prompts) <= self.max_seqs or any(len(p) == 0 for p in prompts):
             raise ValueError(f"between 1 and {self.max_seqs} prompts, none empty")
+        if any(not 0 <= t < self.model.V for p in prompts for t in p):
+            raise ValueError(f"token ids must be in [0, {self.model.V})")
+        if steps < 0:
+            raise ValueError("steps must not be negative")
         with self.model.ctx.torch_stream():
             return self._generate(prompts, steps, repetition, presence, frequency, bias, allowed, temperature, top_k, seed)
 

@@ -105,3 +105,23 @@ def test_step_is_ordered_with_the_current_stream(torch, model):
     assert torch.equal(got, want)
     c.free()
     bt.free()
+
+
+def test_generator_refuses_what_it_cannot_run(torch, model):
+    """When it is made, not at the first cut."""
+    from llm_mojo_b200.paged_generate import PagedGenerator
+
+    for bad in (dict(max_len=64, limit=100, budget=70), dict(max_len=64, limit=100, budget=64),
+                dict(limit=32, budget=16), dict(limit=32, budget=16, recent=10, sinks=7), dict(limit=32, budget=32),
+                dict(limit=32), dict(limit=32, budget=16, recent=8, sinks=-1), dict(page_size=0), dict(max_len=0)):
+        with pytest.raises(ValueError):
+            PagedGenerator(model, 2, **bad)
+    gen = PagedGenerator(model, 1, max_len=40, limit=100, budget=39, recent=30, sinks=9)
+    for prompt in ([-1], [5, 50257]):
+        with pytest.raises(ValueError):
+            gen.generate([prompt], 2)
+    with pytest.raises(ValueError):
+        gen.generate([[1]], -1)
+    assert gen.generate([[1]], 0) == [[]]
+    assert len(gen.generate([[1]], 60)[0]) == 60  # cut at 40, 20 times
+    gen.free()
