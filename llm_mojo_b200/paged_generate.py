@@ -69,7 +69,9 @@ class PagedGenerator:
         allowed(step, texts) -> bool CPU tensor [n, V], or None, is a
         grammar's say on each step; where it leaves nothing, and at
         temperature 0, the token is process_logits's argmax (EOT 50256 if
-        there is none), else a draw of sample."""
+        there is none), else a draw of sample. Prompt b's draws, one per token
+        of its answer, come from a generator of its own, of seed + b: what the
+        other prompts are does not change them."""
         if not 0 < len(prompts) <= self.max_seqs or any(len(p) == 0 for p in prompts):
             raise ValueError(f"between 1 and {self.max_seqs} prompts, none empty")
         if any(not 0 <= t < self.model.V for p in prompts for t in p):
@@ -108,26 +110,35 @@ class PagedGenerator:
             rules.bias = (torch.arange(B + 1, dtype=torch.int32, device=dev) * len(ids),
                           torch.tensor(ids * B, dtype=torch.int32, device=dev),
                           torch.tensor([bias[i] for i in ids] * B, device=dev))
-        rng = kernels.Rng(seed)
+        rngs = [kernels.Rng(seed + b) for b in range(B)] if temperature > 0 else []
         logits = torch.empty(B, V, device=dev)
         held = [0] * B  # positions in each cache
         texts = [list(p) for p in prompts]
+        ends = [len(p) + steps - 1 for p in prompts]  # the step after a text's last
         for at in range(total - 1):
-            # sequences whose text is done go on at their last position; their results are not used
+            # a text that is done stores nothing, attends to nothing and gives its pages back
+            live = [b for b in range(B) if at < ends[b]]
+            for b in range(B):
+                if at >= ends[b] and pages[b]:
+                    pool.give(pages[b])
+                    pages[b] = []
+                    table[b] = -1
             if self.limit:
-                full = [b for b in range(B) if held[b] >= self.cap]
+                full = [b for b in live if held[b] >= self.cap]
                 if full:
                     self._cut(full, held, pages, table, weights, pool)
-            for b in range(B):
+            slots = [-1] * B
+            for b in live:
                 if held[b] % ps == 0:
                     pages[b] += pool.take(1)
                     table[b, held[b] // ps] = pages[b][-1]
-            slots = torch.tensor(held, dtype=torch.int32, device=dev)
-            held = [h + 1 for h in held]
+                slots[b] = held[b]
+                held[b] += 1
+            slots = torch.tensor(slots, dtype=torch.int32, device=dev)
             lens = slots + 1
             pos = torch.full((B,), at, dtype=torch.int32, device=dev)
-            self.batch.paged_step(self.cache, history[:, at].contiguous(), pos, slots, table, lens, max(held), logits,
-                                  weights)
+            self.batch.paged_step(self.cache, history[:, at].contiguous(), pos, slots, table, lens,
+                                  max(held[b] for b in live), logits, weights)
             rules.n_ids.fill_(at + 1)
             rules.mask = None
             if allowed is not None:
@@ -136,13 +147,13 @@ class PagedGenerator:
             out, top = process_logits(self.model.ctx, logits, rules)
             nxt = torch.where(top < 0, 50256, top)
             if temperature > 0:
-                for b in range(B):
-                    if int(top[b]) >= 0:
-                        kernels.sample(self.model.ctx, out[b], temperature, top_k, rng, nxt[b:b + 1])
+                for b in live:
+                    if len(prompts[b]) <= at + 1 and int(top[b]) >= 0:
+                        kernels.sample(self.model.ctx, out[b], temperature, top_k, rngs[b], nxt[b:b + 1])
             # inside a prompt its own next token stands
             history[:, at + 1] = torch.where(at + 1 < n_prompt, history[:, at + 1], nxt)
             if allowed is not None:
-                for b in range(B):
+                for b in live:
                     if len(prompts[b]) <= at + 1:
                         texts[b].append(int(history[b, at + 1]))
         done = history.cpu()

@@ -125,3 +125,49 @@ def test_generator_refuses_what_it_cannot_run(torch, model):
     assert gen.generate([[1]], 0) == [[]]
     assert len(gen.generate([[1]], 60)[0]) == 60  # cut at 40, 20 times
     gen.free()
+
+
+def test_neighbours_do_not_change_a_sampled_text(torch, model):
+    from llm_mojo_b200.paged_generate import PagedGenerator
+
+    gen = PagedGenerator(model, 3, max_len=64)
+    prompts = [[5, 6], list(range(100, 120)), [7]]
+    all_three = gen.generate(prompts, 8, temperature=0.9)
+    assert gen.generate(prompts[:1], 8, temperature=0.9) == all_three[:1]
+    assert gen.generate(prompts[:2], 8, temperature=0.9) == all_three[:2]
+    assert gen.generate([[1] * 30, *prompts[1:]], 8, temperature=0.9)[1:] == all_three[1:]
+    assert gen.generate([[1], [2], prompts[0]], 8, temperature=0.9, seed=1335)[2] == all_three[0]
+    assert gen.generate(prompts, 8, temperature=0.9, seed=1) != all_three
+    gen.free()
+
+
+@pytest.mark.parametrize("bounded", [False, True])
+def test_a_text_that_is_done_holds_nothing(torch, model, monkeypatch, bounded):
+    """It takes no pages beyond its own, gives them back, grows no further for
+    `allowed`, and its end changes nothing for the others."""
+    from llm_mojo_b200 import paged_generate
+
+    taken, pools = [], []
+
+    class Pool(paged_generate.PagePool):
+        def __init__(self, n):
+            super().__init__(n)
+            pools.append(self)
+
+        def take(self, n):
+            taken.append(n)
+            return super().take(n)
+
+    monkeypatch.setattr(paged_generate, "PagePool", Pool)
+    kw = dict(limit=24, budget=12, sinks=2, recent=4) if bounded else dict(max_len=64)
+    gen = paged_generate.PagedGenerator(model, 2, page_size=8, **kw)
+    prompts = [[1], list(range(40))]
+    seen = []
+    out = gen.generate(prompts, 5, allowed=lambda at, texts: seen.append([len(t) for t in texts]))
+    assert [max(x) for x in zip(*seen)] == [6, 44]  # the whole of the shorter, the longer before its last token
+    if not bounded:
+        assert sum(taken) == -(-5 // 8) + -(-44 // 8)
+    assert len(pools[0].free) == gen.cache.n_pages - (3 if bounded else 6)  # the longer's last 20 positions, or all 44
+    for b in range(2):
+        assert gen.generate([prompts[b]], 5) == [out[b]]
+    gen.free()
