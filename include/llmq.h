@@ -297,7 +297,8 @@ llmq_status llmq_score_rows(llmq_ctx *ctx, const float *logits_dev, const float 
 /* No counterpart in the reference, which decodes one sequence at a time
  * (generate, gpt2t.mojo:942-980). State for the greedy decode of up to
  * max_seqs independent sequences with prompts of up to max_prompt tokens,
- * each with its own QuantKV[8] cache of the model's max_t positions. The
+ * each with its own QuantKV[8] cache of the model's max_t positions; with
+ * max_prompt 0, for llmq_batch_paged_step alone, without those caches. The
  * model must use the QuantKV[8] cache. */
 typedef struct llmq_batch llmq_batch;
 llmq_status llmq_batch_create(llmq_ctx *ctx, llmq_model *m, int max_seqs, int max_prompt, llmq_batch **out);

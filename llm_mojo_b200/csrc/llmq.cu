@@ -2599,7 +2599,7 @@ extern "C" {
 llmq_status llmq_batch_create(llmq_ctx *ctx, llmq_model *m, int max_seqs, int max_prompt, llmq_batch **out) {
   if (m && m->float_only)
     return fail(ctx, LLMQ_ERR_UNSUPPORTED, "batched decode runs the A16 formats");
-  if (!ctx || !m || !out || max_seqs <= 0 || max_prompt <= 0 || max_prompt > m->max_t)
+  if (!ctx || !m || !out || max_seqs <= 0 || max_prompt < 0 || max_prompt > m->max_t)
     return fail(ctx, LLMQ_ERR_INVALID, "bad batch arguments");
   if (m->kv->kind != LLMQ_KV_QUANT8) return fail(ctx, LLMQ_ERR_UNSUPPORTED, "batched decode takes the QuantKV[8] cache");
   *out = nullptr;
@@ -2610,7 +2610,9 @@ llmq_status llmq_batch_create(llmq_ctx *ctx, llmq_model *m, int max_seqs, int ma
   bt->max_seqs = max_seqs;
   bt->max_prompt = max_prompt;
   const int C = m->C, HS = C / m->n_head;
-  const size_t seq = (size_t)m->n_layer * m->max_t * m->n_head * HS, rows = (size_t)max_seqs * max_prompt;
+  const size_t seq = (size_t)m->n_layer * m->max_t * m->n_head * HS, rows = (size_t)max_seqs * std::max(1, max_prompt);
+  // a batch without prompts runs paged steps alone and has no caches of its own
+  const size_t cached = max_prompt > 0 ? seq * max_seqs : 0;
   KV8View &v = bt->kv;
   v.n_layer = m->n_layer;
   v.max_t = m->max_t;
@@ -2620,10 +2622,17 @@ llmq_status llmq_batch_create(llmq_ctx *ctx, llmq_model *m, int max_seqs, int ma
   int maxu = 0;
   for (const llmq_weight *w : m->mats) maxu = std::max(maxu, w->cols / w->group);
   maxu = std::max(maxu, m->head->cols / m->head->group);
-  cudaError_t e = cudaMalloc(&v.k, seq * max_seqs);
-  if (e == cudaSuccess) e = cudaMalloc(&v.v, seq * max_seqs);
-  if (e == cudaSuccess) e = cudaMalloc(&v.ks, seq / HS * max_seqs * 4);
-  if (e == cudaSuccess) e = cudaMalloc(&v.vs, seq / HS * max_seqs * 4);
+  cudaError_t e = cudaSuccess;
+  if (cached) {
+    e = cudaMalloc(&v.k, cached);
+    if (e == cudaSuccess) e = cudaMalloc(&v.v, cached);
+    if (e == cudaSuccess) e = cudaMalloc(&v.ks, cached / HS * 4);
+    if (e == cudaSuccess) e = cudaMalloc(&v.vs, cached / HS * 4);
+    if (e == cudaSuccess) e = cudaMemset(v.k, 0, cached);
+    if (e == cudaSuccess) e = cudaMemset(v.v, 0, cached);
+    if (e == cudaSuccess) e = cudaMemset(v.ks, 0, cached / HS * 4);
+    if (e == cudaSuccess) e = cudaMemset(v.vs, 0, cached / HS * 4);
+  }
   if (e == cudaSuccess) e = cudaMalloc(&bt->x, rows * C * 4);
   if (e == cudaSuccess) e = cudaMalloc(&bt->xn, rows * C * 4);
   if (e == cudaSuccess) e = cudaMalloc(&bt->qkv, rows * 3 * C * 4);
@@ -2642,10 +2651,6 @@ llmq_status llmq_batch_create(llmq_ctx *ctx, llmq_model *m, int max_seqs, int ma
   const size_t nparts = std::max((size_t)(m->V + BG_ROWS - 1) / BG_ROWS, (size_t)4 * ((m->V + TC_M - 1) / TC_M));
   if (e == cudaSuccess) e = cudaMalloc(&bt->part_val, (size_t)max_seqs * nparts * 4);
   if (e == cudaSuccess) e = cudaMalloc(&bt->part_idx, (size_t)max_seqs * nparts * 4);
-  if (e == cudaSuccess) e = cudaMemset(v.k, 0, seq * max_seqs);
-  if (e == cudaSuccess) e = cudaMemset(v.v, 0, seq * max_seqs);
-  if (e == cudaSuccess) e = cudaMemset(v.ks, 0, seq / HS * max_seqs * 4);
-  if (e == cudaSuccess) e = cudaMemset(v.vs, 0, seq / HS * max_seqs * 4);
   if (e == cudaSuccess) e = cudaMallocHost(&bt->ids_host, (size_t)max_seqs * m->max_t * 4);
   if (e == cudaSuccess) e = cudaMallocHost(&bt->prompt_host, rows * 4);
   const int tcl_seqs = (max_seqs + TCL_TT - 1) / TCL_TT * TCL_TT;

@@ -142,7 +142,8 @@ class Batch:
     """Greedy decode of independent sequences together (no counterpart in
     the reference, which decodes one at a time): up to max_seqs sequences
     with prompts of up to max_prompt tokens, each with its own QuantKV[8]
-    cache. Each sequence's ids equal Model.generate on it alone."""
+    cache. Each sequence's ids equal Model.generate on it alone. With
+    max_prompt 0 there are no such caches: the batch runs paged_step alone."""
 
     def __init__(self, model: Model, max_seqs: int, max_prompt: int):
         self.model, self.max_seqs, self.max_prompt = model, max_seqs, max_prompt

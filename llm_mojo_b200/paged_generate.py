@@ -56,7 +56,7 @@ class PagedGenerator:
         self.limit, self.budget, self.sinks, self.recent = limit, budget, sinks, recent
         self.cap = min(max_len, limit or max_len)  # positions that a sequence's cache may hold
         self.cols = -(-self.cap // page_size)
-        self.batch = Batch(model, max_seqs, 1)
+        self.batch = Batch(model, max_seqs, 0)
         n_pages = max_seqs * self.cols + (-(-budget // page_size) * max_seqs if limit else 0)
         n_head = 12
         self.cache = PagedKVCache(model.ctx, kind, model.n_layer, n_pages, page_size, n_head, 64)

@@ -171,3 +171,35 @@ def test_a_text_that_is_done_holds_nothing(torch, model, monkeypatch, bounded):
     for b in range(2):
         assert gen.generate([prompts[b]], 5) == [out[b]]
     gen.free()
+
+
+def test_the_pool_is_the_only_cache(torch, model):
+    """A generator's memory for cache positions is its pool; its batch has no
+    contiguous caches beside it, and generates nothing by itself."""
+    from llm_mojo_b200._lib import ERR_INVALID, LlmqError
+    from llm_mojo_b200.model import Batch
+    from llm_mojo_b200.paged_generate import PagedGenerator
+
+    def used(make):
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        x = make()
+        torch.cuda.synchronize()
+        return x, before - torch.cuda.mem_get_info()[0]
+
+    Batch(model, 1, 1).free()  # the kernels' own memory
+    n, position = 256, 2 * 12 * 2 * (64 + 4)  # layers, heads, keys and values with their scales
+    whole, with_caches = used(lambda: Batch(model, n, 1))
+    whole.free()
+    torch.cuda.empty_cache()
+    gen, got = used(lambda: PagedGenerator(model, n, max_len=16))
+    # the pool holds 16 positions a sequence, the caches the model's 128; 2 MB a buffer at most
+    assert got <= with_caches + n * (16 - 128) * position + (8 << 20)
+    with pytest.raises(LlmqError) as e:
+        gen.batch.generate([[1]], 1)
+    assert e.value.status == ERR_INVALID
+    assert len(gen.generate([[1]], 3)[0]) == 3
+    gen.free()
+    for bad in (-1, 129):
+        with pytest.raises(LlmqError):
+            Batch(model, 1, bad)
