@@ -307,7 +307,8 @@ llmq_status llmq_batch_free(llmq_batch *b);
  * int4-g32 rows and the per-channel int8 head; dot_row_i16 per sequence,
  * tensor.mojo:522-566): AUTO (the lane-mode tcgen05 GEMM from 16 sequences
  * on), CUDA_CORE (the dp2a batched GEMVs) or TCGEN05 (the GEMM for any
- * count). Results are identical; no counterpart in the reference, which
+ * count). Layers and heads of other formats run on the CUDA cores whatever
+ * the choice. Results are identical; no counterpart in the reference, which
  * decodes one sequence at a time. */
 #define LLMQ_BATCH_AUTO 0
 #define LLMQ_BATCH_CUDA_CORE 1

@@ -2284,13 +2284,16 @@ int fmt_code(const llmq_weight *w) { return fmt_of(w->view()); }
 constexpr int TCL_TT = 16;          // sequences per lane-mode GEMM tile
 constexpr int TCL_MIN_SEQS = 16;    // AUTO: the lane-mode GEMM from this many sequences
 
-// Whether batch_linear runs w for B sequences as the lane-mode tcgen05 GEMM:
-// BLOCKED int4 rows as a layer (its epilogue writes the outputs, with bias,
-// GELU and residual), per-channel int8 rows as the head (argmax candidates or
-// the plain logits).
+// Whether the lane-mode tcgen05 GEMM takes w in its place: BLOCKED int4 rows
+// as a layer (its epilogue writes the outputs, with bias, GELU and residual),
+// per-channel int8 rows as the head (argmax candidates or the plain logits).
+bool tcl_takes(const llmq_batch *bt, const llmq_weight *w) {
+  return (w == bt->m->head) == (w->bits == 8) && w->kind == WK_AFFINE && w->a16 && tcl_supported(w->view());
+}
+
+// Whether batch_linear runs w for B sequences as that GEMM.
 bool batch_uses_tcl(const llmq_batch *bt, const llmq_weight *w, int B) {
-  if ((w == bt->m->head) != (w->bits == 8)) return false;
-  if (!w->tcl_a || bt->kernel == LLMQ_BATCH_CUDA_CORE) return false;
+  if (!tcl_takes(bt, w) || bt->kernel == LLMQ_BATCH_CUDA_CORE) return false;
   return bt->kernel == LLMQ_BATCH_TCGEN05 || B >= TCL_MIN_SEQS;
 }
 
@@ -2365,8 +2368,8 @@ llmq_status batch_prepare_tcl(llmq_batch *bt) {
   std::vector<const llmq_weight *> ws(bt->m->mats.begin(), bt->m->mats.end());
   ws.push_back(bt->m->head);
   for (const llmq_weight *w : ws) {
+    if (w->tcl_a || !tcl_takes(bt, w)) continue;
     const WeightView v = w->view();
-    if (w->tcl_a || w->kind != WK_AFFINE || !w->a16 || !tcl_supported(v)) continue;
     const int nt = (v.rows + TC_M - 1) / TC_M, nkb = v.cols / TC_KB;
     CK(cudaMalloc(&w->tcl_a, (size_t)nt * nkb * TCT_A_BYTES));
     tcl_prep_a_kernel<<<dim3(nt, nkb), 256, 0, ctx->stream>>>(v, v.bits == 4 ? TCL_BLK4 : TCL_CH8, w->tcl_a);

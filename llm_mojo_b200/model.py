@@ -156,7 +156,9 @@ class Batch:
     def set_kernel(self, kind: str):
         """Which kernel runs the batched one-token matmuls: 'auto' (the
         lane-mode tcgen05 GEMM from 16 sequences on), 'cuda_core' (dp2a
-        batched GEMVs) or 'tcgen05' (the GEMM at any count)."""
+        batched GEMVs) or 'tcgen05' (the GEMM at any count). The GEMM takes
+        BLOCKED int4 layers and the per-channel int8 head; other formats run
+        on the CUDA cores whatever the choice."""
         check(lib().llmq_batch_set_kernel(self.h, self.KERNELS[kind]), self.model.ctx.h)
 
     def generate(self, prompts, steps: int) -> np.ndarray:

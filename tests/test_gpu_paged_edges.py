@@ -203,3 +203,37 @@ def test_the_pool_is_the_only_cache(torch, model):
     for bad in (-1, 129):
         with pytest.raises(LlmqError):
             Batch(model, 1, bad)
+
+
+@pytest.mark.parametrize("dtype,head", [("int8-ch-a16", "int8"), ("int4-g32-a16", "same"), ("int4-g32-a16", "int8")])
+def test_tiles_are_built_where_they_are_read(torch, dtype, head):
+    """A model's first batch builds the lane-mode GEMM's copies of the weights
+    that it takes: BLOCKED int4 layers and the per-channel int8 head, rows to
+    a multiple of 128."""
+    from llm_mojo_b200 import synth
+    from llm_mojo_b200.model import Batch, Model
+    from llm_mojo_b200.tensor import Context
+
+    def used(make):
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        x = make()
+        torch.cuda.synchronize()
+        return x, before - torch.cuda.mem_get_info()[0]
+
+    ctx = Context(0)
+    layers = 4
+    tensors = synth.gpt2_random_init(0, n_layer=layers)
+    first = Model(ctx, tensors, n_layer=layers, max_t=32)
+    Batch(first, 16, 1).free()  # the kernels' own memory
+    first.free()
+    m = Model(ctx, tensors, dtype, head, n_layer=layers, max_t=32)
+    a, first = used(lambda: Batch(m, 16, 1))
+    b, second = used(lambda: Batch(m, 16, 1))
+    copies = [n * 768 * 768 for n in (3, 1, 4, 4)] * layers * (dtype[:4] == "int4") + [50304 * 768] * (head == "int8")
+    page = 2 << 20
+    assert sum(copies) <= first - second <= sum(-(-x // page) * page for x in copies), (first, second)
+    a.free()
+    b.free()
+    m.free()
+    ctx.close()
