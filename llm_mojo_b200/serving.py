@@ -17,7 +17,7 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import KV_BF16, KV_F32, KV_QUANT8, OK, check, lib
-from .tensor import CUDA_STREAM_LEGACY, Context, torch_stream
+from .tensor import Context
 
 F32, I32 = torch.float32, torch.int32
 
@@ -43,6 +43,22 @@ def _rows_contiguous(t, inner: int) -> bool:
     return True
 
 
+def _row_stride(name: str, t) -> int:
+    """The distance of t's rows [..., row] from one another, which must be the
+    same over all leading dimensions; a dimension of one has no say."""
+    if t.is_contiguous():
+        return t.shape[-1]
+    step, rows = None, 1
+    for n, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n != 1:
+            if step is None:
+                step = stride
+            elif stride != step * rows:
+                raise ValueError(f"{name} must have evenly spaced rows")
+        rows *= n
+    return t.shape[-1] if step is None else step
+
+
 def _shape(name: str, t, want):
     if t.shape != want:
         raise ValueError(f"{name} must be {tuple(want)}, not {tuple(t.shape)}")
@@ -50,7 +66,7 @@ def _shape(name: str, t, want):
 
 def _call(ctx: Context, fn, *args):
     """fn(ctx, *args) in order with torch's current stream."""
-    if ctx.stream == (torch_stream(ctx.device) or CUDA_STREAM_LEGACY):
+    if ctx.on_torch_stream():
         status = fn(ctx.h, *args)
         if status != OK:
             check(status, ctx.h)
@@ -147,17 +163,13 @@ class PagedKVCache:
                 raise ValueError("weights without weights_out")
         else:
             wop = _check(ctx, "weights_out", weights_out, F32, 3)
-            rows = weights_out.stride()
-            stride = rows[1]
-            if n > 1 and rows[0] != stride * self.n_kv_head:
-                raise ValueError("weights_out must have evenly spaced rows")
+            stride = _row_stride("weights_out", weights_out)
             shape = weights_out.shape
             if shape[0] != n or shape[1] != self.n_kv_head or shape[2] < max_len:
                 raise ValueError(f"weights_out must be [{n}, {self.n_kv_head}, >= {max_len}]")
             if weights is not None:
                 wp = _check(ctx, "weights", weights, F32, 3)
-                if weights.shape != shape or weights.stride()[1:] != rows[1:] or (
-                        n > 1 and weights.stride(0) != rows[0]):
+                if weights.shape != shape or _row_stride("weights", weights) != stride:
                     raise ValueError("weights must have the shape and strides of weights_out")
         _call(ctx, self._attend, self.h, layer, qp, q.stride(0), op, out.stride(0), n, n_head, tp,
               table.stride(0), table.shape[1], lp, max_len, self.scale if scale is None else scale, wp, wop, stride)
@@ -183,10 +195,7 @@ class PagedKVCache:
         wp = _check(ctx, "weights", weights, F32, 4)
         if tuple(weights.shape[:3]) != (n_layers, n, self.n_kv_head) or weights.shape[3] < max_len:
             raise ValueError(f"weights must be [{n_layers}, {n}, {self.n_kv_head}, >= {max_len}]")
-        ws = weights.stride(2)
-        if (n > 1 and weights.stride(1) != ws * self.n_kv_head) or (
-                n_layers > 1 and weights.stride(0) != ws * self.n_kv_head * n):
-            raise ValueError("weights must have evenly spaced rows")
+        ws = _row_stride("weights", weights)
         if budget <= 0:
             raise ValueError("budget must be positive")
         rows = (n_layers, n, self.n_kv_head, budget)

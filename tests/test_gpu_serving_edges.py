@@ -252,3 +252,42 @@ def test_evict_refuses_positions_without_a_page(torch, ctx, kind, budget):
             tol = 2.0 ** -23 * (32 * smax + 4 * n ** 0.5 + 16) * float(vb.abs().max())
             assert float((out[b, h].double() - p @ vb).abs().max()) <= tol
     c.free()
+
+
+# ---- views -------------------------------------------------------------------
+
+
+def test_weights_of_one_head_or_sequence(torch, ctx):
+    """The stride of a dimension of one says nothing: rows of a wider buffer
+    with such a dimension put in are taken; rows that are not evenly spaced,
+    or overlap, are not."""
+    from llm_mojo_b200._lib import LlmqError
+
+    c, k, v = pool(torch, ctx, "bf16", 8, 16, 1, 64, 3)
+    q = torch.randn(2, 3, 64, device="cuda")
+    table = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([40, 33], dtype=torch.int32, device="cuda")
+    want = torch.zeros(2, 1, 48, device="cuda")
+    c.attend(0, q, table, lens, 48, weights_out=want)
+    wide = torch.zeros(2, 60, device="cuda")
+    rows = wide[:, :48].unsqueeze(1)
+    assert rows.stride() == (60, 48, 1)
+    c.attend(0, q, table, lens, 48, weights=rows, weights_out=rows)
+    assert torch.equal(rows, want) and torch.count_nonzero(wide[:, 48:]) == 0
+    one = torch.zeros(48, device="cuda").as_strided((1, 1, 48), (5, 7, 1))
+    c.attend(0, q[:1], table[:1], lens[:1], 48, weights_out=one)
+    assert torch.equal(one, want[:1])
+    dst = torch.tensor([[6], [7]], dtype=torch.int32, device="cuda")
+    kept, w, n = c.evict(table, lens, 48, want[None], 16, dst)
+    kept2, w2, n2 = c.evict(table, lens, 48, rows[None], 16, dst)
+    assert torch.equal(kept, kept2) and torch.equal(w, w2) and torch.equal(n, n2)
+    with pytest.raises(LlmqError):
+        c.attend(0, q, table, lens, 48, weights_out=torch.zeros(1, 1, 48, device="cuda").expand(2, 1, 48))
+    two, _, _ = pool(torch, ctx, "bf16", 8, 16, 2, 64, 3)
+    uneven = torch.zeros(2, 3, 48, device="cuda")[:, :2]
+    with pytest.raises(ValueError):
+        two.attend(0, torch.randn(2, 2, 64, device="cuda"), table, lens, 48, weights_out=uneven)
+    with pytest.raises(ValueError):
+        two.evict(table, lens, 48, uneven[None], 16, dst)
+    c.free()
+    two.free()
