@@ -291,3 +291,29 @@ def test_weights_of_one_head_or_sequence(torch, ctx):
         two.evict(table, lens, 48, uneven[None], 16, dst)
     c.free()
     two.free()
+
+
+# ---- logits ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n,H", [(5, 700), (6, 700), (12, 5000), (30, 1), (256, 300)])
+def test_rules_of_full_batches(torch, ctx, n, H):
+    """1024, 2048 and 4096 logits a tile, the argmax by tickets (5 rows) and
+    by a second launch (from 6 on), each rule at work, infinities among
+    the logits, in place too."""
+    from llm_mojo_b200.serving import process_logits
+
+    V = 50257
+    r = make_rules(V, n, H, n)
+    x = (np.random.default_rng(n).standard_normal((n, V)) * 3).astype(np.float32)
+    x[0, 40000], x[1, :: 7], x[-1, 5] = np.inf, np.float32(2.5), -np.inf
+    r["mask"][-1] = 0  # nothing is left
+    r["mask"][-2] = 0
+    r["mask"][-2, 50256 // 32] = 1 << (50256 % 32)  # the last token alone
+    want, best = rules_reference(x, **r)
+    assert best[-1] == -1 and best[-2] == 50256
+    logits = torch.from_numpy(x).cuda()
+    out, top = process_logits(ctx, logits, to_rules(torch, r))
+    assert np.array_equal(out.cpu().numpy(), want) and np.array_equal(top.cpu().numpy(), best)
+    process_logits(ctx, logits, to_rules(torch, r), out=logits, argmax=top.fill_(-9))
+    assert torch.equal(out, logits) and np.array_equal(top.cpu().numpy(), best)
