@@ -2,8 +2,8 @@
 // repeated tokens, biases and a mask of the allowed tokens.
 //
 // Each logit is read and written once, so memory bounds a call in the end:
-// 256 x 50257 without rules takes 20 us, 5.2 TB/s (a device-to-device copy of
-// the same rows through torch 34 us). With every rule 33 us, 3.2 TB/s: 830
+// 256 x 50257 without rules takes 20 us, 5.2 TB/s (torch.mul from the same
+// rows to others 16.6 us). With every rule 33 us, 3.2 TB/s: 830
 // instructions a warp per 512 logits, 440 of them without rules, fill 73% of
 // the issue slots, and CTAs wait at their barriers for the history. Tried and
 // slower: persistent CTAs with the next tile's loads ahead (66 us), counts

@@ -36,7 +36,7 @@
 // slots, without ldmatrix: L1 at 77% and 157 us.)
 //
 // mma.sync, not tcgen05: a new token brings 8 columns to a row of the cache,
-// and the tensor pipe is 18-29% busy while memory is the limit; tcgen05 would
+// and the tensor pipe is 15-18% busy while memory is the limit; tcgen05 would
 // want the rows as 16-bit tiles in shared memory, so int8 codes converted,
 // written back and read again.
 //
@@ -44,10 +44,11 @@
 // long calls, 8 sequences x <=32768 positions, 32 heads on 8 of 128, bfloat16:
 // 99 us, 5.3 TB/s (104 with the weights); one sequence x 131071, 12 heads of 64, int8: 48 us, 4.4
 // TB/s, of which about 9 us are the start and the join of the chunks (524288
-// positions: 164 us, 5.2 TB/s), and 190 instructions per 16 positions fill
-// half of the issue slots; latency and those instructions in batches of short
-// sequences, 256 x <=256, 12 heads of 64, int8: 18 us, 3.1 TB/s; the latency
-// of one CTA in the smallest, 1 x 200: 4.1 us.
+// positions: 164 us, 5.2 TB/s), and 246 instructions per 16 positions, start
+// and join among them, fill 57% of the issue slots; latency and those
+// instructions (61%) in batches of short sequences, 256 x <=256, 12 heads of
+// 64, int8: 18 us, 3.1 TB/s; the latency of one CTA in the smallest, 1 x 200:
+// 3.9 us.
 #pragma once
 
 #include "paged.cuh"

@@ -341,9 +341,15 @@ llmq_status llmq_paged_attend(llmq_ctx *ctx, const llmq_paged *p, int layer, con
   a.head_chunks = (G + a.unit_heads - 1) / a.unit_heads;
   const long long units = (long long)n_seqs * p->v.n_kv_head * a.head_chunks;
   // Fewer warps a CTA for many units of short sequences, whose prologues and
-  // joins then cost less than idle warps do (int8, 64 dimensions, us with 1 /
-  // 2 / 4 warps: 3072 units x <=100 positions 13 / 17 / 23, 1536 x <=256 18 /
-  // 14 / 16, 576 x <=256 12 / 11 / 8)
+  // joins then cost less than idle warps do. 64 dimensions, us with 1 / 2 / 4
+  // warps:
+  //                    int8 x <=256        x <=320             x <=384             bfloat16 x <=256    x <=320
+  //   3072 units       18.6/20.3/24.5      21.3/23.2/27.0      25.9/25.2/28.6      26.5/27.3/34.2      32.2/31.0/37.8
+  //   2448             20.3/17.2/20.8      24.1/19.5/23.0      26.1/21.6/24.0      19.9/22.4/27.6      24.7/25.6/30.7
+  //   1344             16.4/10.8/12.8      19.1/13.4/14.7      19.3/14.2/15.1      18.1/14.0/16.8      21.6/16.5/19.0
+  //   768              14.0/11.3/9.7       15.1/14.1/9.1       14.8/15.0/9.4       16.4/10.9/12.0      16.6/10.5/12.6
+  // (int8's 2448 units leave room for two one-warp chunks each, which have to
+  // be joined: there two warps would do better)
   int warps = units >= ctx->num_sms * 16 && a.max_len <= 256 ? 1 : units >= ctx->num_sms * 8 ? 2 : 4;
   AttendKernel *k;
   if ((st = attend_kernel(ctx, a, warps, &k)) != LLMQ_OK) return st;
